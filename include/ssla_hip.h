@@ -429,6 +429,118 @@ typedef struct SslaHipOevaDiff {
 int ssla_hip_oeva_diff(const char* path_a, const char* path_b, double tol_abs,
                        SslaHipOevaDiff* out);
 
+/* ---- sequence operators ------------------------------------------------
+ * No counterpart in the reference.  Its layers are gated linear recurrences
+ * h = sigmoid(g) h + v read out by q * h, per channel and per grid cell; these
+ * are the general forms for models around the drain: linear attention with a
+ * decay for each head over token sequences of any length (whole prompts and
+ * single tokens, with the state carried between calls) and group norm with
+ * an activation over channels-last data.
+ *
+ * All pointers are device pointers on the calling thread's current device.
+ * Every call only queues kernels on `stream` (hipStream_t or NULL): it
+ * allocates nothing, copies nothing to the host, waits for nothing and keeps
+ * nothing between calls, so it may be captured into a HIP graph.  A workspace
+ * belongs to one call (or captured graph) at a time. */
+#define SSLA_F32  0
+#define SSLA_BF16 1
+#define SSLA_F16  2
+
+#define SSLA_LINATTN_MAX_DIM 256
+
+/* With S (dk x dv, fp32) a head's state and g_t its log decay:
+ *     S_t = exp(g_t) S_{t-1} + k_t v_t^T,    out_t = scale q_t^T S_t
+ * q, k, v and out are rows of tokens: element (token, head, i) lies at
+ * token * stride[0] + head * stride[1] + i (strides in elements, >= 0; q's and
+ * k's head counts `qk_heads`, which divides `heads`: head h uses q and k of
+ * h / (heads / qk_heads)).  log_decay is fp32 at token * stride[0] + head *
+ * stride[1]; stride[0] = 0 gives one decay for each head.  Values below -65536
+ * count as -65536 (a decay of zero).
+ * Sums, decays and states are fp32 or wider; out is rounded once.
+ * An infinity or NaN in k or v reaches the outputs of its own token and those
+ * behind it in its sequence (and its head, and for v its column), which are
+ * then not finite; tokens before it and other sequences are unaffected.
+ *
+ * Sequences are packed: sequence s holds the tokens cu_seqlens[s] up to
+ * cu_seqlens[s + 1] (n_seqs + 1 values in device memory, rising from >= 0 to
+ * <= n_tokens; values outside are clamped, so no call reads or writes past
+ * n_tokens rows), or, with cu_seqlens NULL, tokens s * max_len up to
+ * (s + 1) * max_len, with n_tokens = n_seqs * max_len.  A sequence may be
+ * empty.  No sequence may hold more than max_len tokens: those past it are
+ * passed over.  Rows of out that belong to no sequence are left as they are.
+ *
+ * state_in (NULL: zeros) and state_out (NULL: not kept) are pools of states:
+ * sequence s reads and writes slot slots[s] (NULL: slot s), [heads][dk][dv]
+ * floats at slot * state_stride.  They may be the same memory, or must not
+ * overlap.  A sequence whose slot is negative or >= n_slots (a row that
+ * pads a batch) is passed over: its out rows are left as they are.  Two
+ * sequences of a call must not have the same slot (their states would
+ * race).  out must not overlap an input. */
+typedef struct SslaHipLinAttn {
+    int dtype;                 /* of q, k, v and out: SSLA_F32, _BF16, _F16 */
+    int heads, qk_heads;
+    int dk, dv;                /* 1 .. SSLA_LINATTN_MAX_DIM */
+    int n_seqs;
+    int max_len;
+    int n_slots;
+    long long n_tokens;
+    const void *q, *k, *v;
+    const float* log_decay;
+    void* out;
+    long long q_stride[2], k_stride[2], v_stride[2], decay_stride[2], out_stride[2];
+    const int* cu_seqlens;
+    const int* slots;
+    const float* state_in;
+    float* state_out;
+    long long state_stride;    /* floats, >= heads * dk * dv */
+    float scale;
+} SslaHipLinAttn;
+
+/* Bytes of workspace that ssla_hip_linattn needs for *d (0 where sequences
+ * are not cut; it depends on dtype, heads, dk, dv, n_seqs, max_len, n_tokens). */
+int ssla_hip_linattn_workspace(const SslaHipLinAttn* d, size_t* nbytes);
+/* Whole sequences, in chunks on the matrix cores.  `workspace` holds at
+ * least ssla_hip_linattn_workspace bytes, 16-byte aligned (NULL if 0). */
+int ssla_hip_linattn(const SslaHipLinAttn* d, void* workspace, size_t workspace_bytes,
+                     void* stream);
+/* One token of every sequence: row s of q, k, v, log_decay and out belongs
+ * to sequence s, whose state is read from state_in and written to state_out
+ * (both needed; usually the same pool).  cu_seqlens, max_len and n_tokens
+ * are not used. */
+int ssla_hip_linattn_step(const SslaHipLinAttn* d, void* stream);
+
+#define SSLA_ACT_NONE    0
+#define SSLA_ACT_SILU    1
+#define SSLA_ACT_SIGMOID 2
+#define SSLA_ACT_RELU    3
+
+/* Group norm over n items of `rows` rows of `channels` channels, channels
+ * innermost; mean and variance over the rows and the channels / groups
+ * neighbouring channels of a group (rows = 1: a norm of each token's heads):
+ *     y = (x - mean) / sqrt(var + eps) * weight_c + bias_c
+ *     out = act(y), or y * act(gate) where gate is set
+ * Element (item, row, c) of x lies at item * stride[0] + row * stride[1] + c
+ * (elements, >= 0), of gate and out likewise.  weight and bias (NULL: 1 and 0)
+ * have the type of x.  Moments are fp32, merged from exact differences (no
+ * difference of large sums), out is rounded once.  out may be x or gate itself,
+ * else it must not overlap an input.  A NaN or infinity reaches its own
+ * group of its own item only. */
+typedef struct SslaHipGroupNorm {
+    int dtype;
+    int n, rows, channels, groups, act;
+    const void *x, *gate, *weight, *bias;
+    void* out;
+    long long x_stride[2], gate_stride[2], out_stride[2];
+    float eps;
+} SslaHipGroupNorm;
+
+int ssla_hip_group_norm_workspace(const SslaHipGroupNorm* d, size_t* nbytes);
+int ssla_hip_group_norm(const SslaHipGroupNorm* d, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* sizeof SslaHipLinAttn, sizeof SslaHipGroupNorm into out[0..1] (cap >= 2). */
+int ssla_hip_ops_layout(long long* out, int cap);
+
 #ifdef __cplusplus
 }
 #endif

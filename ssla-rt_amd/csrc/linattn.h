@@ -1,0 +1,116 @@
+// linattn.h -- linear attention with a decay for each head: what the C ABI
+// (ops.cpp) hands to the kernels, and how work is cut into them.
+//
+//   S_t = exp(g_t) S_{t-1} + k_t v_t^T,     o_t = scale q_t^T S_t     (S: dk x dv)
+//
+// A workgroup runs one segment of one sequence for one head and one slice of
+// the dv columns, chunk by chunk with the state in registers (linattn16.h,
+// linattn32.h).  Sequences longer than a segment take three launches: the
+// segments' own states from zero (FULL = false), the states before each
+// segment (k_linattn_chain), then every segment from its state (FULL = true).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "ssla_hip.h"
+
+namespace ssla {
+
+constexpr int kLinAttnMaxDim = 256;      // dk, dv
+constexpr float kMinLogDecay = -65536.0f;
+
+struct LinAttnArgs {
+    const void *q, *k, *v;
+    void* out;
+    const float* g;                       // log decay
+    long long qt, qh, kt, kh, vt, vh, ot, oh, gt, gh;   // strides, elements: token, head
+    const int* cu;                        // first token of each sequence, or null
+    const int* slots;                     // state slot of each sequence, or null
+    const float* s_in;
+    float* s_out;
+    long long s_stride;                   // floats between slots
+    float* ws_state;                      // [segment][head][dk][dv] (more than one segment a sequence)
+    float* ws_decay;                      // [segment][head]
+    long long n_tokens;
+    int n_seqs, n_slots, max_len;
+    int heads, rep, dk, dv, slices;       // rep: heads sharing q and k
+    int seg_shift, n_segs;                // log2 of a segment's tokens; segments of the call
+    int vec_in, vec_out;                  // 16-byte loads of q, k, v; wide stores of out
+    float scale;
+};
+
+// Where a segment lies: sequence `seq`, tokens [t0, t1) of its `len`, which
+// begin at row `row`.  Segment slots of sequence s begin at
+// (cu[s] >> seg_shift) + s: as many as it can need whatever the lengths, so
+// the grid needs only the number of tokens and sequences.
+struct Segment {
+    long long row;
+    int seq, index, t0, t1, len;
+    bool ok;
+};
+
+#ifdef __HIP_DEVICE_COMPILE__
+__device__ __forceinline__ long long linattn_first(const LinAttnArgs& a, int s) {
+    const long long c = a.cu[s];
+    return c < 0 ? 0 : c > a.n_tokens ? a.n_tokens : c;
+}
+#endif
+
+__device__ __forceinline__ Segment linattn_segment(const LinAttnArgs& a, int j, int lane) {
+    Segment g;
+#ifdef __HIP_DEVICE_COMPILE__
+    long long len;
+    if (a.cu) {
+        // the last sequence whose first slot is at or before j, 64 candidates a round
+        int lo = 0, n = a.n_seqs;
+        while (n > 1) {
+            const int step = (n + 63) >> 6;
+            const int s = lo + lane * step;
+            const bool in = lane * step < n &&
+                            (linattn_first(a, s < a.n_seqs ? s : a.n_seqs) >> a.seg_shift) + s <= j;
+            const int hits = __popcll(__ballot(in));
+            const int at = hits ? hits - 1 : 0;
+            lo += at * step;
+            n = min(step, n - at * step);
+        }
+        g.seq = __builtin_amdgcn_readfirstlane(lo);
+        g.row = linattn_first(a, g.seq);
+        len = linattn_first(a, g.seq + 1) - g.row;
+        g.index = j - (int)((g.row >> a.seg_shift) + g.seq);
+    } else {
+        const int per = a.n_segs / a.n_seqs;
+        g.seq = j / per;
+        g.index = j - g.seq * per;
+        len = a.max_len;
+        g.row = (long long)g.seq * a.max_len;
+    }
+    g.len = (int)(len < 0 ? 0 : len > a.max_len ? a.max_len : len);
+    const long long t0 = (long long)g.index << a.seg_shift;
+    const long long t1 = t0 + (1ll << a.seg_shift);
+    g.ok = g.index >= 0 && (t0 < g.len || g.index == 0);
+    g.t0 = g.ok ? (int)t0 : 0;
+    g.t1 = t1 < g.len ? (int)t1 : g.len;
+#endif
+    return g;
+}
+
+// The state slot of a sequence, or -1: its slot is no slot of the pool, and
+// the sequence is passed over.
+__device__ __forceinline__ int linattn_slot(const LinAttnArgs& a, int seq) {
+    if (!a.slots) return seq;
+    const int s = a.slots[seq];
+    return s >= 0 && s < a.n_slots ? s : -1;
+}
+
+// Launchers, one object file each.  `full`: outputs and final states, else
+// the segments' own states.  hipError_t of the launch.
+hipError_t linattn_launch_bf16(const LinAttnArgs& a, bool full, hipStream_t st);
+hipError_t linattn_launch_f16(const LinAttnArgs& a, bool full, hipStream_t st);
+hipError_t linattn_launch_f32(const LinAttnArgs& a, bool full, hipStream_t st);
+hipError_t linattn_launch_chain(const LinAttnArgs& a, hipStream_t st);
+hipError_t linattn_launch_step(const LinAttnArgs& a, int dtype, hipStream_t st);
+
+// Columns of out that one workgroup owns: 32 for each of its two or four waves.
+inline int linattn_waves(int dv) { return dv > 64 ? 4 : 2; }
+
+}  // namespace ssla

@@ -122,6 +122,31 @@ class SslaHipOevaDiff(ctypes.Structure):
                 ("max_abs_delta", ctypes.c_double), ("n_mismatched_cp", ctypes.c_size_t)]
 
 
+# element types and activations of the sequence operators
+SSLA_F32, SSLA_BF16, SSLA_F16 = 0, 1, 2
+SSLA_ACT_NONE, SSLA_ACT_SILU, SSLA_ACT_SIGMOID, SSLA_ACT_RELU = 0, 1, 2, 3
+LINATTN_MAX_DIM = 256
+
+
+class SslaHipLinAttn(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in
+                ("dtype", "heads", "qk_heads", "dk", "dv", "n_seqs", "max_len", "n_slots")] + [
+        ("n_tokens", ctypes.c_longlong)] + [
+        (n, ctypes.c_void_p) for n in ("q", "k", "v", "log_decay", "out")] + [
+        (n, ctypes.c_longlong * 2) for n in
+        ("q_stride", "k_stride", "v_stride", "decay_stride", "out_stride")] + [
+        (n, ctypes.c_void_p) for n in ("cu_seqlens", "slots", "state_in", "state_out")] + [
+        ("state_stride", ctypes.c_longlong), ("scale", ctypes.c_float)]
+
+
+class SslaHipGroupNorm(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in
+                ("dtype", "n", "rows", "channels", "groups", "act")] + [
+        (n, ctypes.c_void_p) for n in ("x", "gate", "weight", "bias", "out")] + [
+        (n, ctypes.c_longlong * 2) for n in ("x_stride", "gate_stride", "out_stride")] + [
+        ("eps", ctypes.c_float)]
+
+
 # return codes of the C ABI (include/ssla_hip.h)
 SSLA_OK, SSLA_ERR_ARG, SSLA_ERR_HIP, SSLA_ERR_IO, SSLA_ERR_FORMAT, SSLA_ERR_STATE = 0, -1, -2, -3, -4, -5
 

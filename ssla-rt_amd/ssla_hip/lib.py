@@ -81,6 +81,13 @@ _SIGNATURES = {
                                 ctypes.c_uint]),
     "ssla_hip_oeva_diff": (_I, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_double,
                                 ctypes.POINTER(abi.SslaHipOevaDiff)]),
+    # descriptors by address: ops.py packs them (struct), abi.py mirrors them (ctypes)
+    "ssla_hip_linattn_workspace": (_I, [_VP, ctypes.POINTER(ctypes.c_size_t)]),
+    "ssla_hip_linattn": (_I, [_VP, _VP, ctypes.c_size_t, _VP]),
+    "ssla_hip_linattn_step": (_I, [_VP, _VP]),
+    "ssla_hip_group_norm_workspace": (_I, [_VP, ctypes.POINTER(ctypes.c_size_t)]),
+    "ssla_hip_group_norm": (_I, [_VP, _VP, ctypes.c_size_t, _VP]),
+    "ssla_hip_ops_layout": (_I, [ctypes.POINTER(_LL), _I]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -11,6 +11,8 @@
 
 namespace ssla {
 
+enum GroupNormKind { kGroupLanes, kGroupOnePass, kGroupTwoPass };
+
 struct GroupNormArgs {
     const void *x, *gate, *weight, *bias;
     void* out;
@@ -20,9 +22,13 @@ struct GroupNormArgs {
     float eps;
     // how the call is cut (group_norm_plan)
     int vec;                              // channels of a piece: 16 bytes where alignment allows
-    int threads, reps;                    // of a workgroup; pieces a thread keeps (one pass)
-    int gb, blocks;                       // groups of a workgroup; workgroups along the groups
-    int parts;                            // workgroups along the rows; 0: one pass
+    int kind;                             // kGroupLanes, kGroupOnePass, kGroupTwoPass
+    int threads, reps;                    // of a workgroup; pieces a thread keeps (one pass).  Lanes:
+                                          // pieces a lane keeps; lanes of a group
+    int gb, blocks, np;                   // groups of a workgroup; workgroups along the groups; pieces of
+                                          // a workgroup's row
+    int parts;                            // workgroups along the rows; 0: not two passes
+    double inv_count;                     // 1 / values of a group
 };
 
 void group_norm_plan(GroupNormArgs& a, int dtype);

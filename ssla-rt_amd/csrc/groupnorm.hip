@@ -5,6 +5,8 @@
 // up to 256 pieces of 16 bytes of a row) and rows of one item.  A thread keeps
 // to one piece of the row, so that its channels, weights and groups are fixed,
 // and steps over rows; neighbouring threads read neighbouring pieces.
+//   lanes      a group is small (a token's head): some lanes of a wave hold it,
+//              and nothing but shuffles joins them (k_group_lanes)
 //   one pass   the item's rows fit in the workgroup's registers: x is read once
 //   two passes k_group<kStats> leaves each part's sums in the workspace,
 //              k_group<kApply> adds them up and reads x again (from the 256 MB
@@ -40,6 +42,12 @@ __device__ __forceinline__ float activate(float x, int act) {
     }
 }
 
+// Mean and 1 / sqrt(var + eps).
+__device__ __forceinline__ float2 moments(Sums s, double inv_count, float eps) {
+    const double mean = s.s * inv_count, var = fma(-mean, mean, s.q * inv_count);
+    return float2{(float)mean, 1.0f / sqrtf((var < 0.0 ? 0.0f : (float)var) + eps)};      // a NaN stays
+}
+
 // Sum over the w lanes (a power of two up to 64) that share a group.
 __device__ __forceinline__ Sums lanes_sum(Sums a, int w) {
     for (int o = w >> 1; o; o >>= 1) {
@@ -49,8 +57,9 @@ __device__ __forceinline__ Sums lanes_sum(Sums a, int w) {
     return a;
 }
 
-template <class T, int V, int R, Mode MODE>
-__global__ __launch_bounds__(R > 4 ? 1024 : 256) void k_group(const GroupNormArgs a) {
+// NT: most threads of a workgroup.
+template <class T, int V, int R, int NT, Mode MODE>
+__global__ __launch_bounds__(NT) void k_group(const GroupNormArgs a) {
     extern __shared__ __align__(16) char smem[];
     typedef Piece<T, V> P;
     const int nt = blockDim.x, tid = threadIdx.x;
@@ -60,8 +69,8 @@ __global__ __launch_bounds__(R > 4 ? 1024 : 256) void k_group(const GroupNormArg
     const int item = ib / a.blocks, block = ib - item * a.blocks;
     const int g0 = block * a.gb, ng = min(a.gb, a.groups - g0);
     // columns [c0, c1) in pieces p0 .. p0 + np - 1 (the outer ones may reach over)
-    const long long c0 = (long long)g0 * cg, c1 = c0 + (long long)ng * cg;
-    const int p0 = (int)(c0 / V), np = (int)((c1 + V - 1) / V) - p0;
+    const int c0 = g0 * cg, c1 = c0 + ng * cg;
+    const int p0 = c0 / V, np = (c1 - 1) / V + 1 - p0;
     const int cols = min(np, nt), lanes = nt / cols;         // threads along a row, rows at a time
     const int py = tid / cols, px = tid - py * cols;
     const bool on = py < lanes;
@@ -72,16 +81,42 @@ __global__ __launch_bounds__(R > 4 ? 1024 : 256) void k_group(const GroupNormArg
     const T* gate = a.gate ? (const T*)a.gate + item * a.gn : nullptr;
     T* out = (T*)a.out + item * a.on;
 
-    // LDS: mean and 1 / sqrt(var + eps) of the groups (their sums while stats
-    // run), then every thread's sums (one a piece, or one a channel)
+    // LDS: the groups' sums, then their mean and 1 / sqrt(var + eps); behind them
+    // every thread's sums (one a piece, or one a channel), then the channels' table
     Sums* total = (Sums*)smem;
     float2* norm = (float2*)smem;
     Sums* own = total + a.gb;
+    float* table = (float*)own;                              // mean, scale, bias of a stretch's channels
+    const int width = cols * V;
     const int per = whole ? 1 : V;
     int w = 1;                                               // lanes that add up a group
     while (w < 64 && 2 * w * ng <= nt) w *= 2;
 
-    P keep[R];
+    // weight and bias of a channel of a stretch; each thread's first one is read ahead
+    auto weight_of = [&](int ch) {
+        const int c = p0 * V + ch;
+        return a.weight && c >= c0 && c < c1 ? (float)((const T*)a.weight)[c] : 1.0f;
+    };
+    auto bias_of = [&](int ch) {
+        const int c = p0 * V + ch;
+        return a.bias && c >= c0 && c < c1 ? (float)((const T*)a.bias)[c] : 0.0f;
+    };
+    float w0 = 1.0f, b0 = 0.0f;
+    if (MODE != kStats) w0 = weight_of(tid), b0 = bias_of(tid);
+
+    // what the last step needs first is out before the sums: the gate's pieces of
+    // the first rows, and x's where this pass has no sums of its own
+    P keep[R], pgate[R];
+    if (MODE != kStats && on) {
+        #pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const int row = r0 + py + k * lanes;
+            if (row < r1) {
+                if (gate) pgate[k] = *(const P*)(gate + row * a.gr + (long long)(p0 + px) * V);
+                if (MODE == kApply) keep[k] = *(const P*)(x + row * a.xr + (long long)(p0 + px) * V);
+            }
+        }
+    }
     if (MODE != kApply) {
         for (int g = tid; g < ng; g += nt) total[g] = Sums{0.0, 0.0};
         for (int pc = 0; pc < np; pc += cols) {              // once, where a row's pieces fit
@@ -90,24 +125,8 @@ __global__ __launch_bounds__(R > 4 ? 1024 : 256) void k_group(const GroupNormArg
             Sums acc[V];
             #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] = Sums{0.0, 0.0};
-            if (MODE == kOnePass) {
-                #pragma unroll
-                for (int k = 0; k < R; ++k) {
-                    const int row = py + k * lanes;
-                    if (in && row < r1) keep[k] = *(const P*)(x + row * a.xr + (long long)p * V);
-                }
-                #pragma unroll
-                for (int k = 0; k < R; ++k)
-                    if (in && py + k * lanes < r1) {
-                        #pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            const double v = (double)(float)keep[k].v[i];
-                            acc[i].s += v;
-                            acc[i].q = fma(v, v, acc[i].q);
-                        }
-                    }
-            } else if (in) {
-                for (int row = r0 + py; row < r1; row += R * lanes) {
+            if (in) {
+                for (int row = r0 + py; row < r1; row += R * lanes) {      // one pass: once
                     #pragma unroll
                     for (int k = 0; k < R; ++k)
                         if (row + k * lanes < r1)
@@ -122,6 +141,7 @@ __global__ __launch_bounds__(R > 4 ? 1024 : 256) void k_group(const GroupNormArg
                                 acc[i].q = fma(v, v, acc[i].q);
                             }
                         }
+                    if (MODE == kOnePass) break;
                 }
             }
             __syncthreads();                                 // `total` is set, `own` free
@@ -132,26 +152,32 @@ __global__ __launch_bounds__(R > 4 ? 1024 : 256) void k_group(const GroupNormArg
                         acc[0].s += acc[i].s;
                         acc[0].q += acc[i].q;
                     }
-                    own[py * cols + px] = acc[0];
+                    own[tid] = acc[0];
                 } else {
                     #pragma unroll
-                    for (int i = 0; i < V; ++i) own[(py * cols + px) * V + i] = acc[i];
+                    for (int i = 0; i < V; ++i) own[tid * V + i] = acc[i];
                 }
             }
             __syncthreads();
             // a group's entries: its units (pieces or channels) of this stretch, of every row lane
             const int unit = whole ? cg / V : cg;
-            const int lo = whole ? p0 + pc : (p0 + pc) * V, width = min(cols, np - pc) * per;
+            const int lo = whole ? p0 + pc : (p0 + pc) * V, wide = min(cols, np - pc) * per;
             for (int g = tid / w; g < ng; g += nt / w) {
-                const long long first = (long long)(g0 + g) * unit;
-                const int u0 = (int)max(0ll, first - lo), u1 = (int)min((long long)width, first + unit - lo);
-                const int n = max(0, u1 - u0);
+                const int first = (g0 + g) * unit;
+                const int u0 = max(0, first - lo), u1 = min(wide, first + unit - lo), n = max(0, u1 - u0);
                 Sums s = {0.0, 0.0};
-                for (int i = tid % w; i < n * lanes; i += w) {
-                    const int y = i / n, u = i - y * n;
-                    const Sums t = own[y * cols * per + u0 + u];
-                    s.s += t.s;
-                    s.q += t.q;
+                if (n) {
+                    int y = tid % w / n, u = tid % w - y * n;      // entry (row lane y, unit u)
+                    const int dy = w / n, du = w - dy * n;
+                    for (; y < lanes; y += dy, u += du) {
+                        if (u >= n) {
+                            u -= n;
+                            if (++y >= lanes) break;
+                        }
+                        const Sums t = own[y * cols * per + u0 + u];
+                        s.s += t.s;
+                        s.q += t.q;
+                    }
                 }
                 s = lanes_sum(s, w);
                 if (tid % w == 0) {
@@ -169,115 +195,200 @@ __global__ __launch_bounds__(R > 4 ? 1024 : 256) void k_group(const GroupNormArg
     }
 
     // ---- means and scales -----------------------------------------------------
-    const double count = (double)cg * a.rows;
     for (int g = tid / w; g < ng; g += nt / w) {
         Sums s = {0.0, 0.0};
         if (MODE == kApply) {
             const Sums* ws = (const Sums*)a.ws + (long long)item * nparts * a.groups + g0 + g;
-            for (int i = tid % w; i < nparts; i += w) {
-                const Sums t = ws[(long long)i * a.groups];
-                s.s += t.s;
-                s.q += t.q;
+            for (int i = tid % w; i < nparts; i += 4 * w) {
+                Sums t[4];
+                #pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    t[u] = i + u * w < nparts ? ws[(long long)(i + u * w) * a.groups] : Sums{0.0, 0.0};
+                #pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    s.s += t[u].s;
+                    s.q += t[u].q;
+                }
             }
             s = lanes_sum(s, w);
         } else {
             s = total[g];
         }
-        const double mean = s.s / count;
-        double var = s.q / count - mean * mean;
-        var = var < 0.0 ? 0.0 : var;                         // a NaN stays
         // in `total`'s place: one group's lanes read it above and write it here
-        if (tid % w == 0) {
-            if (MODE == kOnePass) {
-                float2* f = (float2*)&total[g];
-                *f = float2{(float)mean, (float)(1.0 / sqrt(var + (double)a.eps))};
-            } else {
-                norm[2 * g] = float2{(float)mean, (float)(1.0 / sqrt(var + (double)a.eps))};
-            }
-        }
+        if (tid % w == 0) norm[2 * g] = moments(s, a.inv_count, a.eps);
     }
     __syncthreads();
 
     for (int pc = 0; pc < np; pc += cols) {
+        if (pc) __syncthreads();                             // the last stretch's readers are done
+        for (int ch = tid; ch < width; ch += nt) {
+            const int at = pc * V + ch, c = p0 * V + at;
+            const bool mine = c >= c0 && c < c1, ahead = at == tid;
+            const float2 f = norm[mine ? 2 * ((c - c0) / cg) : 0];
+            table[ch] = f.x;
+            table[width + ch] = f.y * (ahead ? w0 : weight_of(at));
+            table[2 * width + ch] = ahead ? b0 : bias_of(at);
+        }
+        __syncthreads();
         const int p = p0 + pc + px;
         if (!on || pc + px >= np) continue;
-        float mean[V], rstd[V], wt[V], bs[V];
-        bool inside = true;
+        float mean[V], scale[V], bias[V];
         #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const long long c = (long long)p * V + i;
-            const bool mine = c >= c0 && c < c1;
-            inside &= mine;
-            const float2 f = norm[mine ? 2 * (int)((c - c0) / cg) : 0];
-            mean[i] = f.x;
-            rstd[i] = f.y;
-            wt[i] = a.weight && mine ? (float)((const T*)a.weight)[c] : 1.0f;
-            bs[i] = a.bias && mine ? (float)((const T*)a.bias)[c] : 0.0f;
+            mean[i] = table[px * V + i];
+            scale[i] = table[width + px * V + i];
+            bias[i] = table[2 * width + px * V + i];
         }
-        auto finish = [&](int row, const P& px_, const P& pg) {
+        const bool inside = p * V >= c0 && p * V + V <= c1;
+        auto finish = [&](int row, const P& in, const P& pg) {
             P y;
             #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float v = fmaf(((float)px_.v[i] - mean[i]) * rstd[i], wt[i], bs[i]);
-                v = gate ? v * activate((float)pg.v[i], a.act) : activate(v, a.act);
-                y.v[i] = (T)v;
+                const float v = fmaf((float)in.v[i] - mean[i], scale[i], bias[i]);
+                y.v[i] = (T)(gate ? v * activate((float)pg.v[i], a.act) : activate(v, a.act));
             }
             T* o = out + (long long)row * a.orow + (long long)p * V;
             if (inside) {
                 *(P*)o = y;
             } else {
                 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const long long c = (long long)p * V + i;
-                    if (c >= c0 && c < c1) o[i] = y.v[i];
-                }
+                for (int i = 0; i < V; ++i)
+                    if (p * V + i >= c0 && p * V + i < c1) o[i] = y.v[i];
             }
         };
-        if (MODE == kOnePass) {
-            #pragma unroll
-            for (int k = 0; k < R; ++k) {
-                const int row = py + k * lanes;
-                if (row < r1) {
-                    P pg{};
-                    if (gate) pg = *(const P*)(gate + row * a.gr + (long long)p * V);
-                    finish(row, keep[k], pg);
-                }
-            }
-        } else {
-            for (int row = r0 + py; row < r1; row += R * lanes) {
-                P pg[R];
+        for (int row = r0 + py; row < r1; row += R * lanes) {              // one pass: once
+            if (MODE == kApply && (pc || row != r0 + py)) {
                 #pragma unroll
                 for (int k = 0; k < R; ++k)
                     if (row + k * lanes < r1) {
                         keep[k] = *(const P*)(x + (long long)(row + k * lanes) * a.xr + (long long)p * V);
                         if (gate)
-                            pg[k] = *(const P*)(gate + (long long)(row + k * lanes) * a.gr + (long long)p * V);
+                            pgate[k] = *(const P*)(gate + (long long)(row + k * lanes) * a.gr + (long long)p * V);
                     }
-                #pragma unroll
-                for (int k = 0; k < R; ++k)
-                    if (row + k * lanes < r1) finish(row + k * lanes, keep[k], pg[k]);
             }
+            #pragma unroll
+            for (int k = 0; k < R; ++k)
+                if (row + k * lanes < r1) finish(row + k * lanes, keep[k], pgate[k]);
+            if (MODE == kOnePass) break;
         }
     }
 }
 
+// ---- small groups --------------------------------------------------------------
+// `w` lanes hold a group of one item, R pieces each; neighbouring lanes' groups
+// are neighbours.  The mean first, then the sum of squared differences from it.
+template <class T, int V, int R>
+__global__ __launch_bounds__(256) void k_group_lanes(const GroupNormArgs a) {
+    typedef Piece<T, V> P;
+    const int w = a.reps;                                    // lanes of a group
+    const int l = threadIdx.x & (w - 1);
+    const long long ig = (long long)blockIdx.x * (256 / w) + threadIdx.x / w;
+    const long long item = ig / a.groups;
+    const int group = (int)(ig - item * a.groups);
+    const bool on = item < a.n;
+    const int cg = a.channels / a.groups, pr = cg / V;       // pieces of a row of the group
+    const int pieces = pr * a.rows;
+    const T* x = (const T*)a.x + item * a.xn + (long long)group * cg;
+    const T* gate = a.gate ? (const T*)a.gate + item * a.gn + (long long)group * cg : nullptr;
+    T* out = (T*)a.out + item * a.on + (long long)group * cg;
+
+    P px[R], pg[R], pw[R], pb[R];
+    #pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int i = l + k * w;
+        #pragma unroll
+        for (int j = 0; j < V; ++j) px[k].v[j] = pg[k].v[j] = pb[k].v[j] = (T)0.0f, pw[k].v[j] = (T)1.0f;
+        if (on && i < pieces) {
+            const int row = i / pr, p = (i - row * pr) * V;
+            px[k] = *(const P*)(x + row * a.xr + p);
+            if (gate) pg[k] = *(const P*)(gate + row * a.gr + p);
+            if (a.weight) pw[k] = *(const P*)((const T*)a.weight + (long long)group * cg + p);
+            if (a.bias) pb[k] = *(const P*)((const T*)a.bias + (long long)group * cg + p);
+        }
+    }
+    float s = 0.0f;
+    #pragma unroll
+    for (int k = 0; k < R; ++k) {                            // by pairs: log2 roundings a term
+        float t[V];
+        #pragma unroll
+        for (int j = 0; j < V; ++j) t[j] = (float)px[k].v[j];
+        #pragma unroll
+        for (int o = V / 2; o; o >>= 1)
+            #pragma unroll
+            for (int j = 0; j < o; ++j) t[j] += t[j + o];
+        s += t[0];
+    }
+    for (int o = w >> 1; o; o >>= 1) s += __shfl_xor(s, o);
+    const float mean = s * (float)a.inv_count;
+    double q = 0.0;                                          // squares do not overflow
+    #pragma unroll
+    for (int k = 0; k < R; ++k)
+        if (l + k * w < pieces) {
+            #pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const double d = (double)((float)px[k].v[j] - mean);
+                q = fma(d, d, q);
+            }
+        }
+    for (int o = w >> 1; o; o >>= 1) q += __shfl_xor(q, o);
+    const float rstd = 1.0f / sqrtf((float)(q * a.inv_count) + a.eps);
+    #pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int i = l + k * w;
+        if (on && i < pieces) {
+            const int row = i / pr, p = (i - row * pr) * V;
+            P y;
+            #pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float v = fmaf(((float)px[k].v[j] - mean) * rstd, (float)pw[k].v[j], (float)pb[k].v[j]);
+                y.v[j] = (T)(gate ? v * activate((float)pg[k].v[j], a.act) : activate(v, a.act));
+            }
+            *(P*)(out + row * a.orow + p) = y;
+        }
+    }
+}
+
+// Pieces a thread of a 1024-thread workgroup keeps: what 128 registers hold.
+template <int V> constexpr int kWideReps = V == 8 ? 2 : 4;
+
+// LDS of a workgroup of k_group: the groups' sums, and the larger of the threads'
+// sums (of every channel, where groups do not begin with pieces) and the table.
+size_t group_norm_lds(const GroupNormArgs& a, int threads, long long np) {
+    const size_t sums = (size_t)threads * (a.channels / a.groups % a.vec ? a.vec : 1) * sizeof(Sums);
+    const size_t table = (size_t)(np < threads ? np : threads) * a.vec * 3 * sizeof(float);
+    return sizeof(Sums) * (size_t)a.gb + (sums > table ? sums : table);
+}
+
 template <class T, int V>
 hipError_t launch(const GroupNormArgs& a, hipStream_t st) {
+    if (a.kind == kGroupLanes) {
+        GroupNormArgs args = a;
+        void* pa[] = {&args};
+        const long long per = 256 / a.reps, wgs = ((long long)a.n * a.groups + per - 1) / per;
+        const void* f = a.threads == 1   ? (const void*)k_group_lanes<T, V, 1>
+                        : a.threads == 2 ? (const void*)k_group_lanes<T, V, 2>
+                                         : (const void*)k_group_lanes<T, V, 4>;
+        return hipLaunchKernel(f, dim3((unsigned)wgs), dim3(256), pa, 0, st);
+    }
     GroupNormArgs args = a;
     void* pa[] = {&args};
-    const int per = a.channels / a.groups % V ? V : 1;
-    const unsigned lds = (unsigned)(sizeof(Sums) * ((size_t)a.gb + (size_t)a.threads * per));
+    const size_t lds = group_norm_lds(a, a.threads, a.np);
     const long long wgs = (long long)a.n * a.blocks;
-    if (!a.parts) {
-        const void* f = a.threads > 256 ? (const void*)k_group<T, V, 16, kOnePass>
-                        : a.reps > 1    ? (const void*)k_group<T, V, 4, kOnePass>
-                                        : (const void*)k_group<T, V, 1, kOnePass>;
+    if (a.kind == kGroupOnePass) {
+        const void* f = a.threads > 256 ? (const void*)k_group<T, V, kWideReps<V>, 1024, kOnePass>
+                        : a.reps > 1    ? (const void*)k_group<T, V, 4, 256, kOnePass>
+                                        : (const void*)k_group<T, V, 1, 256, kOnePass>;
+        if (lds > 65536) {
+            const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e != hipSuccess) return e;
+        }
         return hipLaunchKernel(f, dim3((unsigned)wgs), dim3(a.threads), pa, lds, st);
     }
     const dim3 grid((unsigned)(wgs * a.parts));
-    const hipError_t e = hipLaunchKernel((const void*)k_group<T, V, 4, kStats>, grid, dim3(a.threads), pa, lds, st);
+    const void* f = (const void*)k_group<T, V, 4, 256, kStats>;
+    const hipError_t e = hipLaunchKernel(f, grid, dim3(a.threads), pa, lds, st);
     if (e != hipSuccess) return e;
-    return hipLaunchKernel((const void*)k_group<T, V, 4, kApply>, grid, dim3(a.threads), pa, lds, st);
+    return hipLaunchKernel((const void*)k_group<T, V, 4, 256, kApply>, grid, dim3(a.threads), pa, lds, st);
 }
 
 template <class T>
@@ -293,27 +404,49 @@ hipError_t launch_vec(const GroupNormArgs& a, hipStream_t st) {
 void group_norm_plan(GroupNormArgs& a, int dtype) {
     const int e = dtype == SSLA_F32 ? 4 : 2;
     // pieces: 16 bytes, or what the addresses, strides and rows are multiples of
-    unsigned long long bits = (unsigned long long)a.channels | a.xr | a.xn | a.orow | a.on | 16 / e;
-    if (a.gate) bits |= (unsigned long long)(a.gr | a.gn);
-    bits = bits * e | (unsigned long long)(size_t)a.x | (size_t)a.out | (size_t)a.gate;
+    unsigned long long bits = (unsigned long long)a.channels | a.orow | a.xr | 16 / e;
+    if (a.n > 1) bits |= (unsigned long long)(a.xn | a.on);
+    if (a.gate) bits |= (unsigned long long)(a.gr | (a.n > 1 ? a.gn : 0));
+    bits = bits * e | (unsigned long long)(size_t)a.x | (size_t)a.out | (size_t)a.gate | (size_t)a.weight |
+           (size_t)a.bias;
     a.vec = (int)((bits & -bits) / e);
     const int cg = a.channels / a.groups;
-    const int pieces = a.channels / a.vec;
-    a.blocks = (pieces + 255) / 256;
+    const double count = (double)cg * a.rows;
+    a.inv_count = 1.0 / count;
+    a.parts = 0;
+    // lanes of a wave, one to four pieces each, hold a group: as few pieces as
+    // 64 lanes allow (a token's groups of 128 bf16 channels: 16 lanes, one piece)
+    int v = a.vec;
+    while (cg % v) v /= 2;
+    const long long pieces = (long long)a.rows * (cg / v);
+    for (int r = 1; r <= 4; r *= 2)
+        if (pieces <= 64 * r) {
+            int w = 1;
+            while (w * r < pieces) w *= 2;
+            a.kind = kGroupLanes;
+            a.vec = v;
+            a.reps = w;
+            a.threads = r;
+            a.gb = a.blocks = 1;
+            return;
+        }
+    const int row = a.channels / a.vec;
+    a.blocks = (row + 255) / 256;
     a.gb = (a.groups + a.blocks - 1) / a.blocks;
     a.blocks = (a.groups + a.gb - 1) / a.gb;
     // pieces of a workgroup's row; one more where its first channel is not a piece's
     const long long np = ((long long)a.gb * cg + a.vec - 1) / a.vec + (cg % a.vec && a.blocks > 1 ? 1 : 0);
-    a.parts = 0;
-    const bool wide = cg % a.vec == 0;      // 1024 threads' sums of every channel would not fit the LDS
-    for (int nt = 64; nt <= (wide ? 1024 : 256); nt *= 4) {
-        if (np > nt) continue;
+    a.np = (int)np;
+    a.kind = kGroupOnePass;
+    for (int nt = 64; nt <= 1024; nt *= 4) {
+        if (np > nt || group_norm_lds(a, nt, np) > 144 * 1024) continue;
         const long long reps = (a.rows + nt / np - 1) / (nt / np);
-        if (reps > (nt == 64 ? 1 : nt == 256 ? 4 : 16)) continue;
+        if (reps > (nt == 64 ? 1 : nt == 1024 && a.vec == 8 ? kWideReps<8> : 4)) continue;
         a.threads = nt;
         a.reps = (int)reps;
         return;
     }
+    a.kind = kGroupTwoPass;
     a.threads = 256;
     a.reps = 4;
     const long long lanes = np > 256 ? 1 : 256 / np;

@@ -4,8 +4,7 @@
 //   S_t = exp(g_t) S_{t-1} + k_t v_t^T,     o_t = scale q_t^T S_t     (S: dk x dv)
 //
 // A workgroup runs one segment of one sequence for one head and one slice of
-// the dv columns, chunk by chunk with the state in registers (linattn16.h,
-// linattn32.h).  Sequences longer than a segment take three launches: the
+// the dv columns, chunk by chunk with the state in registers (linattn_kernel.h).  Sequences longer than a segment take three launches: the
 // segments' own states from zero (FULL = false), the states before each
 // segment (k_linattn_chain), then every segment from its state (FULL = true).
 #pragma once
@@ -35,7 +34,7 @@ struct LinAttnArgs {
     int n_seqs, n_slots, max_len;
     int heads, rep, dk, dv, slices;       // rep: heads sharing q and k
     int seg_shift, n_segs;                // log2 of a segment's tokens; segments of the call
-    int vec_in, vec_out;                  // 16-byte loads of q, k, v; wide stores of out
+    int vec;                              // buffer loads of q, k, v and stores of out, in pieces
     float scale;
 };
 
@@ -110,7 +109,20 @@ hipError_t linattn_launch_f32(const LinAttnArgs& a, bool full, hipStream_t st);
 hipError_t linattn_launch_chain(const LinAttnArgs& a, hipStream_t st);
 hipError_t linattn_launch_step(const LinAttnArgs& a, int dtype, hipStream_t st);
 
-// Columns of out that one workgroup owns: 32 for each of its two or four waves.
-inline int linattn_waves(int dv) { return dv > 64 ? 4 : 2; }
+// Waves of a workgroup: each owns 16 columns of out.
+inline int linattn_waves(int dk, int dv) { return dk > 128 || dv <= 64 ? 4 : dv <= 96 ? 6 : 8; }
+
+// Launches a chunked kernel with `lds` bytes.  More than 64 KB of LDS has to be
+// asked for; the attribute is the function's, and setting it again costs a lookup.
+inline hipError_t linattn_launch(const void* f, const LinAttnArgs& a, int waves, size_t lds, hipStream_t st) {
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    LinAttnArgs args = a;
+    void* pa[] = {&args};
+    const long long blocks = (long long)a.n_segs * a.heads * a.slices;
+    return hipLaunchKernel(f, dim3((unsigned)blocks), dim3(64 * waves), pa, lds, st);
+}
 
 }  // namespace ssla

@@ -1,8 +1,8 @@
-// linattn_f16.hip -- chunked linear attention over fp16 tokens (linattn16.h).
-#include "linattn16.h"
+// linattn_f16.hip -- chunked linear attention over fp16 tokens (linattn_kernel.h).
+#include "linattn_kernel.h"
 
 namespace ssla {
 hipError_t linattn_launch_f16(const LinAttnArgs& a, bool full, hipStream_t st) {
-    return la16::launch<_Float16>(a, full, st);
+    return chunk::launch<_Float16>(a, full, st);
 }
 }  // namespace ssla

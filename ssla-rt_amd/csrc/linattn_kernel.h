@@ -1,0 +1,504 @@
+// linattn_kernel.h -- chunked linear attention on the 16 x 16 x 32 bf16 matrix
+// instruction, for bf16, fp16 and fp32 tokens.
+//
+// Over a chunk of C tokens, b_i = g_1 + ... + g_i and S the state before it:
+//   P_ij = (q_i . k_j) exp(b_i - b_j)  for j <= i, else 0
+//   o_i  = scale (exp(b_i) q_i^T S + sum_j P_ij v_j)
+//   S'   = exp(b_C) S + sum_j k_j (exp(b_C - b_j) v_j)^T
+// Everything is computed transposed, so that what one product leaves in the
+// D registers (row 4 g + r, column m of lane 16 g + m) is the next one's A or
+// B operand as it lies (column or row m, eight values of the contraction a
+// lane): the state is S[d][e] with d along the registers, which is the A
+// operand of O^T = S^T Q^T, a lane's eight values of a step being rows 4 g + r
+// of two tiles.  The order of a contraction is free, so q's columns and P's
+// are put into that order on their way to LDS (operand_at), and tokens are
+// taken in it from k and v.
+//
+// Precision: an operand is the sum of bf16 terms, each the rounding of what the
+// ones before leave (2^-8 each time): a bf16 token value is one term, an fp16
+// value two, both exactly; an fp32 value, and P and S there, three.  For 16-bit
+// tokens P and the copy of S that multiplies q have two (2^-16, well below the
+// output's 2^-8 or 2^-11), exp(b_C - b_j) v_j three, since these products make
+// up the fp32 state.  Products of terms whose orders add up to more than the
+// last kept one's are left out.  fp32 tokens take 6 bf16 products of 16 cycles
+// where the fp32 instruction takes 256 cycles for the same block.
+//
+// Each wave owns 16 columns of v, the state and the output; the C x C products
+// P are dealt over the waves and shared through LDS.
+#pragma once
+
+#include "linattn_chunk.h"
+
+namespace ssla {
+namespace chunk {
+
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f4 mma(bf8 a, bf8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// Two values rounded to bf16, packed; x keeps what is left of them.
+__device__ __forceinline__ unsigned split2(float& x, float& y) {
+    const unsigned h = __builtin_bit_cast(unsigned, __builtin_convertvector(f2{x, y}, bf2));
+    x -= __builtin_bit_cast(float, h << 16);
+    y -= __builtin_bit_cast(float, h & 0xffff0000u);
+    return h;
+}
+__device__ __forceinline__ unsigned round2(float x, float y) {
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{x, y}, bf2));
+}
+// x as N bf16 terms.
+template <int N>
+__device__ __forceinline__ void split(f8 x, bf8 (&t)[N]) {
+    #pragma unroll
+    for (int n = 0; n < N; ++n) {
+        u4 h;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float a = x[2 * i], b = x[2 * i + 1];
+            h[i] = n + 1 < N ? split2(a, b) : round2(a, b);
+            x[2 * i] = a;
+            x[2 * i + 1] = b;
+        }
+        t[n] = __builtin_bit_cast(bf8, h);
+    }
+}
+template <int N>
+__device__ __forceinline__ void split(f4 x, u2 (&t)[N]) {
+    #pragma unroll
+    for (int n = 0; n < N; ++n)
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float a = x[2 * i], b = x[2 * i + 1];
+            t[n][i] = n + 1 < N ? split2(a, b) : round2(a, b);
+            x[2 * i] = a;
+            x[2 * i + 1] = b;
+        }
+}
+
+__device__ __forceinline__ f8 join(f4 a, f4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ s8 join(s4 a, s4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// Four rows of a column-major operand: lane m of each group of 16 gets column
+// m of rows 0..3 of the 4 x 16 block whose 8-byte pieces the group's lanes
+// address (lane n: row n / 4, columns 4 (n % 4) ..).
+__device__ __forceinline__ s4 tr4(const void* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s4*)(__attribute__((address_space(3))) void*)p);
+}
+
+// Place of index i of a contraction in an operand's row: a lane's eight values of
+// a step, 32 s + 4 g .. and 32 s + 16 + 4 g .., lie together at 32 s + 8 g.
+__device__ __forceinline__ int operand_at(int i) { return (i & ~31) | (i & 12) << 1 | (i & 16) >> 2 | (i & 3); }
+
+// Elements behind a row of w (a multiple of 32) bf16 in LDS.  Rows then begin an odd
+// multiple of four of the 64 banks apart, and four in turn at least eight apart:
+// 16 rows' pieces of 8 or 16 bytes and 4 rows' 32 bytes (tr4) meet no bank twice.
+constexpr int pad(int w) { return w % 128 == 0 || w % 128 == 32 ? 24 : 8; }
+
+// Token types: terms of a value; how v lies in LDS, comes from there and is
+// searched for infinities and NaN.
+template <class T> struct Token;
+template <class T> struct Token16 {
+    typedef T V8 __attribute__((ext_vector_type(8)));
+    template <int W> static constexpr int stride() { return W + pad(W); }
+    // column m of the wave's 16 columns at `col`, tokens t + 4 g .. and t + 16 + 4 g ..
+    template <int VS> static __device__ __forceinline__ V8 column(const T* v, int t, int col, int m, int g) {
+        const T* p = &v[(t + 4 * g + (m >> 2)) * VS + col + 4 * (m & 3)];
+        return __builtin_bit_cast(V8, join(tr4(p), tr4(p + 16 * VS)));
+    }
+    static __device__ __forceinline__ f8 wide(V8 x) { return __builtin_convertvector(x, f8); }
+};
+template <> struct Token<__bf16> : Token16<__bf16> {
+    static constexpr int TERMS = 1;
+    static constexpr unsigned EXP = 0x7f807f80u;           // exponent bits of two values
+    static __device__ __forceinline__ void terms(V8 x, bf8 (&t)[1]) { t[0] = x; }
+};
+template <> struct Token<_Float16> : Token16<_Float16> {
+    static constexpr int TERMS = 2;
+    static constexpr unsigned EXP = 0x7c007c00u;
+    static __device__ __forceinline__ void terms(V8 x, bf8 (&t)[2]) { split(wide(x), t); }
+};
+template <> struct Token<float> {
+    typedef f8 V8;
+    static constexpr int TERMS = 3;
+    template <int W> static constexpr int stride() { return W + 4; }     // four rows 16 banks apart
+    template <int VS> static __device__ __forceinline__ f8 column(const float* v, int t, int col, int m, int g) {
+        f8 x;
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = v[(t + (i >> 2) * 16 + 4 * g + (i & 3)) * VS + col + m];
+        return x;
+    }
+    static __device__ __forceinline__ f8 wide(f8 x) { return x; }
+    static __device__ __forceinline__ void terms(f8 x, bf8 (&t)[3]) { split(x, t); }
+};
+
+// Whether any of a lane's values is an infinity or NaN.
+template <class T, int N, class V8>
+__device__ __forceinline__ bool odd_values(const V8 (&v)[N]) {
+    if constexpr (sizeof(T) == 2) {
+        us2 most = {0, 0};                     // largest exponents of two interleaved sets
+        #pragma unroll
+        for (int s = 0; s < N; ++s)
+            #pragma unroll
+            for (int i = 0; i < 4; ++i)
+                most = __builtin_elementwise_max(
+                    most, __builtin_bit_cast(us2, __builtin_bit_cast(u4, v[s])[i] & Token<T>::EXP));
+        const unsigned short ex = (unsigned short)Token<T>::EXP;
+        return most[0] == ex || most[1] == ex;
+    } else {
+        unsigned most = 0;
+        #pragma unroll
+        for (int s = 0; s < N; ++s)
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) most = max(most, __builtin_bit_cast(unsigned, (float)v[s][i]) & 0x7f800000u);
+        return most == 0x7f800000u;
+    }
+}
+__device__ __forceinline__ bool not_finite(float x) {
+    return (__builtin_bit_cast(unsigned, x) & 0x7f800000u) == 0x7f800000u;
+}
+
+// A piece's four values at `x`, `part` of it, as terms.
+template <class T>
+__device__ __forceinline__ void piece_terms(u4 x, int part, u2 (&t)[Token<T>::TERMS]) {
+    if constexpr (sizeof(T) == 4) {
+        split(__builtin_bit_cast(f4, x), t);
+    } else if constexpr (Token<T>::TERMS == 2) {
+        const u2 y = {x[2 * part], x[2 * part + 1]};
+        split(__builtin_convertvector(__builtin_bit_cast(h4, y), f4), t);
+    } else {
+        t[0] = u2{x[2 * part], x[2 * part + 1]};
+    }
+}
+
+template <class T, int DK, int NW>
+struct Lds {
+    static constexpr int TERMS = Token<T>::TERMS, PT = TERMS == 3 ? 3 : 2;       // PT: terms of P and S
+    // Tokens of a chunk: 64, or 32 where 64 would take a compute unit's LDS alone
+    // (three terms: 133 KB for dk = dv = 96) or not fit it (fp16, dk = 256: 171 KB).
+    static constexpr int C = TERMS == 3 || (TERMS == 2 && DK > 128) ? 32 : 64;
+    static constexpr int DV = 16 * NW;
+    static constexpr int QS = DK + pad(DK), PS = C + pad(C), VS = Token<T>::template stride<DV>();
+    __bf16 q[TERMS][C * QS];     // columns in operand order
+    __bf16 k[TERMS][C * QS];
+    T v[C * VS];
+    __bf16 p[PT][C * PS];        // rows i, columns j in operand order
+    Decays<C> b[2];              // of this chunk and the next
+};
+
+template <class T, int DK, int NW, bool FULL, bool VEC>
+__global__ __launch_bounds__(64 * NW, waves_per_simd(DK, FULL)) void k_linattn(const LinAttnArgs a) {
+    typedef Token<T> Tk;
+    typedef typename Tk::V8 V8;
+    typedef Lds<T, DK, NW> L;
+    constexpr int NT = 64 * NW, TERMS = L::TERMS, PT = L::PT, C = L::C;
+    constexpr int DT = DK / 16, KS = DK / 32;              // tiles, steps along d
+    constexpr int IT = C / 16, CS = C / 32;                // tiles, steps along tokens
+    constexpr int OUT_ORDER = PT - 1;                      // highest order of terms' products kept
+    extern __shared__ __align__(16) char smem[];
+    L& lds = *reinterpret_cast<L*>(smem);
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int m = lane & 15, g = lane >> 4;
+    Place<T, NW> pl;
+    if (!pl.find(a, FULL, wave, lane)) return;
+    const Segment& sg = pl.sg;
+    const int dvs = a.dv - pl.slice * L::DV;               // columns of v from the slice's first
+
+    f4 S[DT];
+    read_state(S, pl, a, FULL, m, g);
+
+    Rows<T, DK, C, NT, VEC> rq, rk;
+    Rows<T, L::DV, C, NT, VEC> rv;
+    float rg = 0.0f;
+    rk.init(a.kt, a.dk, tid);
+    rv.init(a.vt, dvs, tid);
+    if (FULL) rq.init(a.qt, a.dk, tid);
+    auto load = [&](int t) {
+        const int n = min(C, sg.t1 - t);
+        const long long row = sg.row + t;
+        rk.load(pl.k + row * a.kt, a.kt, a.dk, n, tid);
+        rv.load(pl.v + row * a.vt, a.vt, dvs, n, tid);
+        if (FULL) rq.load(pl.q + row * a.qt, a.qt, a.dk, n, tid);
+        if (wave == NW - 1) rg = lane < n ? pl.g[(row + lane) * a.gt] : 0.0f;
+    };
+
+    if (FULL) {     // the tiles of P above the diagonal are never written again
+        for (int i = tid; i < PT * C * L::PS; i += NT) (&lds.p[0][0])[i] = (__bf16)0.0f;
+    }
+    float decay = 1.0f;                        // of the whole segment (exp of the sum of g)
+    if (sg.t0 < sg.t1) {
+        load(sg.t0);
+        if (wave == NW - 1) lds.b[0].set(rg, a.scale, lane);
+    }
+    int buf = 0;
+    for (int t = sg.t0; t < sg.t1; t += C, buf ^= 1) {
+        const int n = min(C, sg.t1 - t);
+        __syncthreads();                       // the last chunk's readers are done
+        #pragma unroll
+        for (int p = 0; p < rk.N; ++p) {
+            const int row = rk.row(p, tid);
+            if (!rk.STEPS && row >= C) continue;
+            #pragma unroll
+            for (int part = 0; part < rk.E / 4; ++part) {
+                const int c = rk.col(p, tid) + 4 * part;
+                u2 x[TERMS];
+                piece_terms<T>(rk.x[p], part, x);
+                #pragma unroll
+                for (int i = 0; i < TERMS; ++i) *(u2*)&lds.k[i][row * L::QS + c] = x[i];
+                if (FULL) {
+                    piece_terms<T>(rq.x[p], part, x);
+                    #pragma unroll
+                    for (int i = 0; i < TERMS; ++i) *(u2*)&lds.q[i][row * L::QS + operand_at(c)] = x[i];
+                }
+            }
+        }
+        #pragma unroll
+        for (int p = 0; p < rv.N; ++p) *(u4*)&lds.v[rv.row(p, tid) * L::VS + rv.col(p, tid)] = rv.x[p];
+        __syncthreads();
+        if (t + C < sg.t1) load(t + C);
+
+        f4 O[IT];
+        if (FULL) {
+            // ---- P^T = K Q^T: the tiles on and below the diagonal ------------
+            for (int u = wave; u < IT * (IT + 1) / 2; u += NW) {
+                const int it = u >= 6 ? 3 : u >= 3 ? 2 : u >= 1 ? 1 : 0;
+                const int jt = u - it * (it + 1) / 2;
+                f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+                constexpr int KH = TERMS > 1 ? 1 : KS > 4 ? 4 : KS;              // steps in flight
+                #pragma unroll
+                for (int s0 = 0; s0 < KS; s0 += KH) {
+                    bf8 ka[KH][TERMS], qa[KH][TERMS];
+                    #pragma unroll
+                    for (int s = 0; s < KH; ++s)
+                        #pragma unroll
+                        for (int i = 0; i < TERMS; ++i) {
+                            const __bf16* p = &lds.k[i][(16 * jt + m) * L::QS + 32 * (s0 + s) + 4 * g];
+                            ka[s][i] = __builtin_bit_cast(bf8, join(*(const s4*)p, *(const s4*)(p + 16)));
+                            qa[s][i] = *(const bf8*)&lds.q[i][(16 * it + m) * L::QS + 32 * (s0 + s) + 8 * g];
+                        }
+                    loads_stay_above();
+                    #pragma unroll
+                    for (int s = 0; s < KH; ++s)
+                        #pragma unroll
+                        for (int i = 0; i < TERMS; ++i)
+                            #pragma unroll
+                            for (int j = 0; j < TERMS; ++j)
+                                if (i + j <= OUT_ORDER) acc = mma(ka[s][i], qa[s][j], acc);
+                }
+                const int i = 16 * it + m, j = 16 * jt + 4 * g;
+                const f4 jh = *(const f4*)&lds.b[buf].hi[j], jl = *(const f4*)&lds.b[buf].lo[j];
+                const float ih = lds.b[buf].hi[i], il = lds.b[buf].lo[i];
+                f4 p;
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) p[r] = acc[r] * (a.scale * exp2_((ih - jh[r]) + (il - jl[r])));
+                if (it == jt)
+                    #pragma unroll
+                    for (int r = 0; r < 4; ++r) p[r] = j + r <= i ? p[r] : 0.0f;
+                u2 x[PT];
+                split(p, x);
+                #pragma unroll
+                for (int h = 0; h < PT; ++h) *(u2*)&lds.p[h][i * L::PS + operand_at(j)] = x[h];
+            }
+            // ---- O^T = S^T Q^T ------------------------------------------------
+            #pragma unroll
+            for (int it = 0; it < IT; ++it) O[it] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            bf8 qa[2][IT][TERMS];
+            auto read_q = [&](int s) {
+                #pragma unroll
+                for (int it = 0; it < IT; ++it)
+                    #pragma unroll
+                    for (int i = 0; i < TERMS; ++i)
+                        qa[s & 1][it][i] = *(const bf8*)&lds.q[i][(16 * it + m) * L::QS + 32 * s + 8 * g];
+            };
+            read_q(0);
+            #pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                if (s + 1 < KS) read_q(s + 1);
+                loads_stay_above();
+                bf8 sa[PT];
+                split(join(S[2 * s], S[2 * s + 1]), sa);
+                #pragma unroll
+                for (int h = 0; h < PT; ++h)
+                    #pragma unroll
+                    for (int i = 0; i < TERMS; ++i)
+                        if (h + i <= OUT_ORDER)
+                            #pragma unroll
+                            for (int it = 0; it < IT; ++it) O[it] = mma(sa[h], qa[s & 1][it][i], O[it]);
+            }
+            #pragma unroll
+            for (int it = 0; it < IT; ++it) O[it] *= lds.b[buf].eb[16 * it + m];
+        }
+        // v^T of the wave's columns
+        V8 vf[CS];
+        #pragma unroll
+        for (int s = 0; s < CS; ++s) vf[s] = Tk::template column<L::VS>(lds.v, 32 * s, 16 * wave, m, g);
+        if (FULL) __syncthreads();             // P is whole
+        // An infinity or NaN of v must not reach the rows before it through their
+        // zeros of P: it is taken out here, and its column set to NaN from its
+        // token on.
+        const bool any_bad = __any(odd_values<T>(vf));
+        int bad = C;                           // the column's first such token
+        if (any_bad) {
+            rare();
+            #pragma unroll
+            for (int s = CS - 1; s >= 0; --s)
+                #pragma unroll
+                for (int i = 7; i >= 0; --i)
+                    if (not_finite((float)vf[s][i])) {
+                        bad = 32 * s + (i >> 2) * 16 + 4 * g + (i & 3);
+                        vf[s][i] = 0;
+                    }
+            bad = min(bad, __shfl_xor(bad, 16));
+            bad = min(bad, __shfl_xor(bad, 32));
+        }
+
+        if (FULL) {
+            // ---- O^T += V^T P^T -------------------------------------------------
+            // (token tile, step): the tiles of the second step take both
+            constexpr int NU = CS == 2 ? 6 : 2;
+            constexpr int PU[6][2] = {{0, 0}, {1, 0}, {2, 0}, {3, 0}, {2, 1}, {3, 1}};
+            bf8 pa[2][PT], vt[CS][TERMS];
+            auto read_p = [&](int u) {
+                #pragma unroll
+                for (int h = 0; h < PT; ++h)
+                    pa[u & 1][h] = *(const bf8*)&lds.p[h][(16 * PU[u][0] + m) * L::PS + 32 * PU[u][1] + 8 * g];
+            };
+            read_p(0);
+            #pragma unroll
+            for (int s = 0; s < CS; ++s) Tk::terms(vf[s], vt[s]);
+            #pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                if (u + 1 < NU) read_p(u + 1);
+                loads_stay_above();
+                const int it = PU[u][0], s = PU[u][1];
+                #pragma unroll
+                for (int h = 0; h < PT; ++h)
+                    #pragma unroll
+                    for (int i = 0; i < TERMS; ++i)
+                        if (h + i <= OUT_ORDER) O[it] = mma(vt[s][i], pa[u & 1][h], O[it]);
+            }
+            if (any_bad) {
+                rare();
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int first = __shfl(bad, 4 * g + r);
+                    #pragma unroll
+                    for (int it = 0; it < IT; ++it)
+                        if (16 * it + m >= first) O[it][r] = __builtin_nanf("");
+                }
+            }
+            T* const ob = (T*)a.out + (sg.row + t) * a.ot + (long long)pl.head * a.oh;
+            const auto bo = buffer(ob, VEC ? ((n - 1) * a.ot + a.dv) * (int)sizeof(T) : 0);
+            const int e = pl.e0 + 4 * g;
+            #pragma unroll
+            for (int it = 0; it < IT; ++it) {
+                const int i = 16 * it + m;
+                T y[4];
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = (T)O[it][r];
+                if (VEC) {
+                    const unsigned at = e < a.dv ? (unsigned)(i * (int)a.ot + e) * (unsigned)sizeof(T) : kOut;
+                    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b128(*(const u4*)y, bo, at, 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b64(*(const u2*)y, bo, at, 0, 0);
+                } else if (i < n) {
+                    #pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (e + r < a.dv) ob[i * a.ot + e + r] = y[r];
+                }
+            }
+        }
+
+        // ---- S = exp(b_C) S + K^T (w v): for the next chunk, or as an answer ----
+        const float eC = lds.b[buf].end;
+        decay *= eC;
+        if (!FULL || !pl.last || t + C < sg.t1 || a.s_out) {
+            bf8 ka[2][TERMS];                  // k^T of a tile of d and a step of tokens
+            auto read_k = [&](int s, int dt) {
+                #pragma unroll
+                for (int i = 0; i < TERMS; ++i) {
+                    const __bf16* p = &lds.k[i][(32 * s + 4 * g + (m >> 2)) * L::QS + 16 * dt + 4 * (m & 3)];
+                    ka[dt & 1][i] = __builtin_bit_cast(bf8, join(tr4(p), tr4(p + 16 * L::QS)));
+                }
+            };
+            read_k(0, 0);
+            #pragma unroll
+            for (int dt = 0; dt < DT; ++dt) S[dt] *= eC;
+            #pragma unroll
+            for (int s = 0; s < CS; ++s) {
+                const float* w = &lds.b[buf].w[32 * s + 4 * g];
+                bf8 x[3];
+                split(Tk::wide(vf[s]) * join(*(const f4*)w, *(const f4*)(w + 16)), x);
+                #pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    if (dt + 1 < DT) read_k(s, dt + 1);
+                    else if (s + 1 < CS) read_k(s + 1, 0);
+                    loads_stay_above();
+                    #pragma unroll
+                    for (int h = 0; h < 3; ++h)
+                        #pragma unroll
+                        for (int i = 0; i < TERMS; ++i)
+                            if (h + i <= 2) S[dt] = mma(ka[dt & 1][i], x[h], S[dt]);
+                }
+            }
+            if (any_bad) {
+                rare();
+                if (bad < C) {
+                    #pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+                        #pragma unroll
+                        for (int r = 0; r < 4; ++r) S[dt][r] = __builtin_nanf("");
+                }
+            }
+        }
+        if (t + C < sg.t1 && wave == NW - 1) lds.b[buf ^ 1].set(rg, a.scale, lane);
+    }
+
+    if (!FULL && pl.slice == 0 && tid == 0) a.ws_decay[(long long)pl.j_seg * a.heads + pl.head] = decay;
+    write_state(S, pl, a, FULL, m, g);
+}
+
+template <class T, int DK, int NW>
+hipError_t launch_one(const LinAttnArgs& a, bool full, hipStream_t st) {
+    const void* f = full ? (a.vec ? (const void*)k_linattn<T, DK, NW, true, true>
+                                  : (const void*)k_linattn<T, DK, NW, true, false>)
+                         : (a.vec ? (const void*)k_linattn<T, DK, NW, false, true>
+                                  : (const void*)k_linattn<T, DK, NW, false, false>);
+    return linattn_launch(f, a, NW, sizeof(Lds<T, DK, NW>), st);
+}
+
+template <class T, int DK>
+hipError_t launch_dk(const LinAttnArgs& a, bool full, hipStream_t st) {
+    if constexpr (DK > 128) {
+        return launch_one<T, DK, 4>(a, full, st);
+    } else {
+        switch (linattn_waves(a.dk, a.dv)) {
+            case 4: return launch_one<T, DK, 4>(a, full, st);
+            case 6: return launch_one<T, DK, 6>(a, full, st);
+            default: return launch_one<T, DK, 8>(a, full, st);
+        }
+    }
+}
+
+template <class T>
+hipError_t launch(const LinAttnArgs& a, bool full, hipStream_t st) {
+    if (a.dk <= 32) return launch_dk<T, 32>(a, full, st);
+    if (a.dk <= 64) return launch_dk<T, 64>(a, full, st);
+    if (a.dk <= 96) return launch_dk<T, 96>(a, full, st);
+    if (a.dk <= 128) return launch_dk<T, 128>(a, full, st);
+    return launch_dk<T, 256>(a, full, st);
+}
+
+}  // namespace chunk
+}  // namespace ssla

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <cstdlib>
 #include <exception>
 #include <string>
 
@@ -88,10 +89,14 @@ int check_linattn(const SslaHipLinAttn* d, bool step, const char* fn) {
     return SSLA_OK;
 }
 
-// 16-byte pieces: the address, both strides and the row's end are whole pieces.
+// Rows that buffer loads of 16-byte pieces can take: the address, both strides
+// and the row's end are whole pieces, rows are apart (what lies past a chunk's
+// last row must lie past the buffer's end) and 64 of them span less than 2^31
+// bytes.
 bool pieces(const void* p, const long long* s, long long width, size_t e) {
     const long long n = 16 / (long long)e;
-    return aligned(p, 16) && s[0] % n == 0 && s[1] % n == 0 && width % n == 0;
+    return aligned(p, 16) && s[0] % n == 0 && s[1] % n == 0 && width % n == 0 && s[0] >= width &&
+           s[0] < (1 << 22);
 }
 
 // Segment length.  A workgroup takes one segment of a head; cutting a
@@ -100,7 +105,7 @@ bool pieces(const void* p, const long long* s, long long width, size_t e) {
 // would leave the 256 CUs idle.
 void cut(const SslaHipLinAttn* d, LinAttnArgs& a) {
     const long long rows = d->n_tokens * d->heads * a.slices;
-    constexpr long long kWant = 512;
+    const char* kw = getenv("LA_WANT"); const long long kWant = kw ? atoll(kw) : 512;
     int shift = 8;
     while ((rows >> shift) > kWant) ++shift;
     if (a.max_len <= (1ll << shift)) shift = 31;       // no sequence is cut
@@ -127,12 +132,11 @@ LinAttnArgs linattn_args(const SslaHipLinAttn* d) {
     a.n_seqs = d->n_seqs, a.n_slots = d->n_slots;
     a.max_len = (int)(d->max_len < d->n_tokens ? d->max_len : d->n_tokens);
     a.heads = d->heads, a.rep = d->heads / d->qk_heads, a.dk = d->dk, a.dv = d->dv;
-    const int cols = 32 * linattn_waves(d->dv);
+    const int cols = 16 * linattn_waves(d->dk, d->dv);
     a.slices = (d->dv + cols - 1) / cols;
     const size_t e = element(d->dtype);
-    a.vec_in = pieces(d->q, d->q_stride, d->dk, e) && pieces(d->k, d->k_stride, d->dk, e) &&
-               pieces(d->v, d->v_stride, d->dv, e);
-    a.vec_out = aligned(d->out, 4 * e) && d->out_stride[0] % 4 == 0 && d->out_stride[1] % 4 == 0 && d->dv % 4 == 0;
+    a.vec = pieces(d->q, d->q_stride, d->dk, e) && pieces(d->k, d->k_stride, d->dk, e) &&
+            pieces(d->v, d->v_stride, d->dv, e) && pieces(d->out, d->out_stride, d->dv, e);
     a.scale = d->scale;
     return a;
 }

@@ -16,6 +16,7 @@
 namespace ssla {
 
 constexpr int kLinAttnMaxDim = 256;      // dk, dv
+constexpr int kCUs = 256;                 // compute units
 constexpr float kMinLogDecay = -65536.0f;
 
 struct LinAttnArgs {
@@ -34,6 +35,7 @@ struct LinAttnArgs {
     int n_seqs, n_slots, max_len;
     int heads, rep, dk, dv, slices;       // rep: heads sharing q and k
     int seg_shift, n_segs;                // log2 of a segment's tokens; segments of the call
+    int by_length;                        // whole sequences of unlike lengths: see linattn_by_length
     int vec;                              // buffer loads of q, k, v and stores of out, in pieces
     float scale;
 };
@@ -55,11 +57,36 @@ __device__ __forceinline__ long long linattn_first(const LinAttnArgs& a, int s) 
 }
 #endif
 
+#ifdef __HIP_DEVICE_COMPILE__
+// Whole sequences (up to 64) of unlike lengths: the longest first, and every
+// second round of the compute units in the other direction, so that those
+// that share a compute unit are not all long.  48 sequences of 340 to 1531 tokens
+// with 16 heads, lengths repeating every 8: 172 -> 120 us.
+__device__ __forceinline__ int linattn_by_length(const LinAttnArgs& a, int j, int lane) {
+    const int n = a.n_seqs, per = a.heads * a.slices;
+    int len = 0;
+    if (lane < n) len = (int)(linattn_first(a, lane + 1) - linattn_first(a, lane));
+    int rank = 0;
+    for (int t = 0; t < n; ++t) {
+        const int other = __builtin_amdgcn_readlane(len, t);
+        rank += other > len || (other == len && t < lane);
+    }
+    const int round = per < kCUs ? kCUs / per : 1, r = j / round, end = min(n, (r + 1) * round);
+    const int want = r & 1 ? end - 1 - (j - r * round) : j;
+    return __ffsll((unsigned long long)__ballot(lane < n && rank == want)) - 1;
+}
+#endif
+
 __device__ __forceinline__ Segment linattn_segment(const LinAttnArgs& a, int j, int lane) {
     Segment g;
 #ifdef __HIP_DEVICE_COMPILE__
     long long len;
-    if (a.cu) {
+    if (a.by_length) {
+        g.seq = linattn_by_length(a, j, lane);
+        g.row = linattn_first(a, g.seq);
+        len = linattn_first(a, g.seq + 1) - g.row;
+        g.index = 0;
+    } else if (a.cu) {
         // the last sequence whose first slot is at or before j, 64 candidates a round
         int lo = 0, n = a.n_seqs;
         while (n > 1) {

@@ -41,9 +41,9 @@ __device__ __forceinline__ double running_sum(double x) {
     return x;
 }
 
-constexpr int waves_per_simd(int dk, bool full) {
-    return dk > 128 ? 1 : full ? (dk <= 32 ? 4 : dk <= 64 ? 3 : 2) : (dk <= 96 ? 4 : 3);
-}
+// Waves of a SIMD that the chunked kernels' registers leave room for: four (two
+// workgroups of eight waves a compute unit) as far as that spills little.
+constexpr int waves_per_simd(int dk, int terms) { return dk > 128 ? 1 : terms == 3 && dk > 96 ? 2 : 4; }
 
 // Keeps a branch a branch: its body is not computed and selected every time.
 __device__ __forceinline__ void rare() { asm volatile(""); }
@@ -89,11 +89,17 @@ struct Place {
 
     // Whether there is anything to do.
     __device__ __forceinline__ bool find(const LinAttnArgs& a, bool full, int wave, int lane) {
-        const int per = a.heads * a.slices;
-        j_seg = blockIdx.x / per;
-        const int hs = blockIdx.x - j_seg * per;
-        head = hs / a.slices;
-        slice = hs - head * a.slices;
+        // Blocks go to the eight XCDs, each with an L2 of its own, in turn; those that
+        // read the same q and k (the heads that share them, the slices of a head)
+        // are put eight apart.
+        const int sharers = a.rep * a.slices, groups = a.heads / a.rep;
+        const int all = a.n_segs * groups, set = 8 * sharers;
+        const int at = blockIdx.x / set, width = min(8, all - 8 * at), in = blockIdx.x - at * set;
+        const int sharer = in / width, group = 8 * at + in - sharer * width;
+        j_seg = group / groups;
+        const int member = sharer / a.slices;
+        slice = sharer - member * a.slices;
+        head = (group - j_seg * groups) * a.rep + member;
         sg = linattn_segment(a, j_seg, lane);
         last = sg.t1 >= sg.len;
         if (!sg.ok || (!full && last)) return false;       // nothing follows the last segment

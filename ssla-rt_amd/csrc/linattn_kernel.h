@@ -111,9 +111,9 @@ template <class T> struct Token;
 template <class T> struct Token16 {
     typedef T V8 __attribute__((ext_vector_type(8)));
     template <int W> static constexpr int stride() { return W + pad(W); }
-    // column m of the wave's 16 columns at `col`, tokens t + 4 g .. and t + 16 + 4 g ..
-    template <int VS> static __device__ __forceinline__ V8 column(const T* v, int t, int col, int m, int g) {
-        const T* p = &v[(t + 4 * g + (m >> 2)) * VS + col + 4 * (m & 3)];
+    // column m of the wave's 16 columns at `col`, tokens 4 g .. and 16 + 4 g ..
+    template <int VS> static __device__ __forceinline__ V8 column(const T* v, int col, int m, int g) {
+        const T* p = &v[(4 * g + (m >> 2)) * VS + col + 4 * (m & 3)];
         return __builtin_bit_cast(V8, join(tr4(p), tr4(p + 16 * VS)));
     }
     static __device__ __forceinline__ f8 wide(V8 x) { return __builtin_convertvector(x, f8); }
@@ -132,10 +132,10 @@ template <> struct Token<float> {
     typedef f8 V8;
     static constexpr int TERMS = 3;
     template <int W> static constexpr int stride() { return W + 4; }     // four rows 16 banks apart
-    template <int VS> static __device__ __forceinline__ f8 column(const float* v, int t, int col, int m, int g) {
+    template <int VS> static __device__ __forceinline__ f8 column(const float* v, int col, int m, int g) {
         f8 x;
         #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = v[(t + (i >> 2) * 16 + 4 * g + (i & 3)) * VS + col + m];
+        for (int i = 0; i < 8; ++i) x[i] = v[((i >> 2) * 16 + 4 * g + (i & 3)) * VS + col + m];
         return x;
     }
     static __device__ __forceinline__ f8 wide(f8 x) { return x; }
@@ -143,24 +143,20 @@ template <> struct Token<float> {
 };
 
 // Whether any of a lane's values is an infinity or NaN.
-template <class T, int N, class V8>
-__device__ __forceinline__ bool odd_values(const V8 (&v)[N]) {
+template <class T, class V8>
+__device__ __forceinline__ bool odd_values(V8 v) {
     if constexpr (sizeof(T) == 2) {
+        const u4 w = __builtin_bit_cast(u4, v);
         us2 most = {0, 0};                     // largest exponents of two interleaved sets
         #pragma unroll
-        for (int s = 0; s < N; ++s)
-            #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                most = __builtin_elementwise_max(
-                    most, __builtin_bit_cast(us2, __builtin_bit_cast(u4, v[s])[i] & Token<T>::EXP));
+        for (int i = 0; i < 4; ++i)
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, w[i] & Token<T>::EXP));
         const unsigned short ex = (unsigned short)Token<T>::EXP;
         return most[0] == ex || most[1] == ex;
     } else {
         unsigned most = 0;
         #pragma unroll
-        for (int s = 0; s < N; ++s)
-            #pragma unroll
-            for (int i = 0; i < 8; ++i) most = max(most, __builtin_bit_cast(unsigned, (float)v[s][i]) & 0x7f800000u);
+        for (int i = 0; i < 8; ++i) most = max(most, __builtin_bit_cast(unsigned, (float)v[i]) & 0x7f800000u);
         return most == 0x7f800000u;
     }
 }
@@ -181,12 +177,17 @@ __device__ __forceinline__ void piece_terms(u4 x, int part, u2 (&t)[Token<T>::TE
     }
 }
 
+// Tokens of a chunk, one step of the contractions over tokens.  Chunks of 64 halve
+// the conversions of the state and the barriers, but take twice the registers and
+// LDS: with half the waves on a compute unit they were slower (fp32, 16 x 2000
+// tokens of 4 heads of 96: 72 against 61 us; bf16, 8192 tokens of 16 heads of 128:
+// 53 against 45) but where there is one workgroup a compute unit anyway (16 x 8192:
+// 716 against 738).
+constexpr int C = 32;
+
 template <class T, int DK, int NW>
 struct Lds {
     static constexpr int TERMS = Token<T>::TERMS, PT = TERMS == 3 ? 3 : 2;       // PT: terms of P and S
-    // Tokens of a chunk: 64, or 32 where 64 would take a compute unit's LDS alone
-    // (three terms: 133 KB for dk = dv = 96) or not fit it (fp16, dk = 256: 171 KB).
-    static constexpr int C = TERMS == 3 || (TERMS == 2 && DK > 128) ? 32 : 64;
     static constexpr int DV = 16 * NW;
     static constexpr int QS = DK + pad(DK), PS = C + pad(C), VS = Token<T>::template stride<DV>();
     __bf16 q[TERMS][C * QS];     // columns in operand order
@@ -197,13 +198,13 @@ struct Lds {
 };
 
 template <class T, int DK, int NW, bool FULL, bool VEC>
-__global__ __launch_bounds__(64 * NW, waves_per_simd(DK, FULL)) void k_linattn(const LinAttnArgs a) {
+__global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void k_linattn(const LinAttnArgs a) {
     typedef Token<T> Tk;
     typedef typename Tk::V8 V8;
     typedef Lds<T, DK, NW> L;
-    constexpr int NT = 64 * NW, TERMS = L::TERMS, PT = L::PT, C = L::C;
+    constexpr int NT = 64 * NW, TERMS = L::TERMS, PT = L::PT;
     constexpr int DT = DK / 16, KS = DK / 32;              // tiles, steps along d
-    constexpr int IT = C / 16, CS = C / 32;                // tiles, steps along tokens
+    constexpr int IT = C / 16;                             // tiles along tokens
     constexpr int OUT_ORDER = PT - 1;                      // highest order of terms' products kept
     extern __shared__ __align__(16) char smem[];
     L& lds = *reinterpret_cast<L*>(smem);
@@ -271,11 +272,10 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, FULL)) void k_linattn(c
 
         f4 O[IT];
         if (FULL) {
-            // ---- P^T = K Q^T: the tiles on and below the diagonal ------------
-            for (int u = wave; u < IT * (IT + 1) / 2; u += NW) {
-                const int it = u >= 6 ? 3 : u >= 3 ? 2 : u >= 1 ? 1 : 0;
-                const int jt = u - it * (it + 1) / 2;
-                f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            // ---- P^T = K Q^T: the three tiles on and below the diagonal -------
+            if (wave < 3) {
+                const int it = wave >= 1 ? 1 : 0, jt = wave - it;
+                f4 acc[2] = {};                // two chains: a product waits for the one before it
                 constexpr int KH = TERMS > 1 ? 1 : KS > 4 ? 4 : KS;              // steps in flight
                 #pragma unroll
                 for (int s0 = 0; s0 < KS; s0 += KH) {
@@ -295,14 +295,18 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, FULL)) void k_linattn(c
                         for (int i = 0; i < TERMS; ++i)
                             #pragma unroll
                             for (int j = 0; j < TERMS; ++j)
-                                if (i + j <= OUT_ORDER) acc = mma(ka[s][i], qa[s][j], acc);
+                                if (i + j <= OUT_ORDER) {
+                                    f4& c = acc[TERMS == 1 ? s & 1 : j & 1];
+                                    c = mma(ka[s][i], qa[s][j], c);
+                                }
                 }
+                acc[0] += acc[1];
                 const int i = 16 * it + m, j = 16 * jt + 4 * g;
                 const f4 jh = *(const f4*)&lds.b[buf].hi[j], jl = *(const f4*)&lds.b[buf].lo[j];
                 const float ih = lds.b[buf].hi[i], il = lds.b[buf].lo[i];
                 f4 p;
                 #pragma unroll
-                for (int r = 0; r < 4; ++r) p[r] = acc[r] * (a.scale * exp2_((ih - jh[r]) + (il - jl[r])));
+                for (int r = 0; r < 4; ++r) p[r] = acc[0][r] * (a.scale * exp2_((ih - jh[r]) + (il - jl[r])));
                 if (it == jt)
                     #pragma unroll
                     for (int r = 0; r < 4; ++r) p[r] = j + r <= i ? p[r] : 0.0f;
@@ -314,18 +318,14 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, FULL)) void k_linattn(c
             // ---- O^T = S^T Q^T ------------------------------------------------
             #pragma unroll
             for (int it = 0; it < IT; ++it) O[it] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-            bf8 qa[2][IT][TERMS];
-            auto read_q = [&](int s) {
+            #pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                bf8 qa[IT][TERMS];
                 #pragma unroll
                 for (int it = 0; it < IT; ++it)
                     #pragma unroll
                     for (int i = 0; i < TERMS; ++i)
-                        qa[s & 1][it][i] = *(const bf8*)&lds.q[i][(16 * it + m) * L::QS + 32 * s + 8 * g];
-            };
-            read_q(0);
-            #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                if (s + 1 < KS) read_q(s + 1);
+                        qa[it][i] = *(const bf8*)&lds.q[i][(16 * it + m) * L::QS + 32 * s + 8 * g];
                 loads_stay_above();
                 bf8 sa[PT];
                 split(join(S[2 * s], S[2 * s + 1]), sa);
@@ -335,15 +335,13 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, FULL)) void k_linattn(c
                     for (int i = 0; i < TERMS; ++i)
                         if (h + i <= OUT_ORDER)
                             #pragma unroll
-                            for (int it = 0; it < IT; ++it) O[it] = mma(sa[h], qa[s & 1][it][i], O[it]);
+                            for (int it = 0; it < IT; ++it) O[it] = mma(sa[h], qa[it][i], O[it]);
             }
             #pragma unroll
             for (int it = 0; it < IT; ++it) O[it] *= lds.b[buf].eb[16 * it + m];
         }
         // v^T of the wave's columns
-        V8 vf[CS];
-        #pragma unroll
-        for (int s = 0; s < CS; ++s) vf[s] = Tk::template column<L::VS>(lds.v, 32 * s, 16 * wave, m, g);
+        V8 vf = Tk::template column<L::VS>(lds.v, 16 * wave, m, g);
         if (FULL) __syncthreads();             // P is whole
         // An infinity or NaN of v must not reach the rows before it through their
         // zeros of P: it is taken out here, and its column set to NaN from its
@@ -353,42 +351,30 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, FULL)) void k_linattn(c
         if (any_bad) {
             rare();
             #pragma unroll
-            for (int s = CS - 1; s >= 0; --s)
-                #pragma unroll
-                for (int i = 7; i >= 0; --i)
-                    if (not_finite((float)vf[s][i])) {
-                        bad = 32 * s + (i >> 2) * 16 + 4 * g + (i & 3);
-                        vf[s][i] = 0;
-                    }
+            for (int i = 7; i >= 0; --i)
+                if (not_finite((float)vf[i])) {
+                    bad = (i >> 2) * 16 + 4 * g + (i & 3);
+                    vf[i] = 0;
+                }
             bad = min(bad, __shfl_xor(bad, 16));
             bad = min(bad, __shfl_xor(bad, 32));
         }
 
         if (FULL) {
             // ---- O^T += V^T P^T -------------------------------------------------
-            // (token tile, step): the tiles of the second step take both
-            constexpr int NU = CS == 2 ? 6 : 2;
-            constexpr int PU[6][2] = {{0, 0}, {1, 0}, {2, 0}, {3, 0}, {2, 1}, {3, 1}};
-            bf8 pa[2][PT], vt[CS][TERMS];
-            auto read_p = [&](int u) {
-                #pragma unroll
-                for (int h = 0; h < PT; ++h)
-                    pa[u & 1][h] = *(const bf8*)&lds.p[h][(16 * PU[u][0] + m) * L::PS + 32 * PU[u][1] + 8 * g];
-            };
-            read_p(0);
+            bf8 vt[TERMS], pa[IT][PT];
             #pragma unroll
-            for (int s = 0; s < CS; ++s) Tk::terms(vf[s], vt[s]);
-            #pragma unroll
-            for (int u = 0; u < NU; ++u) {
-                if (u + 1 < NU) read_p(u + 1);
-                loads_stay_above();
-                const int it = PU[u][0], s = PU[u][1];
+            for (int it = 0; it < IT; ++it)
                 #pragma unroll
-                for (int h = 0; h < PT; ++h)
-                    #pragma unroll
-                    for (int i = 0; i < TERMS; ++i)
-                        if (h + i <= OUT_ORDER) O[it] = mma(vt[s][i], pa[u & 1][h], O[it]);
-            }
+                for (int h = 0; h < PT; ++h) pa[it][h] = *(const bf8*)&lds.p[h][(16 * it + m) * L::PS + 8 * g];
+            Tk::terms(vf, vt);
+            #pragma unroll
+            for (int h = 0; h < PT; ++h)
+                #pragma unroll
+                for (int i = 0; i < TERMS; ++i)
+                    if (h + i <= OUT_ORDER)
+                        #pragma unroll
+                        for (int it = 0; it < IT; ++it) O[it] = mma(vt[i], pa[it][h], O[it]);
             if (any_bad) {
                 rare();
                 #pragma unroll
@@ -424,33 +410,29 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, FULL)) void k_linattn(c
         const float eC = lds.b[buf].end;
         decay *= eC;
         if (!FULL || !pl.last || t + C < sg.t1 || a.s_out) {
-            bf8 ka[2][TERMS];                  // k^T of a tile of d and a step of tokens
-            auto read_k = [&](int s, int dt) {
-                #pragma unroll
-                for (int i = 0; i < TERMS; ++i) {
-                    const __bf16* p = &lds.k[i][(32 * s + 4 * g + (m >> 2)) * L::QS + 16 * dt + 4 * (m & 3)];
-                    ka[dt & 1][i] = __builtin_bit_cast(bf8, join(tr4(p), tr4(p + 16 * L::QS)));
-                }
-            };
-            read_k(0, 0);
+            const float* w = &lds.b[buf].w[4 * g];
+            bf8 x[3];
+            split(Tk::wide(vf) * join(*(const f4*)w, *(const f4*)(w + 16)), x);
             #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) S[dt] *= eC;
-            #pragma unroll
-            for (int s = 0; s < CS; ++s) {
-                const float* w = &lds.b[buf].w[32 * s + 4 * g];
-                bf8 x[3];
-                split(Tk::wide(vf[s]) * join(*(const f4*)w, *(const f4*)(w + 16)), x);
+            for (int dt = 0; dt < DT; dt += 2) {           // two chains: a product waits for the one before it
+                bf8 ka[2][TERMS];              // k^T of two tiles of d
                 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    if (dt + 1 < DT) read_k(s, dt + 1);
-                    else if (s + 1 < CS) read_k(s + 1, 0);
-                    loads_stay_above();
+                for (int y = 0; y < 2; ++y) {
                     #pragma unroll
-                    for (int h = 0; h < 3; ++h)
-                        #pragma unroll
-                        for (int i = 0; i < TERMS; ++i)
-                            if (h + i <= 2) S[dt] = mma(ka[dt & 1][i], x[h], S[dt]);
+                    for (int i = 0; i < TERMS; ++i) {
+                        const __bf16* p = &lds.k[i][(4 * g + (m >> 2)) * L::QS + 16 * (dt + y) + 4 * (m & 3)];
+                        ka[y][i] = __builtin_bit_cast(bf8, join(tr4(p), tr4(p + 16 * L::QS)));
+                    }
+                    S[dt + y] *= eC;
                 }
+                loads_stay_above();
+                #pragma unroll
+                for (int h = 0; h < 3; ++h)
+                    #pragma unroll
+                    for (int i = 0; i < TERMS; ++i)
+                        if (h + i <= 2)
+                            #pragma unroll
+                            for (int y = 0; y < 2; ++y) S[dt + y] = mma(ka[y][i], x[h], S[dt + y]);
             }
             if (any_bad) {
                 rare();

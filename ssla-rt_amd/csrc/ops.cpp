@@ -3,7 +3,6 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
-#include <cstdlib>
 #include <exception>
 #include <string>
 
@@ -99,20 +98,27 @@ bool pieces(const void* p, const long long* s, long long width, size_t e) {
            s[0] < (1 << 22);
 }
 
-// Segment length.  A workgroup takes one segment of a head; cutting a
-// sequence costs its k and v a second reading and a state written, chained
-// and read for each segment, so sequences are cut only where whole ones
-// would leave the 256 CUs idle.
+// Segment length.  A workgroup takes one segment of a head; cutting a sequence
+// costs its k and v a second reading and a state written, chained and read for
+// each segment.  Whole sequences are taken while none holds more than one and a
+// half of a compute unit's share of all tokens and heads (16 sequences of 8192
+// tokens, 16 heads of 128, one workgroup a compute unit: 0.74 ms whole, 0.95 cut
+// in two).  Else segments are the smallest power of two, from 256 tokens on, that
+// leaves each of the 256 compute units two (one sequence of 8192: 0.087 ms; with
+// one each 0.088).
 void cut(const SslaHipLinAttn* d, LinAttnArgs& a) {
     const long long rows = d->n_tokens * d->heads * a.slices;
-    const char* kw = getenv("LA_WANT"); const long long kWant = kw ? atoll(kw) : 512;
     int shift = 8;
-    while ((rows >> shift) > kWant) ++shift;
-    if (a.max_len <= (1ll << shift)) shift = 31;       // no sequence is cut
-    a.seg_shift = shift;
-    if (shift == 31)
+    while ((rows >> shift) > 2 * kCUs) ++shift;
+    if (a.max_len <= (1ll << shift) || 2 * kCUs * (long long)a.max_len <= 3 * rows) {
+        a.seg_shift = 31;                              // no sequence is cut
         a.n_segs = d->n_seqs;
-    else if (d->cu_seqlens)
+        a.by_length = d->cu_seqlens && d->n_seqs > 1 && d->n_seqs <= 64 &&
+                      (long long)d->n_seqs * a.max_len > d->n_tokens;
+        return;
+    }
+    a.seg_shift = shift;
+    if (d->cu_seqlens)
         a.n_segs = (int)((d->n_tokens >> shift) + d->n_seqs);
     else
         a.n_segs = d->n_seqs * (int)((a.max_len + (1ll << shift) - 1) >> shift);

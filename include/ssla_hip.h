@@ -441,7 +441,9 @@ int ssla_hip_oeva_diff(const char* path_a, const char* path_b, double tol_abs,
  * Every call only queues kernels on `stream` (hipStream_t or NULL): it
  * allocates nothing, copies nothing to the host, waits for nothing and keeps
  * nothing between calls, so it may be captured into a HIP graph.  A workspace
- * belongs to one call (or captured graph) at a time. */
+ * belongs to one call (or captured graph) at a time.  Tokens, rows and channels
+ * are counted up to 2^31 - 2^16; a call that would need a grid of 2^32 threads
+ * is refused.  There is no backward pass: nothing here is trained. */
 #define SSLA_F32  0
 #define SSLA_BF16 1
 #define SSLA_F16  2
@@ -521,8 +523,7 @@ int ssla_hip_linattn_step(const SslaHipLinAttn* d, void* stream);
  *     out = act(y), or y * act(gate) where gate is set
  * Element (item, row, c) of x lies at item * stride[0] + row * stride[1] + c
  * (elements, >= 0), of gate and out likewise.  weight and bias (NULL: 1 and 0)
- * have the type of x.  Moments are fp32, merged from exact differences (no
- * difference of large sums), out is rounded once.  out may be x or gate itself,
+ * have the type of x.  Sums of squares are 64 bits wide, out is rounded once.  out may be x or gate itself,
  * else it must not overlap an input.  A NaN or infinity reaches its own
  * group of its own item only. */
 typedef struct SslaHipGroupNorm {

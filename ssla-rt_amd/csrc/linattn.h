@@ -4,7 +4,8 @@
 //   S_t = exp(g_t) S_{t-1} + k_t v_t^T,     o_t = scale q_t^T S_t     (S: dk x dv)
 //
 // A workgroup runs one segment of one sequence for one head and one slice of
-// the dv columns, chunk by chunk with the state in registers (linattn_kernel.h).  Sequences longer than a segment take three launches: the
+// the dv columns, chunk by chunk with the state in registers
+// (linattn_kernel.h).  Sequences longer than a segment take three launches: the
 // segments' own states from zero (FULL = false), the states before each
 // segment (k_linattn_chain), then every segment from its state (FULL = true).
 #pragma once

@@ -19,7 +19,7 @@ __global__ __launch_bounds__(256) void k_linattn_chain(const LinAttnArgs a) {
         const long long len = linattn_first(a, seq + 1) - first;
         const int l = (int)(len < 0 ? 0 : len > a.max_len ? a.max_len : len);
         j = (int)(first >> a.seg_shift) + seq;
-        n = (l + (1 << a.seg_shift) - 1) >> a.seg_shift;
+        n = (int)(((unsigned)l + (1u << a.seg_shift) - 1) >> a.seg_shift);
 #endif
     } else {
         n = a.n_segs / a.n_seqs;

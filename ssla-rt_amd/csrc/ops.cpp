@@ -36,7 +36,13 @@ bool apart(long long n0, long long s0, long long n1, long long s1, long long wid
     return s1 >= width && (s0 - width) / s1 >= n1 - 1;
 }
 
-constexpr long long kMaxBlocks = 0x7fffffff;
+// Whether a launch of a * b * c workgroups fits: HIP counts a grid's threads in 32 bits.
+bool launchable(long long a, long long b, long long c, int threads) {
+    return (__int128)a * b * c <= 0xffffffffll / threads;
+}
+
+// Kernels count tokens, rows and channels in 32 bits and step past the last one.
+constexpr int kMaxCount = 0x7fff0000;
 constexpr long long kMaxStride = 1ll << 40;      // offsets stay within 64 bits
 
 // ---- linear attention ----------------------------------------------------------
@@ -57,8 +63,8 @@ int check_linattn(const SslaHipLinAttn* d, bool step, const char* fn) {
             return refuse(f + "strides must be 0 .. 2^40");
     long long tokens = d->n_seqs;
     if (!step) {
-        if (d->n_tokens < 0 || d->n_tokens > 0x7fffffff || d->max_len < 0)
-            return refuse(f + "n_tokens and max_len must be 0 .. 2^31 - 1");
+        if (d->n_tokens < 0 || d->n_tokens > kMaxCount || d->max_len < 0)
+            return refuse(f + "n_tokens must be 0 .. 2^31 - 2^16, max_len not negative");
         if (!d->cu_seqlens && d->n_tokens != (long long)d->n_seqs * d->max_len)
             return refuse(f + "without cu_seqlens n_tokens must be n_seqs * max_len");
         tokens = d->n_tokens;
@@ -68,6 +74,7 @@ int check_linattn(const SslaHipLinAttn* d, bool step, const char* fn) {
         if (!d->q || !d->k || !d->v || !d->log_decay || !d->out) return refuse(f + "null tensor");
         if (!apart(tokens, d->out_stride[0], d->heads, d->out_stride[1], d->dv))
             return refuse(f + "rows of out overlap");
+        if (d->out == d->q || d->out == d->k || d->out == d->v) return refuse(f + "out is an input");
     }
     if (!aligned(d->q, e) || !aligned(d->k, e) || !aligned(d->v, e) || !aligned(d->out, e) ||
         !aligned(d->log_decay, 4) || !aligned(d->cu_seqlens, 4) || !aligned(d->slots, 4) ||
@@ -105,8 +112,8 @@ bool pieces(const void* p, const long long* s, long long width, size_t e) {
 // tokens, 16 heads of 128, one workgroup a compute unit: 0.74 ms whole, 0.95 cut
 // in two).  Else segments are the smallest power of two, from 256 tokens on, that
 // leaves each of the 256 compute units two (one sequence of 8192: 0.087 ms; with
-// one each 0.088).
-void cut(const SslaHipLinAttn* d, LinAttnArgs& a) {
+// one each 0.088).  False where the segments cannot be counted.
+bool cut(const SslaHipLinAttn* d, LinAttnArgs& a) {
     const long long rows = d->n_tokens * d->heads * a.slices;
     int shift = 8;
     while ((rows >> shift) > 2 * kCUs) ++shift;
@@ -115,13 +122,13 @@ void cut(const SslaHipLinAttn* d, LinAttnArgs& a) {
         a.n_segs = d->n_seqs;
         a.by_length = d->cu_seqlens && d->n_seqs > 1 && d->n_seqs <= 64 &&
                       (long long)d->n_seqs * a.max_len > d->n_tokens;
-        return;
+        return true;
     }
     a.seg_shift = shift;
-    if (d->cu_seqlens)
-        a.n_segs = (int)((d->n_tokens >> shift) + d->n_seqs);
-    else
-        a.n_segs = d->n_seqs * (int)((a.max_len + (1ll << shift) - 1) >> shift);
+    const long long segs = d->cu_seqlens ? (d->n_tokens >> shift) + d->n_seqs
+                                         : d->n_seqs * ((a.max_len + (1ll << shift) - 1) >> shift);
+    a.n_segs = (int)segs;
+    return segs <= 0x7fffffff;
 }
 
 LinAttnArgs linattn_args(const SslaHipLinAttn* d) {
@@ -160,6 +167,8 @@ int check_group_norm(const SslaHipGroupNorm* d) {
     if (d->dtype != SSLA_F32 && d->dtype != SSLA_BF16 && d->dtype != SSLA_F16)
         return refuse(f + "dtype must be SSLA_F32, SSLA_BF16 or SSLA_F16");
     if (d->n < 0 || d->rows < 0 || d->channels < 0) return refuse(f + "negative size");
+    if (d->rows > kMaxCount || d->channels > kMaxCount)
+        return refuse(f + "rows and channels must be at most 2^31 - 2^16");
     if (d->groups < 1 || d->channels % d->groups) return refuse(f + "groups must divide channels");
     if (d->act < SSLA_ACT_NONE || d->act > SSLA_ACT_RELU) return refuse(f + "unknown activation");
     if (!(d->eps >= 0.0f)) return refuse(f + "eps must not be negative");
@@ -221,7 +230,7 @@ int ssla_hip_linattn_workspace(const SslaHipLinAttn* d, size_t* nbytes) try {
     *nbytes = 0;
     if (const int rc = check_linattn(d, false, "ssla_hip_linattn_workspace")) return rc;
     LinAttnArgs a = linattn_args(d);
-    cut(d, a);
+    if (!cut(d, a)) return refuse("ssla_hip_linattn_workspace: too many sequences");
     *nbytes = linattn_bytes(a);
     return SSLA_OK;
 } catch (const std::exception&) {
@@ -232,11 +241,11 @@ int ssla_hip_linattn(const SslaHipLinAttn* d, void* workspace, size_t workspace_
     if (const int rc = check_linattn(d, false, "ssla_hip_linattn")) return rc;
     if (d->n_seqs == 0) return SSLA_OK;
     LinAttnArgs a = linattn_args(d);
-    cut(d, a);
-    if ((long long)a.n_segs * a.heads * a.slices > kMaxBlocks ||
-        (long long)a.n_seqs * a.heads * ((a.dk * a.dv + 255) / 256) > kMaxBlocks)
-        return refuse("ssla_hip_linattn: too many sequences and heads");
+    if (!cut(d, a)) return refuse("ssla_hip_linattn: too many sequences");
     const size_t need = linattn_bytes(a);
+    if (!launchable(a.n_segs, a.heads, a.slices, 64 * linattn_waves(a.dk, a.dv)) ||
+        (need && !launchable(a.n_seqs, a.heads, (a.dk * a.dv + 255) / 256, 256)))
+        return refuse("ssla_hip_linattn: too many sequences and heads");
     if (need) {
         if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
             return refuse("ssla_hip_linattn: the workspace is missing, too small or not 16-byte aligned");
@@ -261,7 +270,7 @@ int ssla_hip_linattn_step(const SslaHipLinAttn* d, void* stream) try {
     if (const int rc = check_linattn(d, true, "ssla_hip_linattn_step")) return rc;
     if (d->n_seqs == 0) return SSLA_OK;
     const LinAttnArgs a = linattn_args(d);
-    if ((long long)a.n_seqs * a.heads * ((a.dk * a.dv + 255) / 256) > kMaxBlocks)
+    if (!launchable(a.n_seqs, a.heads, 1, 256))
         return refuse("ssla_hip_linattn_step: too many sequences and heads");
     const hipError_t e = linattn_launch_step(a, d->dtype, (hipStream_t)stream);
     return e == hipSuccess ? SSLA_OK : hip_failed("ssla_hip_linattn_step", e);
@@ -284,7 +293,8 @@ int ssla_hip_group_norm(const SslaHipGroupNorm* d, void* workspace, size_t works
     if (!d->n || !d->rows || !d->channels) return SSLA_OK;
     GroupNormArgs a = group_norm_args(d);
     const size_t need = group_norm_bytes(a);
-    if ((long long)a.n * (a.parts ? a.parts : 1) * a.blocks > kMaxBlocks)
+    if (a.kind == kGroupLanes ? !launchable(a.n, a.groups, a.reps, 1)
+                              : !launchable(a.n, a.parts ? a.parts : 1, a.blocks, a.threads))
         return refuse("ssla_hip_group_norm: too many items and groups");
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return refuse("ssla_hip_group_norm: the workspace is missing, too small or not 16-byte aligned");

@@ -84,6 +84,32 @@ def test_many_sequences_are_found():
     assert torch.equal(out, out2)
 
 
+@pytest.mark.parametrize("n", [17, 24, 41, 64])
+def test_sequences_of_unlike_lengths(n):
+    """Short sequences in rounds of 16 (16 heads; the last round whole, partial,
+    in either direction), some empty, with states in other slots."""
+    lens = [(37 * i) % 61 for i in range(n)]
+    q, k, v, g = make(sum(lens), 16, 16, 16, 72, torch.bfloat16, 41)
+    slots = torch.arange(n - 1, -1, -1, dtype=torch.int32, device=DEV)
+    s0 = torch.randn(n, 16, 16, 72, device=DEV)
+    want = R.linear_attention(q, k, v, g, lens, 1.0, s0.flip(0))
+    out = ops().linear_attention(q, k, v, g, cu_seqlens=cu_of(lens), max_len=60, state_in=s0, state_out=s0,
+                                 slots=slots)
+    R.check_linear_attention(out, s0.flip(0), want, torch.bfloat16, 16, 60)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lens", [[700, 300], [300], [30, 40, 10, 20]], ids=str)
+def test_shared_heads_and_slices(dtype, lens):
+    """Heads that share q and k, columns in four slices, segments and heads that
+    do not fill eights: cut sequences and whole ones."""
+    t = R.TYPES[dtype]
+    q, k, v, g = make(sum(lens), 9, 3, 130, 200, t, 42)
+    s1 = torch.full((len(lens), 9, 130, 200), 7.0, device=DEV)
+    out = ops().linear_attention(q, k, v, g, scale=0.1, cu_seqlens=cu_of(lens), max_len=max(lens), state_out=s1)
+    R.check_linear_attention(out, s1, R.linear_attention(q, k, v, g, lens, 0.1), t, 130, max(lens))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("layout", ["fused", "heads_first", "odd_offset", "padded_rows"])
 def test_strides(dtype, layout):
@@ -199,6 +225,22 @@ def test_non_finite_values_reach_no_earlier_token(dtype, what, value):
         sbad[1, 1, :, 3] = True
     s = s1.cpu()
     assert not torch.isfinite(s[sbad]).any() and torch.isfinite(s[~sbad]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_nan_decay_reaches_no_earlier_token(dtype):
+    t, lens, at = R.TYPES[dtype], [20, 600, 30], 20 + 333
+    q, k, v, g = make(sum(lens), 2, 2, 32, 48, t, 43)
+    want = R.linear_attention(q, k, v, g, lens, 1.0)
+    g[at, 1] = float("nan")
+    s1 = torch.zeros(3, 2, 32, 48, device=DEV)
+    out = ops().linear_attention(q, k, v, g, cu_seqlens=cu_of(lens), state_out=s1).cpu()
+    bad = torch.zeros(sum(lens), 2, 48, dtype=torch.bool)
+    bad[at:620, 1] = True
+    assert not torch.isfinite(out[bad]).any() and torch.isnan(s1[1, 1]).all()
+    ref = [torch.where(bad, 0.0, x) for x in want[:2]] + [None, None]
+    R.check_linear_attention(torch.where(bad, 0.0, out), None, ref, t, 32, 600)
+    assert torch.isfinite(s1[[0, 2]]).all() and torch.isfinite(s1[1, 0]).all()
 
 
 def test_values_behind_a_sequence_are_not_read_into_it():

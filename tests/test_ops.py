@@ -49,15 +49,6 @@ def test_descriptor_layouts():
     lib.check(lib.load().ssla_hip_ops_layout(out, 2))
     assert list(out) == [ctypes.sizeof(abi.SslaHipLinAttn), ctypes.sizeof(abi.SslaHipGroupNorm)]
     assert lib.load().ssla_hip_ops_layout(out, 1) == abi.SSLA_ERR_ARG
-    # the packed form the Python calls send is the ctypes form
-    d = linattn(scale=0.25, cu_seqlens=P, slots=P + 64)
-    f = [getattr(d, n) for n, _ in d._fields_]
-    flat = [x for v in f for x in (list(v) if hasattr(v, "__len__") else [v])]
-    assert ops._LINATTN.pack(*flat) == bytes(d)
-    d = norm()
-    flat = [x for v in (getattr(d, n) for n, _ in d._fields_)
-            for x in (list(v) if hasattr(v, "__len__") else [v or 0])]
-    assert ops._NORM.pack(*flat) == bytes(d)
 
 
 BAD_BOTH = [dict(dtype=3), dict(dtype=-1), dict(heads=0), dict(qk_heads=0), dict(qk_heads=3),
@@ -67,9 +58,12 @@ BAD_BOTH = [dict(dtype=3), dict(dtype=-1), dict(heads=0), dict(qk_heads=0), dict
             dict(q=P + 1), dict(out=P + 1), dict(log_decay=P + 2), dict(slots=P + 2),
             dict(state_out=P + 3), dict(state_stride=4 * 32 * 64 - 1), dict(n_slots=1),
             dict(out_stride=[0, 64]), dict(out_stride=[256, 0]), dict(out_stride=[200, 64]),
-            dict(state_out=P + (5 << 24) + 4)]
+            dict(state_out=P + (5 << 24) + 4), dict(out=P), dict(out=P + (2 << 24))]
 BAD_PROMPT = [dict(n_tokens=-1), dict(n_tokens=1 << 31, cu_seqlens=P), dict(max_len=-1),
-              dict(n_tokens=21), dict(cu_seqlens=P + 1)]
+              dict(n_tokens=21), dict(cu_seqlens=P + 1),
+              dict(n_tokens=(1 << 31) - (1 << 16) + 1, cu_seqlens=P),
+              dict(n_tokens=(1 << 31) - (1 << 16), max_len=1 << 30, cu_seqlens=P, n_seqs=(1 << 31) - 1,
+                   state_in=None, state_out=None, heads=1, qk_heads=1)]
 
 
 @pytest.mark.parametrize("bad", BAD_BOTH + BAD_PROMPT, ids=str)
@@ -93,6 +87,22 @@ def test_linattn_refuses_nulls_and_missing_states():
         assert L.ssla_hip_linattn_step(ctypes.addressof(linattn(**bad)), None) == abi.SSLA_ERR_ARG
 
 
+def test_grids_that_cannot_be_launched_are_refused():
+    L, n = lib.load(), (1 << 31) - 1
+    for heads in (1, n):
+        d = linattn(n_seqs=n, heads=heads, qk_heads=1, n_tokens=0, max_len=0, n_slots=n, state_in=None,
+                    state_out=None)
+        assert L.ssla_hip_linattn(ctypes.addressof(d), None, 0, None) == abi.SSLA_ERR_ARG
+        assert b"too many" in L.ssla_hip_last_error()
+    d = linattn(n_seqs=1 << 24, n_slots=1 << 24, heads=1, qk_heads=1, state_out=P + (5 << 24))
+    assert L.ssla_hip_linattn_step(ctypes.addressof(d), None) == abi.SSLA_ERR_ARG
+    assert b"too many" in L.ssla_hip_last_error()
+    d = norm(n=1 << 24, rows=100, channels=64, groups=1, x_stride=[6400, 64], gate_stride=[6400, 64],
+             out_stride=[6400, 64], out=P + (1 << 45))
+    assert L.ssla_hip_group_norm(ctypes.addressof(d), None, 0, None) == abi.SSLA_ERR_ARG
+    assert b"too many" in L.ssla_hip_last_error()
+
+
 def test_linattn_workspace():
     """None for short sequences; a state for each piece of cut ones, refused when
     missing, too small or misaligned."""
@@ -111,7 +121,7 @@ def test_linattn_workspace():
 
 @pytest.mark.parametrize("bad", [
     dict(dtype=3), dict(n=-1), dict(rows=-1), dict(channels=-48), dict(groups=0), dict(groups=5),
-    dict(act=4), dict(act=-1), dict(eps=-1.0), dict(eps=float("nan")), dict(x=None), dict(out=None),
+    dict(act=4), dict(act=-1), dict(rows=0x7fff0001), dict(channels=0x7fff0001, groups=1), dict(eps=-1.0), dict(eps=float("nan")), dict(x=None), dict(out=None),
     dict(x=P + 2), dict(gate=P + 1), dict(weight=P + 1), dict(bias=P + 3), dict(out=P + 1),
     dict(x_stride=[-1, 48]), dict(gate_stride=[480, -1]), dict(out_stride=[480, 1 << 41]),
     dict(out_stride=[0, 48]), dict(out_stride=[480, 47]), dict(out_stride=[479, 48]),
@@ -153,6 +163,17 @@ def test_python_refuses_tensors_off_the_gpu():
         ops.group_norm(q, 2)
 
 
+def test_python_refuses_what_is_no_argument():
+    q = torch.zeros(5, 2, 8)
+    for f in (lambda: ops.linear_attention(q.numpy(), q, q, q), lambda: ops.group_norm(None, 2),
+              lambda: ops.linear_attention_step(q, q, q, q, None),
+              lambda: ops.group_norm(q, 2, act="gelu")):
+        with pytest.raises(ValueError):
+            f()
+    with pytest.raises(ValueError):            # the module itself
+        ops._ops.group_norm(q)
+
+
 @pytest.mark.gpu
 def test_python_refuses_wrong_tensors():
     D = "cuda"
@@ -182,7 +203,15 @@ def test_python_refuses_wrong_tensors():
            lambda: gn(q, 2, g), lambda: gn(q, 2, torch.zeros(8, device=D).half()),
            lambda: gn(q, 2, gate=v), lambda: gn(q, 2, out=v), lambda: gn(q.transpose(1, 2), 2),
            lambda: gn(torch.zeros(4, 5, 6, 8, device=D).transpose(1, 2), 2)]
+    grad = q.clone().requires_grad_()
+    bad += [lambda: la(grad, q, v, g), lambda: gn(grad, 2), lambda: la(q, q, v, g, n_seqs=1.5),
+            lambda: la(q, q, v, g, scale="1"), lambda: la(q, q, v, g, cu_seqlens=cu, max_len=-1),
+            lambda: la(q, q, v, g.to_sparse()), lambda: gn(q.to_sparse(), 2), lambda: st(q, q, v, g, s.to_sparse())]
     for i, f in enumerate(bad):
         with pytest.raises(ValueError):
             f()
             pytest.fail(f"call {i} was taken")
+    with pytest.raises(lib.SslaHipError, match="out"):
+        la(q, q, q, g[:2], q)
+    with torch.no_grad():
+        assert gn(grad, 2).shape == q.shape

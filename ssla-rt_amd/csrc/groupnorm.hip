@@ -6,7 +6,8 @@
 // to one piece of the row, so that its channels, weights and groups are fixed,
 // and steps over rows; neighbouring threads read neighbouring pieces.
 //   lanes      a group is small (a token's head): some lanes of a wave hold it,
-//              and nothing but shuffles joins them (k_group_lanes)
+//              and nothing but shuffles joins them; or a workgroup holds it
+//              (k_group_lanes)
 //   one pass   the item's rows fit in the workgroup's registers: x is read once
 //   two passes k_group<kStats> leaves each part's sums in the workspace,
 //              k_group<kApply> adds them up and reads x again (from the 256 MB
@@ -274,15 +275,32 @@ __global__ __launch_bounds__(NT) void k_group(const GroupNormArgs a) {
     }
 }
 
+// Pieces a thread of a 1024-thread workgroup keeps: what 128 registers hold.
+template <int V> constexpr int kWideReps = V == 8 ? 2 : 4;
+
 // ---- small groups --------------------------------------------------------------
-// `w` lanes hold a group of one item, R pieces each; neighbouring lanes' groups
-// are neighbours.  The mean first, then the sum of squared differences from it.
-template <class T, int V, int R>
-__global__ __launch_bounds__(256) void k_group_lanes(const GroupNormArgs a) {
+// `w` threads hold a group of one item, R pieces each: some lanes of a wave, with
+// neighbouring lanes' groups neighbours, or (WHOLE) a workgroup.  The mean first, then the sum of squared differences from it.
+template <class S, int NT, bool WHOLE>
+__device__ __forceinline__ S group_sum(S s, int w, S* waves) {
+    for (int o = WHOLE ? 32 : w >> 1; o; o >>= 1) s += __shfl_xor(s, o);
+    if (WHOLE) {
+        if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = waves[0];
+        #pragma unroll
+        for (int i = 1; i < NT / 64; ++i) s += waves[i];
+    }
+    return s;
+}
+
+template <class T, int V, int R, int NT, bool WHOLE>
+__global__ __launch_bounds__(NT) void k_group_lanes(const GroupNormArgs a) {
     typedef Piece<T, V> P;
-    const int w = a.reps;                                    // lanes of a group
+    __shared__ double sums[NT / 64], squares[NT / 64];
+    const int w = WHOLE ? NT : a.reps;                       // threads of a group
     const int l = threadIdx.x & (w - 1);
-    const long long ig = (long long)blockIdx.x * (256 / w) + threadIdx.x / w;
+    const long long ig = (long long)blockIdx.x * (NT / w) + threadIdx.x / w;
     const long long item = ig / a.groups;
     const int group = (int)(ig - item * a.groups);
     const bool on = item < a.n;
@@ -318,7 +336,7 @@ __global__ __launch_bounds__(256) void k_group_lanes(const GroupNormArgs a) {
             for (int j = 0; j < o; ++j) t[j] += t[j + o];
         s += t[0];
     }
-    for (int o = w >> 1; o; o >>= 1) s += __shfl_xor(s, o);
+    s = group_sum<float, NT, WHOLE>(s, w, (float*)sums);
     const float mean = s * (float)a.inv_count;
     double q = 0.0;                                          // squares do not overflow
     #pragma unroll
@@ -330,7 +348,7 @@ __global__ __launch_bounds__(256) void k_group_lanes(const GroupNormArgs a) {
                 q = fma(d, d, q);
             }
         }
-    for (int o = w >> 1; o; o >>= 1) q += __shfl_xor(q, o);
+    q = group_sum<double, NT, WHOLE>(q, w, squares);
     const float rstd = 1.0f / sqrtf((float)(q * a.inv_count) + a.eps);
     #pragma unroll
     for (int k = 0; k < R; ++k) {
@@ -348,9 +366,6 @@ __global__ __launch_bounds__(256) void k_group_lanes(const GroupNormArgs a) {
     }
 }
 
-// Pieces a thread of a 1024-thread workgroup keeps: what 128 registers hold.
-template <int V> constexpr int kWideReps = V == 8 ? 2 : 4;
-
 // LDS of a workgroup of k_group: the groups' sums, and the larger of the threads'
 // sums (of every channel, where groups do not begin with pieces) and the table.
 size_t group_norm_lds(const GroupNormArgs& a, int threads, long long np) {
@@ -364,11 +379,14 @@ hipError_t launch(const GroupNormArgs& a, hipStream_t st) {
     if (a.kind == kGroupLanes) {
         GroupNormArgs args = a;
         void* pa[] = {&args};
-        const long long per = 256 / a.reps, wgs = ((long long)a.n * a.groups + per - 1) / per;
-        const void* f = a.threads == 1   ? (const void*)k_group_lanes<T, V, 1>
-                        : a.threads == 2 ? (const void*)k_group_lanes<T, V, 2>
-                                         : (const void*)k_group_lanes<T, V, 4>;
-        return hipLaunchKernel(f, dim3((unsigned)wgs), dim3(256), pa, 0, st);
+        const int nt = a.reps > 256 ? 1024 : 256;
+        const long long per = nt / a.reps, wgs = ((long long)a.n * a.groups + per - 1) / per;
+        const void* f = a.reps > 256  ? (const void*)k_group_lanes<T, V, kWideReps<V>, 1024, true>
+                        : a.reps > 64 ? (const void*)k_group_lanes<T, V, 4, 256, true>
+                        : a.threads == 1 ? (const void*)k_group_lanes<T, V, 1, 256, false>
+                        : a.threads == 2 ? (const void*)k_group_lanes<T, V, 2, 256, false>
+                                         : (const void*)k_group_lanes<T, V, 4, 256, false>;
+        return hipLaunchKernel(f, dim3((unsigned)wgs), dim3(nt), pa, 0, st);
     }
     GroupNormArgs args = a;
     void* pa[] = {&args};
@@ -430,6 +448,20 @@ void group_norm_plan(GroupNormArgs& a, int dtype) {
             a.gb = a.blocks = 1;
             return;
         }
+    // A workgroup for each larger group, while the 128-byte lines that its rows
+    // touch, which the groups beside it read again, are few: one item of 320 rows of
+    // 48 fp32 channels in 8 groups takes 4.9 us instead of 10.0 by whole rows, 32 of
+    // them (82 thousand lines) 6.2 instead of 10.5, 128 14 instead of 11; one of 4096
+    // rows of 96 channels in 24 groups (98 thousand) 9.8 instead of 10.6, two 13.1
+    // instead of 10.9.
+    const long long lines = (long long)a.n * a.groups * a.rows * (((long long)cg * e + 127) / 128);
+    if (lines <= 65536 && pieces <= 1024 * (v == 8 ? 2 : 4)) {
+        a.kind = kGroupLanes;
+        a.vec = v;
+        a.reps = pieces <= 1024 ? 256 : 1024;
+        a.gb = a.blocks = 1;
+        return;
+    }
     const int row = a.channels / a.vec;
     a.blocks = (row + 255) / 256;
     a.gb = (a.groups + a.blocks - 1) / a.blocks;

@@ -134,7 +134,11 @@ struct Place {
     }
 };
 
-// The state in registers, S[dt][r] = (16 dt + 4 g + r, column m) of lane 16 g + m.
+// The state in registers: S[dt][r] of lane 16 g + m is (d, column m) with the d of
+// two tiles such that a lane has eight neighbouring ones.
+__device__ __forceinline__ int state_row(int dt, int r, int g) {
+    return 16 * (dt & ~1) + 8 * g + 4 * (dt & 1) + r;
+}
 template <int DT, class P>
 __device__ __forceinline__ void read_state(f4 (&S)[DT], const P& pl, const LinAttnArgs& a, bool full, int m, int g) {
     const float* src = pl.source(a, full);
@@ -144,7 +148,7 @@ __device__ __forceinline__ void read_state(f4 (&S)[DT], const P& pl, const LinAt
         #pragma unroll
         for (int r = 0; r < 4; ++r)
             S[dt][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
-                                                     b, pl.state_at(a, 16 * dt + 4 * g + r, m), 0, 0));
+                                                     b, pl.state_at(a, state_row(dt, r, g), m), 0, 0));
 }
 template <int DT, class P>
 __device__ __forceinline__ void write_state(const f4 (&S)[DT], const P& pl, const LinAttnArgs& a, bool full, int m,
@@ -156,7 +160,7 @@ __device__ __forceinline__ void write_state(const f4 (&S)[DT], const P& pl, cons
         #pragma unroll
         for (int r = 0; r < 4; ++r)
             __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, (float)S[dt][r]), b,
-                                                  pl.state_at(a, 16 * dt + 4 * g + r, m), 0, 0);
+                                                  pl.state_at(a, state_row(dt, r, g), m), 0, 0);
 }
 
 // A tensor's rows of a chunk of C tokens on their way to LDS: W columns (the

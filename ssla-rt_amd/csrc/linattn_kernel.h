@@ -100,17 +100,18 @@ __device__ __forceinline__ s4 tr4(const void* p) {
 // a step, 32 s + 4 g .. and 32 s + 16 + 4 g .., lie together at 32 s + 8 g.
 __device__ __forceinline__ int operand_at(int i) { return (i & ~31) | (i & 12) << 1 | (i & 16) >> 2 | (i & 3); }
 
-// Elements behind a row of w (a multiple of 32) bf16 in LDS.  Rows then begin an odd
-// multiple of four of the 64 banks apart, and four in turn at least eight apart:
-// 16 rows' pieces of 8 or 16 bytes and 4 rows' 32 bytes (tr4) meet no bank twice.
-constexpr int pad(int w) { return w % 128 == 0 || w % 128 == 32 ? 24 : 8; }
+// Elements behind a row of bf16 in LDS (a multiple of 32): rows then begin an odd
+// multiple of 32 bytes apart modulo 64, at which 16 rows' 16-byte pieces are read
+// in 5.5 cycles a wave (9.4 at other steps; 8-byte pieces, straight or
+// transposed, take 7.5 to 8 at any).
+constexpr int kPad = 16;
 
 // Token types: terms of a value; how v lies in LDS, comes from there and is
 // searched for infinities and NaN.
 template <class T> struct Token;
 template <class T> struct Token16 {
     typedef T V8 __attribute__((ext_vector_type(8)));
-    template <int W> static constexpr int stride() { return W + pad(W); }
+    template <int W> static constexpr int stride() { return W + kPad; }
     // column m of the wave's 16 columns at `col`, tokens 4 g .. and 16 + 4 g ..
     template <int VS> static __device__ __forceinline__ V8 column(const T* v, int col, int m, int g) {
         const T* p = &v[(4 * g + (m >> 2)) * VS + col + 4 * (m & 3)];
@@ -189,8 +190,8 @@ template <class T, int DK, int NW>
 struct Lds {
     static constexpr int TERMS = Token<T>::TERMS, PT = TERMS == 3 ? 3 : 2;       // PT: terms of P and S
     static constexpr int DV = 16 * NW;
-    static constexpr int QS = DK + pad(DK), PS = C + pad(C), VS = Token<T>::template stride<DV>();
-    __bf16 q[TERMS][C * QS];     // columns in operand order
+    static constexpr int QS = DK + kPad, PS = C + kPad, VS = Token<T>::template stride<DV>();
+    __bf16 q[TERMS][C * QS];
     __bf16 k[TERMS][C * QS];
     T v[C * VS];
     __bf16 p[PT][C * PS];        // rows i, columns j in operand order
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void 
                 if (FULL) {
                     piece_terms<T>(rq.x[p], part, x);
                     #pragma unroll
-                    for (int i = 0; i < TERMS; ++i) *(u2*)&lds.q[i][row * L::QS + operand_at(c)] = x[i];
+                    for (int i = 0; i < TERMS; ++i) *(u2*)&lds.q[i][row * L::QS + c] = x[i];
                 }
             }
         }
@@ -284,8 +285,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void 
                     for (int s = 0; s < KH; ++s)
                         #pragma unroll
                         for (int i = 0; i < TERMS; ++i) {
-                            const __bf16* p = &lds.k[i][(16 * jt + m) * L::QS + 32 * (s0 + s) + 4 * g];
-                            ka[s][i] = __builtin_bit_cast(bf8, join(*(const s4*)p, *(const s4*)(p + 16)));
+                            ka[s][i] = *(const bf8*)&lds.k[i][(16 * jt + m) * L::QS + 32 * (s0 + s) + 8 * g];
                             qa[s][i] = *(const bf8*)&lds.q[i][(16 * it + m) * L::QS + 32 * (s0 + s) + 8 * g];
                         }
                     loads_stay_above();
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void 
                 for (int y = 0; y < 2; ++y) {
                     #pragma unroll
                     for (int i = 0; i < TERMS; ++i) {
-                        const __bf16* p = &lds.k[i][(4 * g + (m >> 2)) * L::QS + 16 * (dt + y) + 4 * (m & 3)];
+                        const __bf16* p = &lds.k[i][(4 * g + (m >> 2)) * L::QS + 16 * dt + 4 * y + 8 * (m & 3)];
                         ka[y][i] = __builtin_bit_cast(bf8, join(tr4(p), tr4(p + 16 * L::QS)));
                     }
                     S[dt + y] *= eC;

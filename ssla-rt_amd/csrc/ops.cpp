@@ -107,17 +107,22 @@ bool pieces(const void* p, const long long* s, long long width, size_t e) {
 
 // Segment length.  A workgroup takes one segment of a head; cutting a sequence
 // costs its k and v a second reading and a state written, chained and read for
-// each segment.  Whole sequences are taken while none holds more than one and a
-// half of a compute unit's share of all tokens and heads (16 sequences of 8192
-// tokens, 16 heads of 128, one workgroup a compute unit: 0.74 ms whole, 0.95 cut
-// in two).  Else segments are the smallest power of two, from 256 tokens on, that
-// leaves each of the 256 compute units two (one sequence of 8192: 0.087 ms; with
-// one each 0.088).  False where the segments cannot be counted.
+// each segment.  Whole sequences are taken where none is longer than 256 tokens
+// (200 tokens of 4 heads of 24: 11.9 us whole, 12.2 cut; 300 of 16 heads of 128:
+// 26 whole, 21 cut), and while none holds more than one and a half of a compute
+// unit's share of all tokens and heads (16 sequences of 8192 tokens, 16 heads of
+// 128, one workgroup a compute unit: 0.74 ms whole, 0.95 cut in two).  Else
+// segments are the smallest power of two, from 64 tokens on, that leaves a
+// sequence at most 128 (they are chained in turn: 20000 tokens of one head of 64,
+// 60 us in 313 segments, 38 in 79), and each of the 256 compute units two (one
+// sequence of 8192, 16 heads of 128: 83 us, with one each 85), or one and a half
+// where segments are shorter than 256 (2000 tokens of 16 heads of 128: 43 us in 500
+// workgroups, 35 in 250).  False where the segments cannot be counted.
 bool cut(const SslaHipLinAttn* d, LinAttnArgs& a) {
     const long long rows = d->n_tokens * d->heads * a.slices;
-    int shift = 8;
-    while ((rows >> shift) > 2 * kCUs) ++shift;
-    if (a.max_len <= (1ll << shift) || 2 * kCUs * (long long)a.max_len <= 3 * rows) {
+    int shift = 6;
+    while ((rows >> shift) > (shift < 8 ? kCUs + kCUs / 2 : 2 * kCUs) || (a.max_len >> shift) > 128) ++shift;
+    if (a.max_len <= 256 || a.max_len <= (1ll << shift) || 2 * kCUs * (long long)a.max_len <= 3 * rows) {
         a.seg_shift = 31;                              // no sequence is cut
         a.n_segs = d->n_seqs;
         a.by_length = d->cu_seqlens && d->n_seqs > 1 && d->n_seqs <= 64 &&

@@ -42,8 +42,13 @@ __device__ __forceinline__ double running_sum(double x) {
 }
 
 // Waves of a SIMD that the chunked kernels' registers leave room for: four (two
-// workgroups of eight waves a compute unit) as far as that spills little.
-constexpr int waves_per_simd(int dk, int terms) { return dk > 128 ? 1 : terms == 3 && dk > 96 ? 2 : 4; }
+// workgroups of eight or six waves a compute unit) as far as that spills little
+// (fp32, heads of 96: three waves' registers spill nothing, but then two workgroups
+// of six waves seldom fit, 72 against 60 us; bf16, heads of 256: 368 us with one,
+// 262 with two, but fp16 129 with one, 138 with two).
+constexpr int waves_per_simd(int dk, int terms) {
+    return dk > 128 ? terms == 1 ? 2 : 1 : terms == 3 && dk > 96 ? 2 : 4;
+}
 
 // Keeps a branch a branch: its body is not computed and selected every time.
 __device__ __forceinline__ void rare() { asm volatile(""); }

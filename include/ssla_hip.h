@@ -499,7 +499,8 @@ typedef struct SslaHipLinAttn {
 } SslaHipLinAttn;
 
 /* Bytes of workspace that ssla_hip_linattn needs for *d (0 where sequences
- * are not cut; it depends on dtype, heads, dk, dv, n_seqs, max_len, n_tokens). */
+ * are not cut; it depends on heads, dk, dv, n_seqs, max_len, n_tokens and
+ * whether there are cu_seqlens). */
 int ssla_hip_linattn_workspace(const SslaHipLinAttn* d, size_t* nbytes);
 /* Whole sequences, in chunks on the matrix cores.  `workspace` holds at
  * least ssla_hip_linattn_workspace bytes, 16-byte aligned (NULL if 0). */

@@ -2,10 +2,11 @@
 
   abi     numpy / ctypes mirrors of include/ssla_abi.h
   lib     ctypes binding of libssla_hip.so (include/ssla_hip.h)
+  ops     sequence operators on torch tensors: linear attention, group norm
   hybrid  device buffers, weight packing, HybridS2S3Config, drain calls
   stub    weight-directory generator (tools/make_ssla_stub.py schema)
   events  seeded synthetic event / ring-record streams
 """
 from . import abi, events, stub  # noqa: F401  (no GPU needed)
 
-__all__ = ["abi", "events", "stub", "lib", "hybrid"]
+__all__ = ["abi", "events", "stub", "lib", "hybrid", "ops"]

@@ -24,7 +24,7 @@ struct GroupNormArgs {
     int vec;                              // channels of a piece: 16 bytes where alignment allows
     int kind;                             // kGroupLanes, kGroupOnePass, kGroupTwoPass
     int threads, reps;                    // of a workgroup; pieces a thread keeps (one pass).  Lanes:
-                                          // pieces a lane keeps; lanes of a group
+                                          // pieces a lane keeps; lanes of a group (over 64: a workgroup)
     int gb, blocks, np;                   // groups of a workgroup; workgroups along the groups; pieces of
                                           // a workgroup's row
     int parts;                            // workgroups along the rows; 0: not two passes

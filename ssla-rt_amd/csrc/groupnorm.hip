@@ -320,8 +320,13 @@ __global__ __launch_bounds__(NT) void k_group_lanes(const GroupNormArgs a) {
             const int row = i / pr, p = (i - row * pr) * V;
             px[k] = *(const P*)(x + row * a.xr + p);
             if (gate) pg[k] = *(const P*)(gate + row * a.gr + p);
-            if (a.weight) pw[k] = *(const P*)((const T*)a.weight + (long long)group * cg + p);
-            if (a.bias) pb[k] = *(const P*)((const T*)a.bias + (long long)group * cg + p);
+            if (k && w % pr == 0) {                          // a thread's pieces have the same channels
+                pw[k] = pw[0];
+                pb[k] = pb[0];
+            } else {
+                if (a.weight) pw[k] = *(const P*)((const T*)a.weight + (long long)group * cg + p);
+                if (a.bias) pb[k] = *(const P*)((const T*)a.bias + (long long)group * cg + p);
+            }
         }
     }
     float s = 0.0f;
@@ -382,7 +387,8 @@ hipError_t launch(const GroupNormArgs& a, hipStream_t st) {
         const int nt = a.reps > 256 ? 1024 : 256;
         const long long per = nt / a.reps, wgs = ((long long)a.n * a.groups + per - 1) / per;
         const void* f = a.reps > 256  ? (const void*)k_group_lanes<T, V, kWideReps<V>, 1024, true>
-                        : a.reps > 64 ? (const void*)k_group_lanes<T, V, 4, 256, true>
+                        : a.reps > 64 ? a.threads > 1 ? (const void*)k_group_lanes<T, V, 4, 256, true>
+                                                      : (const void*)k_group_lanes<T, V, 1, 256, true>
                         : a.threads == 1 ? (const void*)k_group_lanes<T, V, 1, 256, false>
                         : a.threads == 2 ? (const void*)k_group_lanes<T, V, 2, 256, false>
                                          : (const void*)k_group_lanes<T, V, 4, 256, false>;
@@ -437,7 +443,20 @@ void group_norm_plan(GroupNormArgs& a, int dtype) {
     int v = a.vec;
     while (cg % v) v /= 2;
     const long long pieces = (long long)a.rows * (cg / v);
-    for (int r = 1; r <= 4; r *= 2)
+    // A workgroup for each larger group, while what its rows' 128-byte lines hold
+    // besides, which the groups beside it read again, is small: one item of 320 rows
+    // of 48 fp32 channels in 8 groups takes 4.3 us instead of 10.0 by whole rows, 64
+    // of them (17 MB besides) 9.2 instead of 10.7, 128 14 instead of 11; 4096 rows of
+    // 96 channels in 24 groups (11 MB) 9.8 instead of 10.6, two such items 13.1
+    // instead of 10.9.  Groups of whole lines: 256 tokens of 16384 fp32 channels in 8
+    // groups 10.8 instead of 65, 64 items of 64 rows of 2048 bf16 channels in 16
+    // groups 16.8 instead of 22.6 (4096 such items, 2 GB, 762 instead of 684).
+    // A piece a thread, or up to four (two) of 256 (1024) threads; more than 512
+    // groups keep to 256 threads (256 tokens of 65536 bf16 channels in 16 groups: 31
+    // us, with 1024 threads 60).
+    const long long rows = (long long)a.n * a.groups * a.rows, width = (long long)cg * e;
+    const bool few = rows * ((width + 127) / 128 * 128 - width) <= 8 << 20;
+    for (int r = 1; r <= (few ? 1 : 4); r *= 2)
         if (pieces <= 64 * r) {
             int w = 1;
             while (w * r < pieces) w *= 2;
@@ -448,17 +467,11 @@ void group_norm_plan(GroupNormArgs& a, int dtype) {
             a.gb = a.blocks = 1;
             return;
         }
-    // A workgroup for each larger group, while the 128-byte lines that its rows
-    // touch, which the groups beside it read again, are few: one item of 320 rows of
-    // 48 fp32 channels in 8 groups takes 4.9 us instead of 10.0 by whole rows, 32 of
-    // them (82 thousand lines) 6.2 instead of 10.5, 128 14 instead of 11; one of 4096
-    // rows of 96 channels in 24 groups (98 thousand) 9.8 instead of 10.6, two 13.1
-    // instead of 10.9.
-    const long long lines = (long long)a.n * a.groups * a.rows * (((long long)cg * e + 127) / 128);
-    if (lines <= 65536 && pieces <= 1024 * (v == 8 ? 2 : 4)) {
+    if (few && pieces <= 1024 * (v == 8 ? 2 : 4)) {
         a.kind = kGroupLanes;
         a.vec = v;
-        a.reps = pieces <= 1024 ? 256 : 1024;
+        a.threads = pieces <= 256 ? 1 : 4;
+        a.reps = pieces <= 256 || (pieces <= 1024 && (long long)a.n * a.groups > 512) ? 256 : 1024;
         a.gb = a.blocks = 1;
         return;
     }

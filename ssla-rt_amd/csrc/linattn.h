@@ -62,7 +62,7 @@ __device__ __forceinline__ long long linattn_first(const LinAttnArgs& a, int s) 
 // Whole sequences (up to 64) of unlike lengths: the longest first, and every
 // second round of the compute units in the other direction, so that those
 // that share a compute unit are not all long.  48 sequences of 340 to 1531 tokens
-// with 16 heads, lengths repeating every 8: 172 -> 120 us.
+// with 16 heads of 64, lengths repeating every 8: 166 -> 121 us.
 __device__ __forceinline__ int linattn_by_length(const LinAttnArgs& a, int j, int lane) {
     const int n = a.n_seqs, per = a.heads * a.slices;
     int len = 0;
@@ -137,7 +137,11 @@ hipError_t linattn_launch_f32(const LinAttnArgs& a, bool full, hipStream_t st);
 hipError_t linattn_launch_chain(const LinAttnArgs& a, hipStream_t st);
 hipError_t linattn_launch_step(const LinAttnArgs& a, int dtype, hipStream_t st);
 
-// Waves of a workgroup: each owns 16 columns of out.
+// Waves of a workgroup: each owns 16 columns of out, and all of a head's columns
+// share one reading of q and k where eight waves' are enough; idle waves cost more
+// than that (16 sequences of 2000 tokens: bf16, 16 heads of 64, four waves 104 us,
+// eight 136; fp32, 4 heads of 96, six 92, eight 99, four twice 136; bf16, 16 heads of
+// 128, eight 173, four twice 185).
 inline int linattn_waves(int dk, int dv) { return dk > 128 || dv <= 64 ? 4 : dv <= 96 ? 6 : 8; }
 
 // Launches a chunked kernel with `lds` bytes.  More than 64 KB of LDS has to be

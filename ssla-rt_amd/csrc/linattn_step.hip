@@ -6,6 +6,9 @@
 // neighbouring columns (16 bytes) and every `lanes`-th row, eight rows in
 // flight.  Rows' q and k wait in LDS, so that the state's first loads are out
 // before them; the products with q are summed over the row lanes through LDS.
+// 64 sequences of 16 heads of 128 x 128 (134 MB) take 23.4 us, 5.8 TB/s out of the
+// caches; 1021 of 8 heads of 96 x 80 (502 MB) 101 us, 5.0 TB/s, as a large copy; one
+// of 16 heads 5 us, which is the launch and two dependent loads.
 #include "linattn.h"
 
 namespace ssla {

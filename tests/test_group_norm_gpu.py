@@ -23,9 +23,11 @@ def make(shape, dtype, seed=0):
     return x, (1 + 0.3 * rnd(c)).to(dtype), (0.3 * rnd(c)).to(dtype), rnd(*shape).to(dtype)
 
 
-SHAPES = [((130, 30, 256), 4), ((600, 100, 24), 1), ((3, 16384), 8), ((40, 65536), 16),
-          ((1, 2000, 24), 3), ((40, 320, 48), 8), ((290, 70, 33), 11), ((1, 1, 1), 1), ((3, 7, 24), 4), ((2, 5, 3, 24), 24), ((1, 20, 16, 48), 8), ((5, 33), 3),
-          ((700, 96), 2), ((129, 2048), 16), ((2, 300, 40), 1), ((2, 1000, 30), 5), ((1, 6000, 48), 16),
+SHAPES = [((2, 24, 606), 1), ((2, 200, 128), 1), ((2, 1500, 9), 1), ((130, 30, 256), 4),
+          ((600, 100, 24), 1), ((3, 16384), 8), ((40, 65536), 16), ((1, 2000, 24), 3),
+          ((40, 320, 48), 8), ((290, 70, 33), 11), ((1, 1, 1), 1), ((3, 7, 24), 4),
+          ((2, 5, 3, 24), 24), ((1, 20, 16, 48), 8), ((5, 33), 3), ((700, 96), 2),
+          ((129, 2048), 16), ((2, 300, 40), 1), ((2, 1000, 30), 5), ((1, 6000, 48), 16),
           ((4, 2500, 96), 8), ((3, 64, 1000), 8), ((1, 30000, 8), 2), ((2, 4, 4096), 32),
           ((1, 2, 20000), 4), ((20, 1, 7), 7)]
 

@@ -259,6 +259,9 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void 
     for (int t = sg.t0; t < sg.t1; t += C, buf ^= 1) {
         const int n = min(C, sg.t1 - t);
         __syncthreads();                       // the last chunk's readers are done
+        rk.settle(a.dk, tid);
+        rv.settle(dvs, tid);
+        if (FULL) rq.settle(a.dk, tid);
         #pragma unroll
         for (int p = 0; p < rk.N; ++p) {
             const int row = rk.row(p, tid);
@@ -409,9 +412,11 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void 
                     const unsigned at = e < a.dv ? (unsigned)(i * (int)a.ot + e) * (unsigned)sizeof(T) : kOut;
                     if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b128(*(const u4*)y, bo, at, 0, 0);
                     else __builtin_amdgcn_raw_buffer_store_b64(*(const u2*)y, bo, at, 0, 0);
+                } else if (i < n && e + 4 <= a.dv) {
+                    __builtin_memcpy(ob + i * a.ot + e, y, sizeof(y));           // at any alignment
                 } else if (i < n) {
                     #pragma unroll
-                    for (int r = 0; r < 4; ++r)
+                    for (int r = 0; r < 3; ++r)
                         if (e + r < a.dv) ob[i * a.ot + e + r] = y[r];
                 }
             }

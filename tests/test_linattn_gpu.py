@@ -137,6 +137,26 @@ def test_strides(dtype, layout):
     R.check_linear_attention(got, None, R.linear_attention(q, k, v, g, [T], 1.0), t, dk, T)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dk,dv", [(9, 15), (63, 65), (7, 97), (130, 5), (31, 2)])
+def test_odd_sizes_read_and_write_their_columns_only(dtype, dk, dv):
+    """Rows that are no whole pieces, in wider rows of NaN, and out in wider rows
+    that keep what lies beside it."""
+    t, T, H, lens = R.TYPES[dtype], 139, 2, [70, 69]
+    q, k, v, g = make(T, H, H, dk, dv, t, 44)
+
+    def wide(x):
+        buf = torch.full((T, H, x.shape[2] + 3), float("nan"), dtype=t, device=DEV)
+        buf[:, :, 1:-2] = x
+        return buf[:, :, 1:-2]
+    buf = torch.full((T, H, dv + 5), 5.0, dtype=t, device=DEV)
+    s1 = torch.zeros(2, H, dk, dv, device=DEV)
+    ops().linear_attention(wide(q), wide(k), wide(v), g, buf[:, :, 3:-2], cu_seqlens=cu_of(lens), max_len=70,
+                           state_out=s1)
+    R.check_linear_attention(buf[:, :, 3:-2], s1, R.linear_attention(q, k, v, g, lens, 1.0), t, dk, 70)
+    assert (buf[:, :, :3] == 5).all() and (buf[:, :, -2:] == 5).all()
+
+
 def test_rows_of_no_sequence_stay():
     T, H = 200, 2
     q, k, v, g = make(T, H, H, 32, 32, torch.bfloat16, 6)

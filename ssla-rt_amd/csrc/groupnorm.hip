@@ -22,6 +22,8 @@
 // of 2048 bf16 channels in 16 groups with a gate (101 MB): 25 us, 4.0 TB/s.
 #include "groupnorm.h"
 
+#include <cmath>
+
 #include "drain_common.h"
 
 namespace ssla {
@@ -501,7 +503,15 @@ void group_norm_plan(GroupNormArgs& a, int dtype) {
     const long long lanes = np > 256 ? 1 : 256 / np;
     long long parts = 2048 / ((long long)a.n * a.blocks);
     const long long most = (a.rows + 4 * lanes - 1) / (4 * lanes);   // four rows a thread at least
-    parts = parts < 1 ? 1 : parts > 128 ? 128 : parts;
+    // Beyond 128 parts, as many as cost a workgroup of the second launch no more sums to
+    // read than values, while that is 1024 workgroups in all: 40000 rows of 512 bf16
+    // channels in 32 groups take 106 us in 128 parts, 63 in the 282 of this rule, 51 in
+    // 512, 84 in 1024, two such items 108, 74, 75, 152; one of 19200 rows of 96 fp32
+    // channels in 8 groups 16.9, 13.6 (240), 14.0, 14.0.
+    const long long even = (long long)sqrt((double)a.rows * (double)cg * e / sizeof(Sums));
+    const long long share = 1024 / ((long long)a.n * a.blocks), few_sums = even < share ? even : share;
+    const long long cap = few_sums > 128 ? few_sums : 128;
+    parts = parts < 1 ? 1 : parts > cap ? cap : parts;
     a.parts = (int)(parts > most ? most : parts);
 }
 

@@ -23,7 +23,8 @@ def make(shape, dtype, seed=0):
     return x, (1 + 0.3 * rnd(c)).to(dtype), (0.3 * rnd(c)).to(dtype), rnd(*shape).to(dtype)
 
 
-SHAPES = [((2, 24, 606), 1), ((2, 200, 128), 1), ((2, 1500, 9), 1), ((130, 30, 256), 4),
+SHAPES = [((1, 9000, 60), 2), ((2, 24, 606), 1), ((2, 200, 128), 1), ((2, 1500, 9), 1),
+          ((130, 30, 256), 4),
           ((600, 100, 24), 1), ((3, 16384), 8), ((40, 65536), 16), ((1, 2000, 24), 3),
           ((40, 320, 48), 8), ((290, 70, 33), 11), ((1, 1, 1), 1), ((3, 7, 24), 4),
           ((2, 5, 3, 24), 24), ((1, 20, 16, 48), 8), ((5, 33), 3), ((700, 96), 2),

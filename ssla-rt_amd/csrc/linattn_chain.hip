@@ -7,7 +7,9 @@ namespace {
 // ws_state holds each segment's own state L_j (from zero) and decay A_j; the
 // state before segment j + 1 is A_j X_j + L_j, from X_0 = the sequence's
 // initial state.  Every thread runs the chain of W neighbouring state values in
-// order and leaves X_j in L_j's place (not X_0, which nothing reads there).
+// order and leaves X_j in L_j's place.  X_0 too: the next launch writes final
+// states to s_out, which may be s_in, so none of its segments may read a cut
+// sequence's s_in.
 // Bound by the states' traffic, each read and written once: 32 segments of 16
 // heads of 128 x 128, 65 MB, take 12.8 us (13.4 with W = 1).
 template <int W>
@@ -49,7 +51,7 @@ __global__ __launch_bounds__(256) void k_linattn_chain(const LinAttnArgs a) {
         #pragma unroll
         for (int u = 0; u < U; ++u)
             if (k0 + u < n - 1) {
-                if (k0 + u) w[(k0 + u) * step] = x;
+                w[(k0 + u) * step] = x;
                 x = dec[u] * x + own[u];
             }
     }

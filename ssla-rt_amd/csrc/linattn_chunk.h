@@ -122,10 +122,13 @@ struct Place {
     __device__ __forceinline__ float* segment_state(const LinAttnArgs& a) const {
         return a.ws_state + (long long)j_seg * a.heads * a.dk * a.dv + state;
     }
-    // Where the state comes from (null: zeros) and goes to (null: nowhere).
+    // Where the state comes from (null: zeros) and goes to (null: nowhere).  Of a
+    // cut sequence every segment's comes from the workspace, the first one's too:
+    // s_out may be s_in, and the last segment's workgroup may end before the
+    // first one's begins.
     __device__ __forceinline__ const float* source(const LinAttnArgs& a, bool full) const {
         if (!full) return nullptr;
-        if (sg.index > 0) return segment_state(a);
+        if (sg.index > 0 || !last) return segment_state(a);
         return a.s_in ? a.s_in + (long long)slot * a.s_stride + state : nullptr;
     }
     __device__ __forceinline__ float* sink(const LinAttnArgs& a, bool full) const {

@@ -61,7 +61,7 @@ __device__ __forceinline__ void loads_stay_above() { __builtin_amdgcn_sched_barr
 // token i as two floats, since b_i - b_j is small where b is large), exp(b_i)
 // times the output's scale, exp(b_C - b_i), and exp(b_C).
 template <int C>
-struct Decays {
+struct alignas(16) Decays {
     float hi[C], lo[C], eb[C], w[C], end;
 
     // By one wave whose lane i holds g_i; lanes from C on hold 0.
@@ -227,7 +227,7 @@ struct Rows {
                         // last E values, shifted by settle()
                         __builtin_memcpy(&x[p], from + min(c, cols - E), 16);
                     } else {
-                        T y[E];
+                        alignas(16) T y[E];
                         #pragma unroll
                         for (int i = 0; i < E; ++i) y[i] = i < cols ? from[i] : (T)0.0f;
                         x[p] = *(const u4*)y;

@@ -38,6 +38,8 @@
 // changed nothing.
 #pragma once
 
+#include <cstddef>
+
 #include "linattn_chunk.h"
 
 namespace ssla {
@@ -208,6 +210,9 @@ struct Lds {
     __bf16 p[PT][C * PS];        // rows i, columns j in operand order
     Decays<C> b[2];              // of this chunk and the next
 };
+// Decays are read four at a time in either of the two.
+static_assert(sizeof(Decays<C>) % 16 == 0 && alignof(Decays<C>) % 16 == 0 && offsetof(Decays<C>, hi) % 16 == 0 &&
+              offsetof(Decays<C>, lo) % 16 == 0 && offsetof(Decays<C>, w) % 16 == 0);
 
 template <class T, int DK, int NW, bool FULL, bool VEC>
 __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void k_linattn(const LinAttnArgs a) {
@@ -405,7 +410,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void 
             #pragma unroll
             for (int it = 0; it < IT; ++it) {
                 const int i = 16 * it + m;
-                T y[4];
+                alignas(16) T y[4];
                 #pragma unroll
                 for (int r = 0; r < 4; ++r) y[r] = (T)O[it][r];
                 if (VEC) {

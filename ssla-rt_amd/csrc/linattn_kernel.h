@@ -17,12 +17,17 @@
 //
 // Precision: an operand is the sum of bf16 terms, each the rounding of what the
 // ones before leave (2^-8 each time): a bf16 token value is one term, an fp16
-// value two, both exactly; an fp32 value, and P and S there, three.  For 16-bit
-// tokens P and the copy of S that multiplies q have two (2^-16, well below the
-// output's 2^-8 or 2^-11), exp(b_C - b_j) v_j three, since these products make
-// up the fp32 state.  Products of terms whose orders add up to more than the
-// last kept one's are left out.  fp32 tokens take 6 bf16 products of 16 cycles
-// where the fp32 instruction takes 256 cycles for the same block.
+// value two, both exactly; an fp32 value, and P and S there, three.  For bf16
+// tokens P has three too: with two its rounding (2^-18) was most of what set the
+// outputs apart from an fp32 computation's, 9.9e-5 against 3.9e-5 of them over 8192
+// tokens of 16 heads of 128 (the third costs 1 to 2%).  P of fp16 tokens has two
+// (4.7e-5; a third costs 3.6%, and the error against 64 bits, 2.074e-4, would fall
+// by a four thousandth of it), and so has, for both, the copy of S that multiplies
+// q, 2^-18 of each value (a third changes the bf16 outputs by 2e-6 and costs 7%).
+// exp(b_C - b_j) v_j has three, since these products make up the fp32 state.
+// Products of terms whose orders add up to more than the last kept one's are
+// left out.  fp32 tokens take 6 bf16 products of 16 cycles where the fp32
+// instruction takes 256 cycles for the same block.
 //
 // Each wave owns 16 columns of v, the state and the output; the C x C products
 // P are dealt over the waves and shared through LDS.
@@ -201,7 +206,8 @@ constexpr int C = 32;
 
 template <class T, int DK, int NW>
 struct Lds {
-    static constexpr int TERMS = Token<T>::TERMS, PT = TERMS == 3 ? 3 : 2;       // PT: terms of P and S
+    static constexpr int TERMS = Token<T>::TERMS;
+    static constexpr int PT = TERMS == 2 ? 2 : 3, ST = TERMS == 3 ? 3 : 2;       // terms of P; of S's copy
     static constexpr int DV = 16 * NW;
     static constexpr int QS = DK + kPad, PS = C + kPad, VS = Token<T>::template stride<DV>();
     __bf16 q[TERMS][C * QS];
@@ -219,10 +225,10 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void 
     typedef Token<T> Tk;
     typedef typename Tk::V8 V8;
     typedef Lds<T, DK, NW> L;
-    constexpr int NT = 64 * NW, TERMS = L::TERMS, PT = L::PT;
+    constexpr int NT = 64 * NW, TERMS = L::TERMS, PT = L::PT, ST = L::ST;
     constexpr int DT = DK / 16, KS = DK / 32;              // tiles, steps along d
     constexpr int IT = C / 16;                             // tiles along tokens
-    constexpr int OUT_ORDER = PT - 1;                      // highest order of terms' products kept
+    constexpr int P_ORDER = PT - 1, S_ORDER = ST - 1;      // highest orders of terms' products kept
     extern __shared__ __align__(16) char smem[];
     L& lds = *reinterpret_cast<L*>(smem);
 
@@ -314,7 +320,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void 
                         for (int i = 0; i < TERMS; ++i)
                             #pragma unroll
                             for (int j = 0; j < TERMS; ++j)
-                                if (i + j <= OUT_ORDER) {
+                                if (i + j <= P_ORDER) {
                                     f4& c = acc[TERMS == 1 ? s & 1 : j & 1];
                                     c = mma(ka[s][i], qa[s][j], c);
                                 }
@@ -346,13 +352,13 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void 
                     for (int i = 0; i < TERMS; ++i)
                         qa[it][i] = *(const bf8*)&lds.q[i][(16 * it + m) * L::QS + 32 * s + 8 * g];
                 loads_stay_above();
-                bf8 sa[PT];
+                bf8 sa[ST];
                 split(join(S[2 * s], S[2 * s + 1]), sa);
                 #pragma unroll
-                for (int h = 0; h < PT; ++h)
+                for (int h = 0; h < ST; ++h)
                     #pragma unroll
                     for (int i = 0; i < TERMS; ++i)
-                        if (h + i <= OUT_ORDER)
+                        if (h + i <= S_ORDER)
                             #pragma unroll
                             for (int it = 0; it < IT; ++it) O[it] = mma(sa[h], qa[it][i], O[it]);
             }
@@ -391,7 +397,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void 
             for (int h = 0; h < PT; ++h)
                 #pragma unroll
                 for (int i = 0; i < TERMS; ++i)
-                    if (h + i <= OUT_ORDER)
+                    if (h + i <= P_ORDER)
                         #pragma unroll
                         for (int it = 0; it < IT; ++it) O[it] = mma(vt[i], pa[it][h], O[it]);
             if (any_bad) {

@@ -1,6 +1,6 @@
 """How many bits linear attention's operands keep, at inputs whose answers have
 few roundings, so that a term of an operand that is left out shows: one product
-chain an output.  The checks themselves are tested on
+chain an output, or two that nearly cancel.  The checks themselves are tested on
 the CPU, where an emulation with a term too few has to fail them.
 
 Log decays are 0 (factors of exactly 1), scale is 1.  A sum on the matrix cores may
@@ -18,6 +18,9 @@ CHUNK = 32
 OUT_ROUNDINGS = 2 * 7 + 2 * 6 + 2
 # The state: six products of terms.
 STATE_ROUNDINGS = 2 * 6 + 1
+# A difference of two P v: four products and their sums a P, three terms of each P
+# times v.
+PAIR_ROUNDINGS = 2 * 4 + 2 * 6 + 1
 
 
 def terms(x, n):
@@ -116,3 +119,49 @@ def test_states_of_16_bit_tokens_are_exact_products(dtype, T):
     ops.linear_attention(q.to(DEV), k.to(DEV), v.to(DEV), torch.zeros(2, device=DEV), state_out=s)
     # bf16: one product; fp16: two terms by two, the lowest three of the sums cut off
     assert chain_error(s[0], state_answer(k, v), 0.5 if dtype == torch.bfloat16 else 8) <= 1.0
+
+
+# ---- two that nearly cancel ----------------------------------------------------------
+
+def pairs(n, dk, dv, seed):
+    """n sequences of one chunk: tokens 0 and 1 have nearly the same key and
+    opposite values, the others none; queries have four dimensions:
+    out_t = (q_t.k_0 - q_t.k_1) v_0 for t > 0, some 2^-14 of each of the two."""
+    gen = torch.Generator().manual_seed(seed)
+    pos = lambda *s: 1.0 + torch.rand(*s, generator=gen)  # noqa: E731
+    q = torch.zeros(n, CHUNK, 1, dk)
+    q[..., :4] = pos(n, CHUNK, 1, 4) * torch.tensor([1.0, 0.3, 0.04, 2.0 ** -6])
+    q = q.bfloat16()
+    k = torch.zeros(n, CHUNK, 1, dk).bfloat16()
+    k[:, 0, 0, :4] = k[:, 1, 0, :4] = pos(n, 4).bfloat16()
+    k[:, 1, 0, 3] += 2.0 ** -6
+    v = torch.zeros(n, CHUNK, 1, dv).bfloat16()
+    v[:, 0, 0] = torch.randn(n, dv, generator=gen).bfloat16()
+    v[:, 1, 0] = -v[:, 0, 0]
+    return q, k, v
+
+
+def pair_error(out, q, k, v):
+    p = torch.matmul(q[:, :, 0].double(), k[:, :2, 0].double().transpose(1, 2))      # (n, CHUNK, 2)
+    v0 = v[:, 0].double()
+    want = (p[..., :1] - p[..., 1:]) * v0
+    tol = PAIR_ROUNDINGS * U * p.sum(2, keepdim=True) * v0.abs() + 2.0 ** -9 * 1.01 * want.abs() + 1e-36
+    return ((out.detach().cpu().double() - want).abs() / tol)[:, 1:].max().item()
+
+
+@pytest.mark.parametrize("n_terms", [2, 3])
+def test_the_check_of_pairs_sees_a_term_too_few(n_terms):
+    q, k, v = pairs(40, 16, 24, 4)
+    p = terms(f32(torch.matmul(q[:, :, 0].double(), k[:, :2, 0].double().transpose(1, 2))), n_terms)
+    out = ((p[..., :1] - p[..., 1:]) * v[:, 0].double()).bfloat16()
+    worst = pair_error(out, q, k, v)
+    assert worst > 1.2 if n_terms == 2 else worst <= 0.3, worst
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dk,dv", [(16, 24), (128, 128), (256, 40)])
+def test_products_within_a_chunk_of_bf16_tokens_keep_three_terms(dk, dv):
+    from ssla_hip import ops
+    q, k, v = pairs(40, dk, dv, 5)
+    out = ops.linear_attention(*(x.flatten(0, 1).to(DEV) for x in (q, k, v)), torch.zeros(1, device=DEV), n_seqs=40)
+    assert pair_error(out.view(40, CHUNK, dv), q, k, v) <= 1.0

@@ -12,11 +12,12 @@
 //   two passes k_group<kStats> leaves each part's sums in the workspace,
 //              k_group<kApply> adds them up and reads x again (from the 256 MB
 //              cache where x fits it)
-// Moments are sums of x and x^2 in 64 bits: the variance's difference then
-// loses nothing that an fp32 input holds (a mean 10^6 standard deviations from
-// zero costs 10^12 of 10^16), the order of summation does not show, and the
-// conversions hide behind the loads.  k_group_lanes has a group's values in
-// registers and takes the mean first, then squared differences from it.
+// Moments are sums of x and x^2 in 64 bits: squares of finite values do not
+// overflow, the variance's difference loses little (with a mean 10^6 standard
+// deviations from zero 10^12 of 10^16), the order of summation does not show, and
+// the conversions hide behind the loads.  k_group_lanes has a group's values in
+// registers and takes the mean first, then squared differences from it, in 64
+// bits too.  The mean is subtracted as two floats (norm_of).
 // 16 items of 19200 rows of 96 fp32 channels (118 MB in, 118 out) take 74 us out of
 // memory, 20 + 39 with x in the cache: three passes at 4.7 to 6 TB/s.  8191 tokens
 // of 2048 bf16 channels in 16 groups with a gate (101 MB): 25 us, 4.0 TB/s.
@@ -49,10 +50,30 @@ __device__ __forceinline__ float activate(float x, int act) {
     }
 }
 
-// Mean and 1 / sqrt(var + eps).
-__device__ __forceinline__ float2 moments(Sums s, double inv_count, float eps) {
+// A group's mean and 1 / sqrt(var + eps), of which
+//     (x - mean) / sqrt(var + eps) = (2^-16 x - hi) scale - lo scale.
+// hi + lo is the mean to 48 bits: hi alone would be off by up to 2^-25 of the
+// mean, which is 0.03 standard deviations where the mean is 10^6 of them.
+// 2^-16 x - hi, one fused operation, is finite for all finite x and mean, and scale
+// is a normal number for any spread of them; what the two lose of the smallest x
+// lies below 2^-133.
+struct alignas(16) Norm {
+    float hi, lo, scale;
+};
+constexpr float kDown = 0x1p-16f;
+
+__device__ __forceinline__ Norm norm_of(double mean, double var, float eps) {
+    const double s = var + (double)eps, m = mean * (double)kDown;
+    // the instruction's root is good to some 2^-24; a Newton step doubles that,
+    // except for 0 and infinity, where it gives a NaN
+    const double r0 = __builtin_amdgcn_rsq(s), r1 = r0 * fma(-0.5 * s * r0, r0, 1.5);
+    const double r = (r1 == r1 ? r1 : r0) / (double)kDown;
+    const float hi = (float)m;
+    return Norm{hi, (float)(m - (double)hi), (float)r};
+}
+__device__ __forceinline__ Norm norm_of(Sums s, double inv_count, float eps) {
     const double mean = s.s * inv_count, var = fma(-mean, mean, s.q * inv_count);
-    return float2{(float)mean, 1.0f / sqrtf((var < 0.0 ? 0.0f : (float)var) + eps)};      // a NaN stays
+    return norm_of(mean, var < 0.0 ? 0.0 : var, eps);        // a NaN stays
 }
 
 // Sum over the w lanes (a power of two up to 64) that share a group.
@@ -91,9 +112,10 @@ __global__ __launch_bounds__(NT) void k_group(const GroupNormArgs a) {
     // LDS: the groups' sums, then their mean and 1 / sqrt(var + eps); behind them
     // every thread's sums (one a piece, or one a channel), then the channels' table
     Sums* total = (Sums*)smem;
-    float2* norm = (float2*)smem;
+    Norm* norm = (Norm*)smem;
+    static_assert(sizeof(Norm) == sizeof(Sums));
     Sums* own = total + a.gb;
-    float* table = (float*)own;                              // mean, scale, bias of a stretch's channels
+    float* table = (float*)own;                              // hi, scale, bias of a stretch's channels
     const int width = cols * V;
     const int per = whole ? 1 : V;
     int w = 1;                                               // lanes that add up a group
@@ -222,7 +244,7 @@ __global__ __launch_bounds__(NT) void k_group(const GroupNormArgs a) {
             s = total[g];
         }
         // in `total`'s place: one group's lanes read it above and write it here
-        if (tid % w == 0) norm[2 * g] = moments(s, a.inv_count, a.eps);
+        if (tid % w == 0) norm[g] = norm_of(s, a.inv_count, a.eps);
     }
     __syncthreads();
 
@@ -231,18 +253,19 @@ __global__ __launch_bounds__(NT) void k_group(const GroupNormArgs a) {
         for (int ch = tid; ch < width; ch += nt) {
             const int at = pc * V + ch, c = p0 * V + at;
             const bool mine = c >= c0 && c < c1, ahead = at == tid;
-            const float2 f = norm[mine ? 2 * ((c - c0) / cg) : 0];
-            table[ch] = f.x;
-            table[width + ch] = f.y * (ahead ? w0 : weight_of(at));
-            table[2 * width + ch] = ahead ? b0 : bias_of(at);
+            const Norm f = norm[mine ? (c - c0) / cg : 0];
+            const float scale = f.scale * (ahead ? w0 : weight_of(at));
+            table[ch] = f.hi;
+            table[width + ch] = scale;
+            table[2 * width + ch] = fmaf(-f.lo, scale, ahead ? b0 : bias_of(at));
         }
         __syncthreads();
         const int p = p0 + pc + px;
         if (!on || pc + px >= np) continue;
-        float mean[V], scale[V], bias[V];
+        float hi[V], scale[V], bias[V];
         #pragma unroll
         for (int i = 0; i < V; ++i) {
-            mean[i] = table[px * V + i];
+            hi[i] = table[px * V + i];
             scale[i] = table[width + px * V + i];
             bias[i] = table[2 * width + px * V + i];
         }
@@ -251,7 +274,7 @@ __global__ __launch_bounds__(NT) void k_group(const GroupNormArgs a) {
             P y;
             #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float v = fmaf((float)in.v[i] - mean[i], scale[i], bias[i]);
+                const float v = fmaf(fmaf((float)in.v[i], kDown, -hi[i]), scale[i], bias[i]);
                 y.v[i] = (T)(gate ? v * activate((float)pg.v[i], a.act) : activate(v, a.act));
             }
             T* o = out + (long long)row * a.orow + (long long)p * V;
@@ -287,8 +310,8 @@ template <int V> constexpr int kWideReps = V == 8 ? 2 : 4;
 // ---- small groups --------------------------------------------------------------
 // `w` threads hold a group of one item, R pieces each: some lanes of a wave, with
 // neighbouring lanes' groups neighbours, or (WHOLE) a workgroup.  The mean first, then the sum of squared differences from it.
-template <class S, int NT, bool WHOLE>
-__device__ __forceinline__ S group_sum(S s, int w, S* waves) {
+template <int NT, bool WHOLE>
+__device__ __forceinline__ double group_sum(double s, int w, double* waves) {
     for (int o = WHOLE ? 32 : w >> 1; o; o >>= 1) s += __shfl_xor(s, o);
     if (WHOLE) {
         if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = s;
@@ -335,32 +358,26 @@ __global__ __launch_bounds__(NT) void k_group_lanes(const GroupNormArgs a) {
             }
         }
     }
-    float s = 0.0f;
+    double s = 0.0;
     #pragma unroll
-    for (int k = 0; k < R; ++k) {                            // by pairs: log2 roundings a term
-        float t[V];
+    for (int k = 0; k < R; ++k)
         #pragma unroll
-        for (int j = 0; j < V; ++j) t[j] = (float)px[k].v[j];
-        #pragma unroll
-        for (int o = V / 2; o; o >>= 1)
-            #pragma unroll
-            for (int j = 0; j < o; ++j) t[j] += t[j + o];
-        s += t[0];
-    }
-    s = group_sum<float, NT, WHOLE>(s, w, (float*)sums);
-    const float mean = s * (float)a.inv_count;
-    double q = 0.0;                                          // squares do not overflow
+        for (int j = 0; j < V; ++j) s += (double)(float)px[k].v[j];
+    s = group_sum<NT, WHOLE>(s, w, sums);
+    const double mean = s * a.inv_count;
+    double q = 0.0;
     #pragma unroll
     for (int k = 0; k < R; ++k)
         if (l + k * w < pieces) {
             #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const double d = (double)((float)px[k].v[j] - mean);
+                const double d = (double)(float)px[k].v[j] - mean;
                 q = fma(d, d, q);
             }
         }
-    q = group_sum<double, NT, WHOLE>(q, w, squares);
-    const float rstd = 1.0f / sqrtf((float)(q * a.inv_count) + a.eps);
+    q = group_sum<NT, WHOLE>(q, w, squares);
+    const Norm f = norm_of(mean, q * a.inv_count, a.eps);
+    const float low = -f.lo * f.scale;
     #pragma unroll
     for (int k = 0; k < R; ++k) {
         const int i = l + k * w;
@@ -369,7 +386,8 @@ __global__ __launch_bounds__(NT) void k_group_lanes(const GroupNormArgs a) {
             P y;
             #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float v = fmaf(((float)px[k].v[j] - mean) * rstd, (float)pw[k].v[j], (float)pb[k].v[j]);
+                const float d = fmaf(fmaf((float)px[k].v[j], kDown, -f.hi), f.scale, low);
+                const float v = fmaf(d, (float)pw[k].v[j], (float)pb[k].v[j]);
                 y.v[j] = (T)(gate ? v * activate((float)pg[k].v[j], a.act) : activate(v, a.act));
             }
             *(P*)(out + row * a.orow + p) = y;

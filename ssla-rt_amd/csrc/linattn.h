@@ -30,12 +30,13 @@ struct LinAttnArgs {
     const float* s_in;
     float* s_out;
     long long s_stride;                   // floats between slots
-    float* ws_state;                      // [segment][head][dk][dv] (more than one segment a sequence)
-    float* ws_decay;                      // [segment][head]
+    float* ws_state;                      // [state][head][dk][dv], of the segments of cut sequences
+    float* ws_decay;                      // [state][head]
     long long n_tokens;
     int n_seqs, n_slots, max_len;
     int heads, rep, dk, dv, slices;       // rep: heads sharing q and k
     int seg_shift, n_segs;                // log2 of a segment's tokens; segments of the call
+    int n_states, paired;                 // states of the workspace; where they lie: linattn_states
     int by_length;                        // whole sequences of unlike lengths: see linattn_by_length
     int vec;                              // buffer loads of q, k, v and stores of out, in pieces
     float scale;
@@ -44,10 +45,11 @@ struct LinAttnArgs {
 // Where a segment lies: sequence `seq`, tokens [t0, t1) of its `len`, which
 // begin at row `row`.  Segment slots of sequence s begin at
 // (cu[s] >> seg_shift) + s: as many as it can need whatever the lengths, so
-// the grid needs only the number of tokens and sequences.
+// the grid needs only the number of tokens and sequences.  Its state is `state` of
+// the workspace, where the sequence is cut.
 struct Segment {
     long long row;
-    int seq, index, t0, t1, len;
+    int seq, index, state, t0, t1, len;
     bool ok;
 };
 
@@ -56,9 +58,18 @@ __device__ __forceinline__ long long linattn_first(const LinAttnArgs& a, int s) 
     const long long c = a.cu[s];
     return c < 0 ? 0 : c > a.n_tokens ? a.n_tokens : c;
 }
-#endif
 
-#ifdef __HIP_DEVICE_COMPILE__
+// Place in the workspace of the first state of a sequence that begins at token
+// `first`: its first segment slot; or (paired) twice the whole segments' lengths of
+// tokens before it.  Only sequences of n > 1 segments have states there, and the
+// next one begins at least n / 2 such lengths later, so that 2 (n_tokens >> shift)
+// states do, however many sequences there are: 511 sequences of a token beside one of
+// 4000 (16 heads of 128, segments of 256) take 36 MB instead of 555.
+__device__ __forceinline__ int linattn_states(const LinAttnArgs& a, long long first, int seq) {
+    const int piece = (int)(first >> a.seg_shift);
+    return a.paired ? 2 * piece : piece + seq;
+}
+
 // Whole sequences (up to 64) of unlike lengths: the longest first, and every
 // second round of the compute units in the other direction, so that those
 // that share a compute unit are not all long.  48 sequences of 340 to 1531 tokens
@@ -86,7 +97,7 @@ __device__ __forceinline__ Segment linattn_segment(const LinAttnArgs& a, int j, 
         g.seq = linattn_by_length(a, j, lane);
         g.row = linattn_first(a, g.seq);
         len = linattn_first(a, g.seq + 1) - g.row;
-        g.index = 0;
+        g.index = g.state = 0;
     } else if (a.cu) {
         // the last sequence whose first slot is at or before j, 64 candidates a round
         int lo = 0, n = a.n_seqs;
@@ -104,10 +115,12 @@ __device__ __forceinline__ Segment linattn_segment(const LinAttnArgs& a, int j, 
         g.row = linattn_first(a, g.seq);
         len = linattn_first(a, g.seq + 1) - g.row;
         g.index = j - (int)((g.row >> a.seg_shift) + g.seq);
+        g.state = linattn_states(a, g.row, g.seq) + g.index;
     } else {
         const int per = a.n_segs / a.n_seqs;
         g.seq = j / per;
         g.index = j - g.seq * per;
+        g.state = j;
         len = a.max_len;
         g.row = (long long)g.seq * a.max_len;
     }

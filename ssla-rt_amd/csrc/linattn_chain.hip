@@ -23,7 +23,7 @@ __global__ __launch_bounds__(256) void k_linattn_chain(const LinAttnArgs a) {
         const long long first = linattn_first(a, seq);
         const long long len = linattn_first(a, seq + 1) - first;
         const int l = (int)(len < 0 ? 0 : len > a.max_len ? a.max_len : len);
-        j = (int)(first >> a.seg_shift) + seq;
+        j = linattn_states(a, first, seq);
         n = (int)(((unsigned)l + (1u << a.seg_shift) - 1) >> a.seg_shift);
 #endif
     } else {

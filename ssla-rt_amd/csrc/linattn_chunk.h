@@ -86,7 +86,7 @@ struct alignas(16) Decays {
 template <class T, int NW>
 struct Place {
     Segment sg;
-    int j_seg, head, slice, slot, e0;          // e0: the wave's first column
+    int head, slice, slot, e0;                 // e0: the wave's first column
     bool last;                                 // of its sequence's segments
     const T *q, *k, *v;
     const float* g;
@@ -101,7 +101,7 @@ struct Place {
         const int all = a.n_segs * groups, set = 8 * sharers;
         const int at = blockIdx.x / set, width = min(8, all - 8 * at), in = blockIdx.x - at * set;
         const int sharer = in / width, group = 8 * at + in - sharer * width;
-        j_seg = group / groups;
+        const int j_seg = group / groups;
         const int member = sharer / a.slices;
         slice = sharer - member * a.slices;
         head = (group - j_seg * groups) * a.rep + member;
@@ -120,7 +120,7 @@ struct Place {
         return true;
     }
     __device__ __forceinline__ float* segment_state(const LinAttnArgs& a) const {
-        return a.ws_state + (long long)j_seg * a.heads * a.dk * a.dv + state;
+        return a.ws_state + (long long)sg.state * a.heads * a.dk * a.dv + state;
     }
     // Where the state comes from (null: zeros) and goes to (null: nowhere).  Of a
     // cut sequence every segment's comes from the workspace, the first one's too:

@@ -474,7 +474,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd(DK, Token<T>::TERMS)) void 
         if (t + C < sg.t1 && wave == NW - 1) lds.b[buf ^ 1].set(rg, a.scale, lane);
     }
 
-    if (!FULL && pl.slice == 0 && tid == 0) a.ws_decay[(long long)pl.j_seg * a.heads + pl.head] = decay;
+    if (!FULL && pl.slice == 0 && tid == 0) a.ws_decay[(long long)sg.state * a.heads + pl.head] = decay;
     write_state(S, pl, a, FULL, m, g);
 }
 

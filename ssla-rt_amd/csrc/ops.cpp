@@ -125,6 +125,7 @@ bool cut(const SslaHipLinAttn* d, LinAttnArgs& a) {
     if (a.max_len <= 256 || a.max_len <= (1ll << shift) || 2 * kCUs * (long long)a.max_len <= 3 * rows) {
         a.seg_shift = 31;                              // no sequence is cut
         a.n_segs = d->n_seqs;
+        a.n_states = 0;
         a.by_length = d->cu_seqlens && d->n_seqs > 1 && d->n_seqs <= 64 &&
                       (long long)d->n_seqs * a.max_len > d->n_tokens;
         return true;
@@ -132,7 +133,10 @@ bool cut(const SslaHipLinAttn* d, LinAttnArgs& a) {
     a.seg_shift = shift;
     const long long segs = d->cu_seqlens ? (d->n_tokens >> shift) + d->n_seqs
                                          : d->n_seqs * ((a.max_len + (1ll << shift) - 1) >> shift);
+    const long long pairs = 2 * (d->n_tokens >> shift);      // see linattn_states
     a.n_segs = (int)segs;
+    a.paired = d->cu_seqlens && pairs < segs;
+    a.n_states = (int)(a.paired ? pairs : segs);
     return segs <= 0x7fffffff;
 }
 
@@ -160,8 +164,7 @@ LinAttnArgs linattn_args(const SslaHipLinAttn* d) {
 }
 
 size_t linattn_bytes(const LinAttnArgs& a) {
-    if (a.seg_shift == 31) return 0;
-    return (size_t)a.n_segs * a.heads * ((size_t)a.dk * a.dv + 1) * 4;
+    return (size_t)a.n_states * a.heads * ((size_t)a.dk * a.dv + 1) * 4;
 }
 
 // ---- group norm ------------------------------------------------------------------
@@ -255,7 +258,7 @@ int ssla_hip_linattn(const SslaHipLinAttn* d, void* workspace, size_t workspace_
         if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
             return refuse("ssla_hip_linattn: the workspace is missing, too small or not 16-byte aligned");
         a.ws_state = (float*)workspace;
-        a.ws_decay = a.ws_state + (size_t)a.n_segs * a.heads * a.dk * a.dv;
+        a.ws_decay = a.ws_state + (size_t)a.n_states * a.heads * a.dk * a.dv;
     }
     const hipStream_t st = (hipStream_t)stream;
     hipError_t (*run)(const LinAttnArgs&, bool, hipStream_t) =

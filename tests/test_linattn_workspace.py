@@ -40,6 +40,20 @@ def test_a_serving_batch():
     assert size(2000, 1, 2000, heads=4) == (2000 // 64 + 1) * 4 * (128 * 128 + 1) * 4
 
 
+def test_sizes_at_the_largest_counts():
+    """The size at the largest number of tokens, and its refusal beyond."""
+    most = (1 << 31) - (1 << 16)
+    # one sequence of one head: 127 whole segments of 2^24 tokens and the rest
+    assert size(most, 1, most, heads=1) == 128 * (128 * 128 + 1) * 4
+    assert size(most, 1_000_000, most, heads=1) == 2 * 127 * (128 * 128 + 1) * 4
+    # 128 sequences of 2^24 tokens: nothing is cut
+    assert size(most, 128, 1 << 24) == 0
+    with pytest.raises(lib.SslaHipError, match="n_tokens"):
+        size(most + 1, 1, most, heads=1)
+    with pytest.raises(lib.SslaHipError, match="n_tokens"):      # the limit comes before the cut
+        size((1 << 31) - 1, 2, 1 << 30, heads=512)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("pool", ["one", "two"])

@@ -15,8 +15,8 @@
 // tokens is free too: P's columns are put into the registers' order on their way
 // to LDS (operand_at), and tokens are taken in it from k and v.
 //
-// Precision: an operand is the sum of bf16 terms, each the rounding of what the
-// ones before leave (2^-8 each time): a bf16 token value is one term, an fp16
+// Precision: an operand is the sum of bf16 terms, each eight bits of what the
+// ones before leave: a bf16 token value is one term, an fp16
 // value two, both exactly; an fp32 value, and P and S there, three.  For bf16
 // tokens P has three too: with two its rounding (2^-18) was most of what set the
 // outputs apart from an fp32 computation's, 9.9e-5 against 3.9e-5 of them over 8192
@@ -74,6 +74,20 @@ __device__ __forceinline__ unsigned split2(float& x, float& y) {
 __device__ __forceinline__ unsigned round2(float x, float y) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector(f2{x, y}, bf2));
 }
+// The same, cut off instead of rounded.
+__device__ __forceinline__ unsigned cut2(float& x, float& y) {
+    const unsigned a = __builtin_bit_cast(unsigned, x), b = __builtin_bit_cast(unsigned, y);
+    x -= __builtin_bit_cast(float, a & 0xffff0000u);
+    y -= __builtin_bit_cast(float, b & 0xffff0000u);
+    return (a >> 16) | (b & 0xffff0000u);
+}
+// Term n of N.  The first of three is cut off: rounded, the largest fp32 values would
+// become infinities, and with two terms behind it the half step does not matter
+// (2^-26 is left instead of 2^-27).
+template <int N>
+__device__ __forceinline__ unsigned term(int n, float& x, float& y) {
+    return n + 1 == N ? round2(x, y) : N == 3 && n == 0 ? cut2(x, y) : split2(x, y);
+}
 // x as N bf16 terms.
 template <int N>
 __device__ __forceinline__ void split(f8 x, bf8 (&t)[N]) {
@@ -83,7 +97,7 @@ __device__ __forceinline__ void split(f8 x, bf8 (&t)[N]) {
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float a = x[2 * i], b = x[2 * i + 1];
-            h[i] = n + 1 < N ? split2(a, b) : round2(a, b);
+            h[i] = term<N>(n, a, b);
             x[2 * i] = a;
             x[2 * i + 1] = b;
         }
@@ -97,7 +111,7 @@ __device__ __forceinline__ void split(f4 x, u2 (&t)[N]) {
         #pragma unroll
         for (int i = 0; i < 2; ++i) {
             float a = x[2 * i], b = x[2 * i + 1];
-            t[n][i] = n + 1 < N ? split2(a, b) : round2(a, b);
+            t[n][i] = term<N>(n, a, b);
             x[2 * i] = a;
             x[2 * i + 1] = b;
         }

@@ -13,11 +13,12 @@ DEV = "cuda"
 U = 2.0 ** -24
 CHUNK = 32
 # Out of one chain: six products of terms for q.k, in two sums that are added (7
-# additions), six for P.v; or six for the state and six for it times q; each operand
-# in three terms is off by 2^-27, and so are the products of terms left out.
-OUT_ROUNDINGS = 2 * 7 + 2 * 6 + 2
-# The state: six products of terms.
-STATE_ROUNDINGS = 2 * 6 + 1
+# additions), six for P.v; or six for the state and six for it times q.  Three terms
+# of an operand, the first of them cut off, leave 2^-26 of it, U / 4 (four operands);
+# of a product's terms the ones left out are 2^-8 2^-17 twice, 1 U (two products).
+OUT_ROUNDINGS = 2 * 7 + 2 * 6 + 4 / 4 + 2
+# The state: six products of terms, two operands, one product.
+STATE_ROUNDINGS = 2 * 6 + 2 / 4 + 1
 # A difference of two P v: four products and their sums a P, three terms of each P
 # times v.
 PAIR_ROUNDINGS = 2 * 4 + 2 * 6 + 1
@@ -165,3 +166,23 @@ def test_products_within_a_chunk_of_bf16_tokens_keep_three_terms(dk, dv):
     q, k, v = pairs(40, dk, dv, 5)
     out = ops.linear_attention(*(x.flatten(0, 1).to(DEV) for x in (q, k, v)), torch.zeros(1, device=DEV), n_seqs=40)
     assert pair_error(out.view(40, CHUNK, dv), q, k, v) <= 1.0
+
+
+# ---- the largest values ----------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [90, 600])
+@pytest.mark.parametrize("what", ["q", "k", "v"])
+@pytest.mark.parametrize("value", [torch.finfo(torch.float32).max, -3.396e38])
+def test_the_largest_fp32_values_are_finite(T, what, value):
+    """They are beyond bf16's largest; other values keep the answers in range."""
+    import seq_ref as R
+    from ssla_hip import ops
+    gen = torch.Generator().manual_seed(6)
+    q, k, v = (1e-10 * torch.randn(T, 2, n, generator=gen) for n in (32, 32, 48))
+    {"q": q, "k": k, "v": v}[what][T // 2 + 5, 1, 3] = value
+    g = torch.full((2,), -0.02)
+    want = R.linear_attention(q, k, v, g, [T], 1.0)
+    s = torch.zeros(1, 2, 32, 48, device=DEV)
+    out = ops.linear_attention(q.to(DEV), k.to(DEV), v.to(DEV), g.to(DEV), state_out=s)
+    R.check_linear_attention(out, s, want, torch.float32, 32, T)

@@ -9,6 +9,7 @@
 
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -79,13 +80,15 @@ int dtype_of(const char* fn, const char* name, const at::Tensor& t) {
     }
 }
 
-// Type and device of a tensor of the call; there is no backward pass.
+// Type and device of a tensor of the call; there are no gradients, backward or forward.
 void alike(const char* fn, const char* name, const at::Tensor& t, at::ScalarType type, at::Device dev) {
     if (t.scalar_type() != type || t.device() != dev || t.layout() != at::kStrided)
         refuse(fn, std::string(name) + " must be a " + c10::toString(type) + " tensor on " + dev.str());
     if (t.is_neg()) refuse(fn, std::string(name) + " is a negated view: call resolve_neg()");
     if (t.requires_grad() && at::GradMode::is_enabled())
         refuse(fn, std::string(name) + " requires a gradient, which there is none of: call under torch.no_grad()");
+    if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        refuse(fn, std::string(name) + " carries a forward gradient, which there is none of: call with its primal");
 }
 
 void shaped(const char* fn, const char* name, const at::Tensor& t, at::IntArrayRef shape) {

@@ -8,9 +8,9 @@ The formulas, layouts and limits are those of include/ssla_hip.h (sequence
 operators).  Calls are queued on torch's current stream of the tensors'
 device, which need not be the current device; outputs and workspaces come
 from torch's allocator, so calls can be captured into a graph.  Arguments that
-do not fit raise ValueError before anything is queued.  There is no backward
-pass: tensors that require a gradient are refused while torch records one.
-There is no fallback either: without the library, or for tensors off the GPU,
+do not fit raise ValueError before anything is queued.  There are no
+gradients: tensors that require one are refused while torch records, and so
+are tensors that carry a forward one.  There is no fallback either: without the library, or for tensors off the GPU,
 a call raises.
 
 The checks and the calls are in csrc/ops_torch.cpp (_ops.so).

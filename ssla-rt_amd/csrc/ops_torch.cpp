@@ -91,6 +91,12 @@ void alike(const char* fn, const char* name, const at::Tensor& t, at::ScalarType
         refuse(fn, std::string(name) + " carries a forward gradient, which there is none of: call with its primal");
 }
 
+// A call has written to t: autograd notices, should it have kept t.  Inference
+// tensors have no version.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void shaped(const char* fn, const char* name, const at::Tensor& t, at::IntArrayRef shape) {
     if (t.sizes() != shape)
         refuse(fn, std::string(name) + " must have the shape " + c10::str(shape) + ", not " + c10::str(t.sizes()));
@@ -220,6 +226,8 @@ at::Tensor linear_attention(const Args& a) {
     check(ssla_hip_linattn_workspace(&d, &bytes), "ssla_hip_linattn_workspace");
     const at::Tensor ws = workspace(dev, bytes);
     check(ssla_hip_linattn(&d, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(dev)), "ssla_hip_linattn");
+    written(out);
+    if (to) written(*to);
     return out;
 }
 
@@ -242,6 +250,8 @@ at::Tensor linear_attention_step(const Args& a) {
     else if (d.n_slots < d.n_seqs) refuse(fn, "there must be a state slot for every sequence");
     const c10::DeviceGuard guard(dev);
     check(ssla_hip_linattn_step(&d, stream_of(dev)), "ssla_hip_linattn_step");
+    written(out);
+    written(state);
     return out;
 }
 
@@ -309,6 +319,7 @@ at::Tensor group_norm(const Args& a) {
     check(ssla_hip_group_norm_workspace(&d, &bytes), "ssla_hip_group_norm_workspace");
     const at::Tensor ws = workspace(dev, bytes);
     check(ssla_hip_group_norm(&d, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(dev)), "ssla_hip_group_norm");
+    written(out);
     return out;
 }
 

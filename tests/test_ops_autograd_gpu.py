@@ -47,3 +47,34 @@ def test_function_transforms_raise(i):
         torch.func.grad(lambda x: f(**dict(kw, **{first: x})).sum())(kw[first])
     with pytest.raises((ValueError, RuntimeError)):
         torch.func.vmap(lambda x: f(**dict(kw, **{first: x})))(kw[first][None])
+
+
+@pytest.mark.parametrize("i,name", [(0, "out"), (0, "state_out"), (1, "out"), (1, "state"), (2, "out")])
+def test_a_saved_tensor_that_a_call_overwrites_is_noticed(i, name):
+    f, kw = calls()[i]
+    x = torch.randn_like(kw[name]).requires_grad_()
+    y = (x * kw[name]).sum()                   # keeps kw[name] for x's gradient
+    before = kw[name]._version
+    f(**kw)
+    assert kw[name]._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+@pytest.mark.parametrize("i", range(3), ids=["sequences", "step", "norm"])
+def test_tensors_that_are_only_read_keep_their_version(i):
+    f, kw = calls()[i]
+    before = {n: t._version for n, t in kw.items()}
+    f(**kw)
+    for n in kw:
+        assert (kw[n]._version == before[n]) == (n not in ("out", "state", "state_out")), n
+
+
+@pytest.mark.parametrize("i", range(3), ids=["sequences", "step", "norm"])
+def test_inference_tensors_are_taken(i):
+    with torch.inference_mode():
+        f, kw = calls()[i]
+        f(**kw)
+    assert kw["out"].is_inference()
+    want = f(**{n: t.clone() for n, t in kw.items()})
+    assert torch.equal(f(**kw), want)

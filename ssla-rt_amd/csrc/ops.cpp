@@ -89,7 +89,11 @@ int check_linattn(const SslaHipLinAttn* d, bool step, const char* fn) {
         if (!d->slots && d->n_slots < d->n_seqs) return refuse(f + "fewer slots than sequences");
         const uintptr_t a = (uintptr_t)d->state_in, b = (uintptr_t)d->state_out;
         const uintptr_t span = d->n_slots ? 4 * (uintptr_t)((d->n_slots - 1) * d->state_stride + state) : 0;
-        if (a && b && a != b && a < b + span && b < a + span)
+        // floats from a slot of the lower pool to the next one of the higher: the slots of
+        // two pools may lie in turn
+        const uintptr_t next = (a < b ? b - a : a - b) / 4 % (uintptr_t)d->state_stride;
+        const bool in_turn = next >= (uintptr_t)state && next + state <= (uintptr_t)d->state_stride;
+        if (a && b && a != b && a < b + span && b < a + span && !in_turn)
             return refuse(f + "state_in and state_out overlap without being the same");
     }
     return SSLA_OK;

@@ -7,6 +7,11 @@
   stub    weight-directory generator (tools/make_ssla_stub.py schema)
   events  seeded synthetic event / ring-record streams
 """
+from importlib.util import find_spec as _find
+
 from . import abi, events, stub  # noqa: F401  (no GPU needed)
 
-__all__ = ["abi", "events", "stub", "lib", "hybrid", "ops"]
+__all__ = ["abi", "events", "stub", "lib", "hybrid"]
+# the operators are on torch's tensors, and built where there is a torch
+if _find("torch") and _find(__name__ + "._ops"):
+    __all__.append("ops")

@@ -507,10 +507,10 @@ void group_norm_plan(GroupNormArgs& a, int dtype) {
     const long long np = ((long long)a.gb * cg + a.vec - 1) / a.vec + (cg % a.vec && a.blocks > 1 ? 1 : 0);
     a.np = (int)np;
     a.kind = kGroupOnePass;
-    for (int nt = 64; nt <= 1024; nt *= 4) {
+    for (int nt = 256; nt <= 1024; nt *= 4) {
         if (np > nt || group_norm_lds(a, nt, np) > 144 * 1024) continue;
         const long long reps = (a.rows + nt / np - 1) / (nt / np);
-        if (reps > (nt == 64 ? 1 : nt == 1024 && a.vec == 8 ? kWideReps<8> : 4)) continue;
+        if (reps > (nt == 1024 && a.vec == 8 ? kWideReps<8> : 4)) continue;
         a.threads = nt;
         a.reps = (int)reps;
         return;

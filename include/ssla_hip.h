@@ -458,7 +458,11 @@ int ssla_hip_oeva_diff(const char* path_a, const char* path_b, double tol_abs,
  * h / (heads / qk_heads)).  log_decay is fp32 at token * stride[0] + head *
  * stride[1]; stride[0] = 0 gives one decay for each head.  Values below -65536
  * count as -65536 (a decay of zero).
- * Sums, decays and states are fp32 or wider; out is rounded once.
+ * Sums, decays and states are fp32 or wider; out is rounded once.  Whole
+ * sequences multiply on the matrix cores, in operands of bf16 terms: tokens
+ * exactly (fp32 ones to 2^-26), the products of q and k within a chunk of
+ * tokens to 2^-26 (fp16 tokens: 2^-18), the state, where it multiplies q, to 2^-26
+ * (16-bit tokens: 2^-18 of each of its values; the state itself stays fp32).
  * An infinity or NaN in k or v reaches the outputs of its own token and those
  * behind it in its sequence (and its head, and for v its column), which are
  * then not finite; tokens before it and other sequences are unaffected.
@@ -473,8 +477,8 @@ int ssla_hip_oeva_diff(const char* path_a, const char* path_b, double tol_abs,
  *
  * state_in (NULL: zeros) and state_out (NULL: not kept) are pools of states:
  * sequence s reads and writes slot slots[s] (NULL: slot s), [heads][dk][dv]
- * floats at slot * state_stride.  They may be the same memory, or must not
- * overlap.  A sequence whose slot is negative or >= n_slots (a row that
+ * floats at slot * state_stride.  They may be the same memory, or no slot of
+ * one may overlap a slot of the other (their slots may lie in turn).  A sequence whose slot is negative or >= n_slots (a row that
  * pads a batch) is passed over: its out rows are left as they are.  Two
  * sequences of a call must not have the same slot (their states would
  * race).  out must not overlap an input. */
@@ -524,8 +528,9 @@ int ssla_hip_linattn_step(const SslaHipLinAttn* d, void* stream);
  *     out = act(y), or y * act(gate) where gate is set
  * Element (item, row, c) of x lies at item * stride[0] + row * stride[1] + c
  * (elements, >= 0), of gate and out likewise.  weight and bias (NULL: 1 and 0)
- * have the type of x.  Sums of squares are 64 bits wide, out is rounded once.  out may be x or gate itself,
- * else it must not overlap an input.  A NaN or infinity reaches its own
+ * have the type of x.  Sums are 64 bits wide, the mean is subtracted to 48 bits,
+ * out is rounded once; finite values of any size are taken.  out may be x or gate
+ * itself, else it must not overlap an input.  A NaN or infinity reaches its own
  * group of its own item only. */
 typedef struct SslaHipGroupNorm {
     int dtype;

@@ -514,7 +514,8 @@ void group_norm_plan(GroupNormArgs& a, int dtype) {
     // 96 channels in 24 groups (11 MB) 9.8 instead of 10.6, two such items 13.1
     // instead of 10.9.  Groups of whole lines: 256 tokens of 16384 fp32 channels in 8
     // groups 10.8 instead of 65, 64 items of 64 rows of 2048 bf16 channels in 16
-    // groups 16.8 instead of 22.6 (4096 such items, 2 GB, 762 instead of 684).
+    // groups 16.8 instead of 22.6.  The number of items is not looked at: 4096 such items,
+    // 2 GB, take 784 us, 684 by whole rows.
     // A piece a thread, or up to four (two) of 256 (1024) threads; more than 512
     // groups keep to 256 threads (256 tokens of 65536 bf16 channels in 16 groups: 31
     // us, with 1024 threads 60).

@@ -33,13 +33,13 @@
 // P are dealt over the waves and shared through LDS.
 //
 // 16 sequences of 8192 tokens, 16 heads of 128 in bf16 (2.1 GB, one workgroup a
-// compute unit) take 0.64 ms, 3.4 TB/s.  The loads and stores alone take 0.46 (a
-// large copy's rate: 0.42), the arithmetic alone 0.53, or 0.42 for each such batch
-// where two workgroups share a compute unit (then 0.57 in all).  A wave and
-// chunk issues some 250 vector instructions (mostly the splits into terms), 45
-// products, 44 LDS and 90 scalar ones; the vector units are busy for 45% of the
-// time, the matrix cores for 27%, LDS for 40%: what is left is the waits of a chunk's
-// phases for one another.  P one chunk ahead with one barrier fewer (two chunks in LDS)
+// compute unit) take 0.64 ms, 3.4 TB/s, a call among others whose inputs come from
+// memory (0.61 to 0.69 by card).  The loads and stores alone take 0.46 (a large copy's
+// rate: 0.42), the arithmetic alone 0.55, or 0.48 for each such batch where two
+// workgroups share a compute unit (then 0.59 in all).  A wave and chunk issues some
+// 250 vector instructions (mostly the splits into terms), 48 products, 44 LDS and 87
+// scalar ones; the vector units are busy for 47% of the time, the matrix cores for
+// 30%, LDS for 31%: what is left is the waits of a chunk's phases for one another.  P one chunk ahead with one barrier fewer (two chunks in LDS)
 // changed nothing.
 #pragma once
 

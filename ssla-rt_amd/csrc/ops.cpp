@@ -115,7 +115,7 @@ bool pieces(const void* p, const long long* s, long long width, size_t e) {
 // (200 tokens of 4 heads of 24: 11.9 us whole, 12.2 cut; 300 of 16 heads of 128:
 // 26 whole, 21 cut), and while none holds more than one and a half of a compute
 // unit's share of all tokens and heads (16 sequences of 8192 tokens, 16 heads of
-// 128, one workgroup a compute unit: 0.70 ms whole, 0.88 cut in two).  Else
+// 128, one workgroup a compute unit: 0.69 ms whole, 0.84 cut in two, on one card).  Else
 // segments are the smallest power of two, from 64 tokens on, that leaves a
 // sequence at most 128 (they are chained in turn: 20000 tokens of one head of 64,
 // 60 us in 313 segments, 38 in 79), and each of the 256 compute units two (one

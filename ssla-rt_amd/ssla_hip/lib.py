@@ -81,7 +81,7 @@ _SIGNATURES = {
                                 ctypes.c_uint]),
     "ssla_hip_oeva_diff": (_I, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_double,
                                 ctypes.POINTER(abi.SslaHipOevaDiff)]),
-    # descriptors by address: ops.py packs them (struct), abi.py mirrors them (ctypes)
+    # descriptors by address: abi.py mirrors them (ctypes), csrc/ops_torch.cpp fills them
     "ssla_hip_linattn_workspace": (_I, [_VP, ctypes.POINTER(ctypes.c_size_t)]),
     "ssla_hip_linattn": (_I, [_VP, _VP, ctypes.c_size_t, _VP]),
     "ssla_hip_linattn_step": (_I, [_VP, _VP]),

@@ -7,11 +7,13 @@
 The formulas, layouts and limits are those of include/ssla_hip.h (sequence
 operators).  Calls are queued on torch's current stream of the tensors'
 device, which need not be the current device; outputs and workspaces come
-from torch's allocator, so calls can be captured into a graph.  Arguments that
-do not fit raise ValueError before anything is queued.  There are no
-gradients: tensors that require one are refused while torch records, and so
-are tensors that carry a forward one.  There is no fallback either: without the library, or for tensors off the GPU,
-a call raises.
+from torch's allocator, so calls can be captured into a graph.  Tensors that do
+not fit raise ValueError, what the library refuses (values out of range, rows of
+out or pools that overlap) lib.SslaHipError, before anything is queued.  There
+are no gradients: tensors that require one are refused while torch records,
+and so are tensors that carry a forward one; tensors that a call writes to get
+a new version.  There is no fallback either: without the library, or for
+tensors off the GPU, a call raises.
 
 The checks and the calls are in csrc/ops_torch.cpp (_ops.so).
 """
@@ -46,7 +48,8 @@ def linear_attention(q, k, v, log_decay, out=None, *, scale: float = 1.0, cu_seq
                 (default: all tokens; a tight bound spares work).  None:
                 n_seqs sequences of the same length
     state_in, state_out  float32 (slots, heads, dk, dv) pools, read from
-                (None: zeros) and written to; may be the same
+                (None: zeros) and written to; may be the same (no slot of one
+                may overlap one of the other otherwise)
     slots       int32 (sequences,) slots of the sequences, each its own (None:
                 slot s for sequence s); a sequence with a negative slot is
                 passed over

@@ -177,8 +177,8 @@ __device__ __forceinline__ void write_state(const f4 (&S)[DT], const P& pl, cons
 // what lies past the rows or columns comes back as zero.  Where a thread's
 // pieces are whole rows apart, one offset serves them all.  Else (odd sizes,
 // strides or addresses): 16-byte loads at any alignment within the row.
-// 16 sequences of 2000 tokens, 16 heads of 127 in bf16: 220 us (by single values
-// 496; heads of 128 172).
+// 16 sequences of 2000 tokens, 16 heads of 127 in bf16: 204 us (heads of 128 184; by
+// single values the former took 496).
 template <class T, int W, int C, int NT, bool VEC>
 struct Rows {
     static constexpr int E = 16 / sizeof(T);               // elements of a piece

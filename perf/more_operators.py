@@ -126,7 +126,7 @@ def draw(rng):
     states = rng.random() < 0.5
     most = 55_000_000 // channels
     if rng.random() < 0.25:
-        seqs = _log_int(rng, 16, 20_000)
+        seqs = _log_int(rng, 16, min(20_000, most // 8))
         return _seq(None, op, dtype, seqs, max(1, min(most, seqs * _log_int(rng, 2, 600))), channels,
                     "cells", read, states, fused)
     seqs = _log_int(rng, 1, min(64, most))

@@ -434,8 +434,9 @@ int ssla_hip_oeva_diff(const char* path_a, const char* path_b, double tol_abs,
  * h = sigmoid(g) h + v read out by q * h, per channel and per grid cell; these
  * are the general forms for models around the drain: linear attention with a
  * decay for each head over token sequences of any length (whole prompts and
- * single tokens, with the state carried between calls) and group norm with
- * an activation over channels-last data.
+ * single tokens, with the state carried between calls), group norm with
+ * an activation over channels-last data, and, with their gradients, the layers'
+ * own recurrence and layer norm over packed rows.
  *
  * All pointers are device pointers on the calling thread's current device.
  * Every call only queues kernels on `stream` (hipStream_t or NULL): it
@@ -443,7 +444,8 @@ int ssla_hip_oeva_diff(const char* path_a, const char* path_b, double tol_abs,
  * nothing between calls, so it may be captured into a HIP graph.  A workspace
  * belongs to one call (or captured graph) at a time.  Tokens, rows and channels
  * are counted up to 2^31 - 2^16; a call that would need a grid of 2^32 threads
- * is refused.  There is no backward pass: nothing here is trained. */
+ * is refused.  The recurrence and layer norm have backward passes, linear
+ * attention and group norm have none. */
 #define SSLA_F32  0
 #define SSLA_BF16 1
 #define SSLA_F16  2
@@ -547,6 +549,119 @@ int ssla_hip_group_norm(const SslaHipGroupNorm* d, void* workspace, size_t works
 
 /* sizeof SslaHipLinAttn, sizeof SslaHipGroupNorm into out[0..1] (cap >= 2). */
 int ssla_hip_ops_layout(long long* out, int cap);
+
+/* The recurrence of an SSLA layer, channel by channel, with a gate for each
+ * token and channel:
+ *     h_t = sigmoid(gate_t) h_{t-1} + v_t,    out_t = q_t h_t   (h_t where q is NULL)
+ * gate, v, q and out are rows of tokens: element (token, c) lies at token *
+ * stride + c (strides in elements, >= 0).  States, gates and products are fp32,
+ * out is rounded once.  An infinity or NaN reaches the outputs of its own token
+ * and those behind it in its own sequence and channel only.
+ *
+ * Sequences are packed: sequence s holds the tokens cu_seqlens[s] up to
+ * cu_seqlens[s + 1] (n_seqs + 1 values in device memory, rising from >= 0 to
+ * <= n_tokens; values outside are clamped, so no call reads or writes past
+ * n_tokens rows), or, with cu_seqlens NULL, all have n_tokens / n_seqs tokens.
+ * A sequence may be empty: its state goes through.  Rows of out that belong to
+ * no sequence are left as they are.
+ *
+ * state_in (NULL: zeros) and state_out (NULL: not kept) are pools of states:
+ * sequence s reads and writes slot slots[s] (NULL: slot s), `channels` floats at
+ * slot * stride.  They may be the same memory (with the same stride), or no slot
+ * of one may overlap a slot of the other.  A sequence whose slot is negative or
+ * >= n_slots is passed over: its out rows are left as they are.  Two sequences
+ * of a call must not have the same slot.  out must not overlap an input.
+ *
+ * `carries` (NULL: not kept) takes what ssla_hip_linrec_backward needs besides
+ * the inputs: states at some of the tokens, ssla_hip_linrec_carries bytes. */
+typedef struct SslaHipLinRec {
+    int dtype;                 /* of gate, v, q and out */
+    int channels;              /* >= 1 */
+    int n_seqs, n_slots;
+    long long n_tokens;
+    const void *gate, *v, *q;
+    void* out;
+    long long gate_stride, v_stride, q_stride, out_stride;
+    const int* cu_seqlens;
+    const int* slots;
+    const float* state_in;
+    float* state_out;
+    long long state_in_stride, state_out_stride;     /* floats, >= channels */
+    float* carries;
+} SslaHipLinRec;
+
+/* Gradients of the call *d that kept its carries, from those of out and of the
+ * last states (NULL: zeros):
+ *     dh_t = q_t dout_t + sigmoid(gate_{t+1}) dh_{t+1}   (the last token: + dstate_out)
+ *     dv_t = dh_t,    dq_t = dout_t h_t,    dstate_in = sigmoid(gate_first) dh_first
+ *     dgate_t = dh_t h_{t-1} sigmoid(gate_t) (1 - sigmoid(gate_t))
+ * dout, dgate, dv and dq are rows of tokens of d's type, dstate_out and dstate_in
+ * rows of sequences; each of the four outputs may be NULL: not wanted.  Rows
+ * that belong to no sequence get zeros.  d->slots must be NULL; d->out,
+ * d->state_out are not looked at.  No output may overlap an input. */
+typedef struct SslaHipLinRecGrad {
+    const void* dout;
+    const float* dstate_out;
+    void *dgate, *dv, *dq;
+    float* dstate_in;
+    long long dout_stride, dstate_out_stride, dgate_stride, dv_stride, dq_stride, dstate_in_stride;
+} SslaHipLinRecGrad;
+
+/* Bytes of `carries`, and of the workspace that ssla_hip_linrec and
+ * ssla_hip_linrec_backward each need for *d; they depend on dtype, channels,
+ * n_tokens, n_seqs and whether there are cu_seqlens. */
+int ssla_hip_linrec_carries(const SslaHipLinRec* d, size_t* nbytes);
+int ssla_hip_linrec_workspace(const SslaHipLinRec* d, size_t* nbytes);
+int ssla_hip_linrec(const SslaHipLinRec* d, void* workspace, size_t workspace_bytes, void* stream);
+int ssla_hip_linrec_backward(const SslaHipLinRec* d, const SslaHipLinRecGrad* g, void* workspace,
+                             size_t workspace_bytes, void* stream);
+/* One token of every sequence: row s of gate, v, q and out belongs to sequence
+ * s, whose state is read from state_in and written to state_out (both needed;
+ * usually the same pool).  n_tokens, cu_seqlens and carries are not used. */
+int ssla_hip_linrec_step(const SslaHipLinRec* d, void* stream);
+
+/* Layer norm of the rows of s = x + residual (residual NULL: x):
+ *     out = (s - mean) / sqrt(var + eps) * weight_c + bias_c
+ * Element (row, c) of x lies at row * x_stride + c (elements, >= 0), of residual
+ * and out likewise.  weight and bias (NULL: 1 and 0) are of weight_dtype, which
+ * is dtype or SSLA_F32.  x + residual is an fp32 sum, mean and variance are 64
+ * bits wide, the mean is subtracted to 48 bits, out is rounded once.  out may be
+ * x or residual itself, else it must not overlap an input.  `stats` (NULL: not
+ * kept) takes three floats a row for the backward pass. */
+typedef struct SslaHipLayerNorm {
+    int dtype, weight_dtype;
+    int rows, channels;
+    const void *x, *residual, *weight, *bias;
+    void* out;
+    long long x_stride, residual_stride, out_stride;
+    float* stats;
+    float eps;
+} SslaHipLayerNorm;
+
+/* Gradients of the call *d that kept its stats; with xh the normed rows and
+ * u = weight dout:
+ *     dx = (u - mean(u) - xh mean(u xh)) / sqrt(var + eps)    (of x and of residual)
+ *     dweight = sum over rows of dout xh,    dbias = sum over rows of dout
+ * dout and dx are rows of d's type, dweight and dbias of weight_dtype; each
+ * output may be NULL: not wanted.  Row sums are taken in a fixed order.  d->out
+ * and d->bias are not looked at.  No output may overlap an input. */
+typedef struct SslaHipLayerNormGrad {
+    const void* dout;
+    void *dx, *dweight, *dbias;
+    long long dout_stride, dx_stride;
+} SslaHipLayerNormGrad;
+
+int ssla_hip_layer_norm(const SslaHipLayerNorm* d, void* stream);
+/* Bytes of workspace of the backward pass (it depends on dtype, rows, channels
+ * and whether dweight or dbias are wanted). */
+int ssla_hip_layer_norm_backward_workspace(const SslaHipLayerNorm* d, const SslaHipLayerNormGrad* g,
+                                           size_t* nbytes);
+int ssla_hip_layer_norm_backward(const SslaHipLayerNorm* d, const SslaHipLayerNormGrad* g,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* sizeof SslaHipLinRec, SslaHipLinRecGrad, SslaHipLayerNorm and
+ * SslaHipLayerNormGrad into out[0..3] (cap >= 4). */
+int ssla_hip_train_layout(long long* out, int cap);
 
 #ifdef __cplusplus
 }

@@ -1,49 +1,14 @@
 // ops.cpp -- C ABI of the sequence operators (include/ssla_hip.h): argument
 // checks, how a call is cut into workgroups, launches.
-#include <hip/hip_runtime.h>
-
-#include <cstdint>
 #include <exception>
 #include <string>
 
-#include "drain_scan.h"
 #include "groupnorm.h"
 #include "linattn.h"
-#include "ssla_hip.h"
+#include "ops_check.h"
 
 namespace ssla {
 namespace {
-
-int refuse(const std::string& msg) {
-    set_error(msg);
-    return SSLA_ERR_ARG;
-}
-
-int hip_failed(const char* what, hipError_t e) {
-    set_error(std::string(what) + ": " + hipGetErrorString(e));
-    return SSLA_ERR_HIP;
-}
-
-size_t element(int dtype) { return dtype == SSLA_F32 ? 4 : 2; }
-
-bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
-// Whether n0 x n1 pieces of `width` elements at strides s0, s1 are apart.
-bool apart(long long n0, long long s0, long long n1, long long s1, long long width) {
-    if (n0 <= 1) return n1 <= 1 || s1 >= width;
-    if (n1 <= 1) return s0 >= width;
-    if (s0 < s1) return s0 >= width && (s1 - width) / s0 >= n0 - 1;
-    return s1 >= width && (s0 - width) / s1 >= n1 - 1;
-}
-
-// Whether a launch of a * b * c workgroups fits: HIP counts a grid's threads in 32 bits.
-bool launchable(long long a, long long b, long long c, int threads) {
-    return (__int128)a * b * c <= 0xffffffffll / threads;
-}
-
-// Kernels count tokens, rows and channels in 32 bits and step past the last one.
-constexpr int kMaxCount = 0x7fff0000;
-constexpr long long kMaxStride = 1ll << 40;      // offsets stay within 64 bits
 
 // ---- linear attention ----------------------------------------------------------
 

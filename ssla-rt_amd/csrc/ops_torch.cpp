@@ -5,102 +5,13 @@
 //
 // The same in Python over ctypes took 10 to 12.5 us a call, twice what the small
 // calls take on the GPU; here one takes 5 to 6.
-#include <torch/csrc/autograd/python_variable.h>
+#include "ops_torch.h"
 
-#include <ATen/core/grad_mode.h>
-#include <ATen/ops/empty.h>
-#include <c10/core/AutogradState.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
+namespace ssla_torch {
 
-#include <stdexcept>
-#include <string>
-
-#include "ssla_hip.h"
+PyObject* g_error = nullptr;
 
 namespace {
-
-PyObject* g_error = nullptr;     // ssla_hip.lib.SslaHipError
-
-[[noreturn]] void refuse(const char* fn, const std::string& what) {
-    throw std::invalid_argument(std::string(fn) + ": " + what);
-}
-
-struct LibraryError : std::runtime_error {
-    using std::runtime_error::runtime_error;
-};
-
-void check(int rc, const char* entry) {
-    if (rc < 0)
-        throw LibraryError(std::string(entry) + " failed (" + std::to_string(rc) + "): " + ssla_hip_last_error());
-}
-
-// The arguments of a call, which ops.py passes by position.
-struct Args {
-    const char* fn;
-    PyObject* const* v;
-
-    const at::Tensor& tensor(int i, const char* name) const {
-        if (!THPVariable_Check(v[i])) refuse(fn, std::string(name) + " must be a tensor");
-        return THPVariable_Unpack(v[i]);
-    }
-    const at::Tensor* optional(int i, const char* name) const {
-        return v[i] == Py_None ? nullptr : &tensor(i, name);
-    }
-    long long integer(int i, const char* name) const {
-        const long long x = PyLong_AsLongLong(v[i]);
-        if (x == -1 && PyErr_Occurred()) {
-            PyErr_Clear();
-            refuse(fn, std::string(name) + " must be an integer");
-        }
-        return x;
-    }
-    int count(int i, const char* name) const {
-        const long long x = integer(i, name);
-        if (x < 0 || x > 0x7fffffff) refuse(fn, std::string(name) + " must be 0 .. 2^31 - 1");
-        return (int)x;
-    }
-    double real(int i, const char* name) const {
-        const double x = PyFloat_AsDouble(v[i]);
-        if (x == -1.0 && PyErr_Occurred()) {
-            PyErr_Clear();
-            refuse(fn, std::string(name) + " must be a number");
-        }
-        return x;
-    }
-};
-
-int dtype_of(const char* fn, const char* name, const at::Tensor& t) {
-    if (!t.is_cuda()) refuse(fn, std::string(name) + " must be on a GPU");
-    switch (t.scalar_type()) {
-        case at::kFloat: return SSLA_F32;
-        case at::kBFloat16: return SSLA_BF16;
-        case at::kHalf: return SSLA_F16;
-        default: refuse(fn, std::string(name) + " must be float32, bfloat16 or float16");
-    }
-}
-
-// Type and device of a tensor of the call; there are no gradients, backward or forward.
-void alike(const char* fn, const char* name, const at::Tensor& t, at::ScalarType type, at::Device dev) {
-    if (t.scalar_type() != type || t.device() != dev || t.layout() != at::kStrided)
-        refuse(fn, std::string(name) + " must be a " + c10::toString(type) + " tensor on " + dev.str());
-    if (t.is_neg()) refuse(fn, std::string(name) + " is a negated view: call resolve_neg()");
-    if (t.requires_grad() && at::GradMode::is_enabled())
-        refuse(fn, std::string(name) + " requires a gradient, which there is none of: call under torch.no_grad()");
-    if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
-        refuse(fn, std::string(name) + " carries a forward gradient, which there is none of: call with its primal");
-}
-
-// A call has written to t: autograd notices, should it have kept t.  Inference
-// tensors have no version.
-void written(const at::Tensor& t) {
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-
-void shaped(const char* fn, const char* name, const at::Tensor& t, at::IntArrayRef shape) {
-    if (t.sizes() != shape)
-        refuse(fn, std::string(name) + " must have the shape " + c10::str(shape) + ", not " + c10::str(t.sizes()));
-}
 
 // (tokens, heads, size) with the last dimension contiguous: strides of the others.
 void rows(const char* fn, const char* name, const at::Tensor& t, at::ScalarType type, at::Device dev,
@@ -124,13 +35,6 @@ long long pool(const char* fn, const char* name, const at::Tensor& t, at::Device
         refuse(fn, std::string(name) + ": a slot must be contiguous");
     if (t.size(0) > 0x7fffffff) refuse(fn, std::string(name) + " has too many slots");
     return t.size(0) > 1 ? t.stride(0) : slot;
-}
-
-const int* index(const char* fn, const char* name, const at::Tensor& t, at::Device dev, int64_t n) {
-    alike(fn, name, t, at::kInt, dev);
-    if (t.dim() != 1 || t.size(0) != n || (n > 1 && t.stride(0) != 1))
-        refuse(fn, std::string(name) + " must be " + std::to_string(n) + " contiguous int32 values");
-    return t.const_data_ptr<int>();
 }
 
 // q, k, v, log_decay and out of a call; out is made where there is none.
@@ -172,12 +76,6 @@ at::Tensor tokens(const char* fn, SslaHipLinAttn& d, const at::Tensor& q, const 
     d.log_decay = g.const_data_ptr<float>();
     d.out = o.mutable_data_ptr();
     return o;
-}
-
-void* stream_of(at::Device dev) { return c10::hip::getCurrentHIPStream(dev.index()).stream(); }
-
-at::Tensor workspace(at::Device dev, size_t bytes) {
-    return bytes ? at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(dev)) : at::Tensor();
 }
 
 // linear_attention(q, k, v, log_decay, out, scale, cu_seqlens, max_len, n_seqs, state_in, state_out, slots)
@@ -323,24 +221,6 @@ at::Tensor group_norm(const Args& a) {
     return out;
 }
 
-// C++ exceptions end here, as Python ones.
-template <at::Tensor (*F)(const Args&)>
-PyObject* call(const char* fn, int want, PyObject* const* v, Py_ssize_t n) {
-    try {
-        if (n != want) refuse(fn, "wrong number of arguments");
-        return THPVariable_Wrap(F(Args{fn, v}));
-    } catch (const std::invalid_argument& e) {
-        PyErr_SetString(PyExc_ValueError, e.what());
-    } catch (const LibraryError& e) {
-        PyErr_SetString(g_error, e.what());
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-    } catch (...) {
-        PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
-    }
-    return nullptr;
-}
-
 PyObject* py_linear_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
     return call<linear_attention>("linear_attention", 12, v, n);
 }
@@ -355,11 +235,17 @@ PyMethodDef g_methods[] = {
     {"linear_attention", (PyCFunction)(void (*)())py_linear_attention, METH_FASTCALL, nullptr},
     {"linear_attention_step", (PyCFunction)(void (*)())py_linear_attention_step, METH_FASTCALL, nullptr},
     {"group_norm", (PyCFunction)(void (*)())py_group_norm, METH_FASTCALL, nullptr},
+    {"linear_recurrence", (PyCFunction)(void (*)())py_linear_recurrence, METH_FASTCALL, nullptr},
+    {"linear_recurrence_step", (PyCFunction)(void (*)())py_linear_recurrence_step, METH_FASTCALL, nullptr},
+    {"layer_norm", (PyCFunction)(void (*)())py_layer_norm, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
+}  // namespace ssla_torch
+
+using namespace ssla_torch;
 
 PyMODINIT_FUNC PyInit__ops(void) {
     PyObject* lib = PyImport_ImportModule("ssla_hip.lib");

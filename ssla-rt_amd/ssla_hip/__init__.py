@@ -2,7 +2,8 @@
 
   abi     numpy / ctypes mirrors of include/ssla_abi.h
   lib     ctypes binding of libssla_hip.so (include/ssla_hip.h)
-  ops     sequence operators on torch tensors: linear attention, group norm
+  ops     sequence operators on torch tensors: linear attention, group norm, and,
+          with gradients, the layers' recurrence and layer norm
   hybrid  device buffers, weight packing, HybridS2S3Config, drain calls
   stub    weight-directory generator (tools/make_ssla_stub.py schema)
   events  seeded synthetic event / ring-record streams

@@ -147,6 +147,35 @@ class SslaHipGroupNorm(ctypes.Structure):
         ("eps", ctypes.c_float)]
 
 
+class SslaHipLinRec(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("dtype", "channels", "n_seqs", "n_slots")] + [
+        ("n_tokens", ctypes.c_longlong)] + [
+        (n, ctypes.c_void_p) for n in ("gate", "v", "q", "out")] + [
+        (n, ctypes.c_longlong) for n in ("gate_stride", "v_stride", "q_stride", "out_stride")] + [
+        (n, ctypes.c_void_p) for n in ("cu_seqlens", "slots", "state_in", "state_out")] + [
+        (n, ctypes.c_longlong) for n in ("state_in_stride", "state_out_stride")] + [
+        ("carries", ctypes.c_void_p)]
+
+
+class SslaHipLinRecGrad(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("dout", "dstate_out", "dgate", "dv", "dq", "dstate_in")] + [
+        (n + "_stride", ctypes.c_longlong) for n in
+        ("dout", "dstate_out", "dgate", "dv", "dq", "dstate_in")]
+
+
+class SslaHipLayerNorm(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("dtype", "weight_dtype", "rows", "channels")] + [
+        (n, ctypes.c_void_p) for n in ("x", "residual", "weight", "bias", "out")] + [
+        (n, ctypes.c_longlong) for n in ("x_stride", "residual_stride", "out_stride")] + [
+        ("stats", ctypes.c_void_p), ("eps", ctypes.c_float)]
+
+
+class SslaHipLayerNormGrad(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dout", "dx", "dweight", "dbias")] + [
+        (n, ctypes.c_longlong) for n in ("dout_stride", "dx_stride")]
+
+
 # return codes of the C ABI (include/ssla_hip.h)
 SSLA_OK, SSLA_ERR_ARG, SSLA_ERR_HIP, SSLA_ERR_IO, SSLA_ERR_FORMAT, SSLA_ERR_STATE = 0, -1, -2, -3, -4, -5
 

@@ -88,6 +88,15 @@ _SIGNATURES = {
     "ssla_hip_group_norm_workspace": (_I, [_VP, ctypes.POINTER(ctypes.c_size_t)]),
     "ssla_hip_group_norm": (_I, [_VP, _VP, ctypes.c_size_t, _VP]),
     "ssla_hip_ops_layout": (_I, [ctypes.POINTER(_LL), _I]),
+    "ssla_hip_linrec_carries": (_I, [_VP, ctypes.POINTER(ctypes.c_size_t)]),
+    "ssla_hip_linrec_workspace": (_I, [_VP, ctypes.POINTER(ctypes.c_size_t)]),
+    "ssla_hip_linrec": (_I, [_VP, _VP, ctypes.c_size_t, _VP]),
+    "ssla_hip_linrec_backward": (_I, [_VP, _VP, _VP, ctypes.c_size_t, _VP]),
+    "ssla_hip_linrec_step": (_I, [_VP, _VP]),
+    "ssla_hip_layer_norm": (_I, [_VP, _VP]),
+    "ssla_hip_layer_norm_backward_workspace": (_I, [_VP, _VP, ctypes.POINTER(ctypes.c_size_t)]),
+    "ssla_hip_layer_norm_backward": (_I, [_VP, _VP, _VP, ctypes.c_size_t, _VP]),
+    "ssla_hip_train_layout": (_I, [ctypes.POINTER(_LL), _I]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

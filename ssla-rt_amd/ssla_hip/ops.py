@@ -3,19 +3,27 @@
   linear_attention       whole sequences (packed, ragged), states in and out
   linear_attention_step  one token of every sequence, states updated in a pool
   group_norm             group norm with an activation, channels last
+  linear_recurrence      an SSLA layer's recurrence over whole sequences (packed,
+                         ragged), states in and out, with gradients
+  linear_recurrence_step  its single tokens, states updated in a pool
+  layer_norm             layer norm, of a sum with a residual too, with gradients
 
 The formulas, layouts and limits are those of include/ssla_hip.h (sequence
 operators).  Calls are queued on torch's current stream of the tensors'
 device, which need not be the current device; outputs and workspaces come
 from torch's allocator, so calls can be captured into a graph.  Tensors that do
 not fit raise ValueError, what the library refuses (values out of range, rows of
-out or pools that overlap) lib.SslaHipError, before anything is queued.  There
-are no gradients: tensors that require one are refused while torch records,
-and so are tensors that carry a forward one; tensors that a call writes to get
-a new version.  There is no fallback either: without the library, or for
-tensors off the GPU, a call raises.
+out or pools that overlap) lib.SslaHipError, before anything is queued.
+linear_recurrence and layer_norm are functions of torch's autograd: where it
+records, their outputs are new tensors with first derivatives (second ones are
+refused), and a call in a capture refuses leaves whose older graph, recorded on
+the default stream, still lives.  The others have no gradients: tensors that
+require one are refused while torch records.  Tensors that carry a forward gradient
+are refused everywhere; tensors that a call writes to get a new version.  There is
+no fallback: without the library, or for tensors off the GPU, a call raises.
 
-The checks and the calls are in csrc/ops_torch.cpp (_ops.so).
+The checks and the calls are in csrc/ops_torch.cpp and csrc/ops_train_torch.cpp
+(_ops.so).
 """
 from __future__ import annotations
 
@@ -80,3 +88,49 @@ def group_norm(x, groups: int, weight=None, bias=None, out=None, *, eps: float =
     if act not in _ACTS:
         raise ValueError(f"group_norm: act must be one of {[a for a in _ACTS if a]}")
     return _ops.group_norm(x, groups, weight, bias, out, eps, _ACTS[act], gate)
+
+
+def linear_recurrence(gate, v, q=None, out=None, *, cu_seqlens=None, n_seqs: int = 1,
+                      state_in=None, state_out=None, slots=None, return_state: bool = False):
+    """h_t = sigmoid(gate_t) h_{t-1} + v_t, out_t = q_t h_t (h_t without q),
+    channel by channel, over packed sequences.
+
+    gate, v, q  (tokens, channels): any stride between tokens, channels contiguous
+    cu_seqlens  int32 (sequences + 1,) on the device: the sequences' first
+                tokens and the last one's end.  None: n_seqs sequences of the
+                same length
+    state_in, state_out  float32 (slots, channels) pools, read from (None: zeros)
+                and written to; may be the same (no slot of one may overlap one of
+                the other otherwise)
+    slots       int32 (sequences,) slots of the sequences, each its own (None:
+                slot s for sequence s); a sequence with a negative slot is
+                passed over
+    return_state  the sequences' last states come with out, float32
+                (sequences, channels), in place of state_out
+    Returns out (tokens, channels) in gate's type, or (out, state).  Rows of no
+    sequence are left as they are (uninitialised where out is made here).
+
+    Where torch records a gradient of gate, v, q or state_in (one row for each
+    sequence then), out, state_out and slots must be None; rows of no sequence are
+    zeros, and so are their gradients."""
+    got = _ops.linear_recurrence(gate, v, q, out, cu_seqlens, n_seqs, state_in, state_out, slots,
+                                 return_state)
+    return got if return_state else got[0]
+
+
+def linear_recurrence_step(gate, v, state, q=None, out=None, *, slots=None) -> torch.Tensor:
+    """One token of every sequence: row s of gate, v and q (sequences, channels)
+    belongs to sequence s.  Its state, slot slots[s] (None: s) of `state` (float32
+    (slots, channels)), is updated in place; out[s] is read from the new one.  A
+    row with a negative slot is passed over.  Returns out."""
+    return _ops.linear_recurrence_step(gate, v, state, q, out, slots)
+
+
+def layer_norm(x, weight=None, bias=None, out=None, *, eps: float = 1e-5,
+               residual=None) -> torch.Tensor:
+    """Layer norm of x, or of x + residual, over the last dimension: (s - mean) /
+    sqrt(var + eps) * weight + bias.  x (..., channels) and residual (of x's
+    shape): channels contiguous, rows at one stride.  weight, bias (channels,)
+    in x's type or both in float32.  out may be x or residual.  Returns out (x's
+    shape and type).  Where torch records a gradient, out must be None."""
+    return _ops.layer_norm(x, weight, bias, out, eps, residual)

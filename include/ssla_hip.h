@@ -563,7 +563,8 @@ int ssla_hip_ops_layout(long long* out, int cap);
  * <= n_tokens; values outside are clamped, so no call reads or writes past
  * n_tokens rows), or, with cu_seqlens NULL, all have n_tokens / n_seqs tokens.
  * A sequence may be empty: its state goes through.  Rows of out that belong to
- * no sequence are left as they are.
+ * no sequence are left as they are.  All tokens are scanned at once, whatever
+ * the sequences' number and lengths.
  *
  * state_in (NULL: zeros) and state_out (NULL: not kept) are pools of states:
  * sequence s reads and writes slot slots[s] (NULL: slot s), `channels` floats at
@@ -573,7 +574,9 @@ int ssla_hip_ops_layout(long long* out, int cap);
  * of a call must not have the same slot.  out must not overlap an input.
  *
  * `carries` (NULL: not kept) takes what ssla_hip_linrec_backward needs besides
- * the inputs: states at some of the tokens, ssla_hip_linrec_carries bytes. */
+ * the inputs: states at some of the tokens, ssla_hip_linrec_carries bytes.  With
+ * it, rows of out that belong to no sequence get zeros (a loss over all rows
+ * stays finite). */
 typedef struct SslaHipLinRec {
     int dtype;                 /* of gate, v, q and out */
     int channels;              /* >= 1 */

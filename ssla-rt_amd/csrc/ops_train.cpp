@@ -55,7 +55,7 @@ int check_linrec(const SslaHipLinRec* d, Call call, const char* fn) {
         tokens = d->n_tokens;
     }
     const size_t e = element(d->dtype);
-    if (tokens > 0 && d->n_seqs > 0) {
+    if (tokens > 0) {
         if (!d->gate || !d->v || (writes && !d->out)) return refuse(f + "null tensor");
         if (writes) {
             if (tokens > 1 && d->out_stride < d->channels) return refuse(f + "rows of out overlap");
@@ -111,6 +111,7 @@ LinRecArgs linrec_args(const SslaHipLinRec* d, const SslaHipLinRecGrad* g) {
     a.s_in = d->state_in, a.s_out = d->state_out, a.si = d->state_in_stride, a.so = d->state_out_stride;
     a.carries = d->carries;
     a.n_tokens = d->n_tokens, a.n_seqs = d->n_seqs, a.n_slots = d->n_slots, a.channels = d->channels;
+    if (!d->slots && !d->state_in && !d->state_out) a.n_slots = d->n_seqs;
     a.seq_len = d->n_seqs ? (int)(d->n_tokens / d->n_seqs) : 0;
     if (g) {
         a.out = nullptr, a.s_out = nullptr;
@@ -121,6 +122,21 @@ LinRecArgs linrec_args(const SslaHipLinRec* d, const SslaHipLinRecGrad* g) {
     }
     linrec_plan(a, d->dtype);
     return a;
+}
+
+// The grid's limit, and the workspace.
+int linrec_bind(LinRecArgs& a, void* workspace, size_t bytes, const char* fn) {
+    if (!launchable(a.tiles, a.blocks, 1, kLinRecThreads) ||
+        !launchable((long long)a.tiles * a.blocks + a.n_seqs / kLinRecThreads + 1, 1, 1, kLinRecThreads) ||
+        !launchable((long long)linrec_words(a) + kLinRecThreads, 1, 1, 1))
+        return refuse(std::string(fn) + ": too many tokens and channels");
+    const size_t need = linrec_bytes(a);
+    if (!need) return SSLA_OK;
+    if (!workspace || bytes < need || !aligned(workspace, 16))
+        return refuse(std::string(fn) + ": the workspace is missing, too small or not 16-byte aligned");
+    a.words = (unsigned long long*)workspace;
+    a.tickets = (unsigned*)(a.words + linrec_words(a));
+    return SSLA_OK;
 }
 
 // ---- layer norm --------------------------------------------------------------------
@@ -216,32 +232,33 @@ int ssla_hip_linrec_carries(const SslaHipLinRec* d, size_t* nbytes) try {
 int ssla_hip_linrec_workspace(const SslaHipLinRec* d, size_t* nbytes) try {
     if (!nbytes) return refuse("ssla_hip_linrec_workspace: null argument");
     *nbytes = 0;
-    return check_linrec(d, kSizes, "ssla_hip_linrec_workspace");
+    if (const int rc = check_linrec(d, kSizes, "ssla_hip_linrec_workspace")) return rc;
+    *nbytes = linrec_bytes(linrec_args(d, nullptr));
+    return SSLA_OK;
 } catch (const std::exception&) {
     return SSLA_ERR_ARG;
 }
 
 int ssla_hip_linrec(const SslaHipLinRec* d, void* workspace, size_t workspace_bytes, void* stream) try {
-    if (const int rc = check_linrec(d, kForward, "ssla_hip_linrec")) return rc;
-    if (d->n_seqs == 0) return SSLA_OK;
-    const LinRecArgs a = linrec_args(d, nullptr);
-    if (!launchable(a.n_seqs, a.channels, 1, 1) || !launchable(a.n_tokens, a.channels, 1, 1))
-        return refuse("ssla_hip_linrec: too many tokens and channels");
+    const char* fn = "ssla_hip_linrec";
+    if (const int rc = check_linrec(d, kForward, fn)) return rc;
+    LinRecArgs a = linrec_args(d, nullptr);
+    if (const int rc = linrec_bind(a, workspace, workspace_bytes, fn)) return rc;
     const hipError_t e = linrec_launch(a, d->dtype, (hipStream_t)stream);
-    return e == hipSuccess ? SSLA_OK : hip_failed("ssla_hip_linrec", e);
+    return e == hipSuccess ? SSLA_OK : hip_failed(fn, e);
 } catch (const std::exception&) {
     return SSLA_ERR_HIP;
 }
 
 int ssla_hip_linrec_backward(const SslaHipLinRec* d, const SslaHipLinRecGrad* g, void* workspace,
                              size_t workspace_bytes, void* stream) try {
-    if (const int rc = check_linrec(d, kBackward, "ssla_hip_linrec_backward")) return rc;
+    const char* fn = "ssla_hip_linrec_backward";
+    if (const int rc = check_linrec(d, kBackward, fn)) return rc;
     if (const int rc = check_linrec_grad(d, g)) return rc;
-    const LinRecArgs a = linrec_args(d, g);
-    if (!launchable(a.n_seqs, a.channels, 1, 1) || !launchable(a.n_tokens, a.channels, 1, 1))
-        return refuse("ssla_hip_linrec_backward: too many tokens and channels");
+    LinRecArgs a = linrec_args(d, g);
+    if (const int rc = linrec_bind(a, workspace, workspace_bytes, fn)) return rc;
     const hipError_t e = linrec_launch_backward(a, d->dtype, (hipStream_t)stream);
-    return e == hipSuccess ? SSLA_OK : hip_failed("ssla_hip_linrec_backward", e);
+    return e == hipSuccess ? SSLA_OK : hip_failed(fn, e);
 } catch (const std::exception&) {
     return SSLA_ERR_HIP;
 }
@@ -249,8 +266,9 @@ int ssla_hip_linrec_backward(const SslaHipLinRec* d, const SslaHipLinRecGrad* g,
 int ssla_hip_linrec_step(const SslaHipLinRec* d, void* stream) try {
     if (const int rc = check_linrec(d, kStep, "ssla_hip_linrec_step")) return rc;
     if (d->n_seqs == 0) return SSLA_OK;
-    LinRecArgs a = linrec_args(d, nullptr);
-    if (!launchable(a.n_seqs, a.channels, 1, 1)) return refuse("ssla_hip_linrec_step: too many sequences and channels");
+    const LinRecArgs a = linrec_args(d, nullptr);
+    if (!launchable((long long)a.n_seqs * a.channels + kLinRecThreads, 1, 1, 1))
+        return refuse("ssla_hip_linrec_step: too many sequences and channels");
     const hipError_t e = linrec_launch_step(a, d->dtype, (hipStream_t)stream);
     return e == hipSuccess ? SSLA_OK : hip_failed("ssla_hip_linrec_step", e);
 } catch (const std::exception&) {

@@ -4,7 +4,6 @@
 // that records takes as long as one that does not, plus autograd's own node.
 #include "ops_torch.h"
 
-#include <ATen/ops/zeros.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/variable.h>
@@ -159,9 +158,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
         const at::Tensor q = plain(maybe_q), state_in = plain(maybe_in), cu = plain(maybe_cu);
         SslaHipLinRec d = describe(gate, v, q, state_in, cu, n_seqs);
         const auto dev = gate.device();
-        // rows of no sequence: a loss over all of them stays finite
-        const at::Tensor out = cu.defined() ? at::zeros(gate.sizes(), gate.options().requires_grad(false))
-                                            : new_rows(gate, d.n_tokens, gate.scalar_type());
+        const at::Tensor out = new_rows(gate, d.n_tokens, gate.scalar_type());
         d.out = out.mutable_data_ptr();
         d.out_stride = d.channels;
         at::Tensor state;

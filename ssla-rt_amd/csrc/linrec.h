@@ -19,7 +19,7 @@ struct LinRecArgs {
     const float* s_in;
     float* s_out;
     long long si, so;                     // floats between slots
-    float* carries;                       // [tile][channels] states before a tile's first token
+    float* carries;                       // [token / carry][channels] states before every carry-th token
     // backward
     const void* dout;
     const float* ds_out;
@@ -33,41 +33,42 @@ struct LinRecArgs {
     int vec;                              // channels of a thread
     int cols, blocks;                     // threads along the channels; workgroups along them
     int lanes, tile, tiles;               // threads along the tokens, their tokens, tiles of all tokens
+    int carry;                            // tokens of a tile of the backward pass
     unsigned* tickets;                    // workspace: a counter for each block of channels
-    unsigned long long* words;            // [place in the chain][block][cols * vec] maps and states
+    unsigned long long* words;            // [block][kBehind + place in the chain][kChannels] maps and states
 };
 
 constexpr int kLinRecThreads = 256;
+constexpr int kChannels = 64;             // most of a workgroup
 constexpr int kTicketStep = 32;           // counters lie 128 bytes apart
+constexpr int kBehind = 32;               // places before a chain's first one, never published
 
-void linrec_plan(LinRecArgs& a, int dtype);
+void linrec_plan(LinRecArgs& a, int dtype, bool backward);
 // Workspace: 0 where one tile holds all tokens.
 inline size_t linrec_words(const LinRecArgs& a) {
-    return a.tiles > 1 ? (size_t)a.tiles * a.blocks * a.cols * a.vec : 0;
+    return a.tiles > 1 ? ((size_t)a.tiles + kBehind) * a.blocks * kChannels : 0;
 }
 inline size_t linrec_bytes(const LinRecArgs& a) {
     return a.tiles > 1 ? linrec_words(a) * 8 + (size_t)a.blocks * kTicketStep * 4 : 0;
+}
+inline size_t linrec_carries(const LinRecArgs& a) {
+    return (size_t)((a.n_tokens + a.carry - 1) / a.carry) * a.channels * 4;
 }
 hipError_t linrec_launch(const LinRecArgs& a, int dtype, hipStream_t st);
 hipError_t linrec_launch_backward(const LinRecArgs& a, int dtype, hipStream_t st);
 hipError_t linrec_launch_step(const LinRecArgs& a, int dtype, hipStream_t st);
 
 #ifdef __HIPCC__
-// A gate a = sigmoid(x) as one float c: the smaller of a and 1 - a, s = sigmoid(-|x|),
-// to a few roundings of itself, negative where it is 1 - a (x > 0).  An open gate
-// keeps the digits of what it forgets, a closed one those of what it lets through.
-__device__ __forceinline__ float gate_of(float x) {
-    const float e = __expf(-fabsf(x));
-    return __builtin_copysignf(e * __builtin_amdgcn_rcpf(1.0f + e), -x);
-}
-// a h, of such a c: h - s h, or s h.
-__device__ __forceinline__ float through(float c, float h) {
-    return fmaf(c, h, __builtin_signbit(c) ? h : 0.0f);
-}
-// a (1 - a)
-__device__ __forceinline__ float slope_of(float c) {
-    const float s = fabsf(c);
-    return fmaf(-s, s, s);
+// A gate a = sigmoid(x), rounded once from 1 - s where x > 0, and its slope a (1 - a) =
+// s (1 - s), with s = sigmoid(-|x|) to a few roundings of itself: 1 - a would have
+// none of a gate's digits that is nearly open.
+struct Gate {
+    float a, slope;
+};
+__device__ __forceinline__ Gate gate_of(float x) {
+    const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(x));
+    const float s = e * __builtin_amdgcn_rcpf(1.0f + e);
+    return Gate{x > 0.0f ? 1.0f - s : s, fmaf(-s, s, s)};
 }
 
 __device__ __forceinline__ int linrec_slot(const LinRecArgs& a, int seq) {

@@ -33,13 +33,28 @@ namespace {
 
 constexpr int NT = kLinRecThreads;
 constexpr float kCut = -1.0f;             // in place of a map's A, which is >= 0 or NaN
-constexpr int kWindow = 8;                // tiles looked at in a step
+constexpr int kWindow = kBehind / 4;      // tiles that a lane looks at
+constexpr unsigned long long kPatience = 500000000;          // 5 s at 100 MHz
 constexpr unsigned kUnset = 0xffffffffu;  // an A that was not published: a NaN that no map has
 
 template <class T, int V>
 struct Piece {
     T v[V];
 };
+
+// What the compiler has made of a piece's values ends here: it would otherwise keep
+// all of them as floats from one use to the next.
+template <class T, int V>
+__device__ __forceinline__ void opaque(Piece<T, V>& p) {
+    if constexpr (sizeof(p) % 4 == 0 && sizeof(T) == 2) {
+        unsigned x[sizeof(p) / 4];
+        __builtin_memcpy(x, &p, sizeof(p));
+        #pragma unroll
+        for (unsigned& w : x) asm("" : "+v"(w));
+        __builtin_memcpy(&p, x, sizeof(p));
+    }
+}
+__device__ __forceinline__ void opaque(int& x) { asm("" : "+v"(x)); }
 
 __device__ __forceinline__ unsigned long long word_of(float A, float L) {
     const unsigned x = __builtin_bit_cast(unsigned, A == A ? A : __builtin_nanf(""));
@@ -48,34 +63,14 @@ __device__ __forceinline__ unsigned long long word_of(float A, float L) {
 __device__ __forceinline__ float map_a(unsigned long long w) { return __builtin_bit_cast(float, (unsigned)w); }
 __device__ __forceinline__ float map_l(unsigned long long w) { return __builtin_bit_cast(float, (unsigned)(w >> 32)); }
 
-// State before place p of a chain (p > 0): word j of it lies at words + j * step.
-__device__ __forceinline__ float look_back(const unsigned long long* words, int p, long long step) {
-    const unsigned long long t0 = wall_clock64();
-    for (;;) {
-        unsigned long long w[kWindow];
-        #pragma unroll
-        for (int j = 0; j < kWindow; ++j)
-            w[j] = __hip_atomic_load(words + max(p - 1 - j, 0) * step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        float h = 0.0f;
-        bool known = false;
-        #pragma unroll
-        for (int j = kWindow - 1; j >= 0; --j) {             // the nearest published state goes last
-            const float A = map_a(w[j]), L = map_l(w[j]);
-            if ((unsigned)w[j] == kUnset) known = false;
-            else if (A < 0.0f) known = true, h = L;
-            else h = fmaf(A, h, L);
-        }
-        if (known) return h;
-        if (wall_clock64() - t0 > 500000000ull) return __builtin_nanf("");      // 5 s at 100 MHz
-        __builtin_amdgcn_s_sleep(1);
-    }
-}
+constexpr int kMaxTile = NT * 8;          // one thread along the channels, eight tokens each
 
-// What a workgroup knows of its tile's tokens.
+// What a workgroup knows of its tile's tokens: where sequences begin (the token behind
+// the tile too), and which.
 struct Shared {
     int ticket;
-    unsigned has[NT / 32];                // threads along the tokens in whose tokens a sequence begins
-    int last[NT];                         // the last of those sequences
+    unsigned mask[kMaxTile / 32 + 1];
+    __device__ __forceinline__ bool begins(int i) const { return mask[i >> 5] >> (i & 31) & 1; }
 };
 
 // Where a thread works.
@@ -84,21 +79,34 @@ struct Place {
     int x, y, cb, tile, place;            // thread's column and row; block of channels; place in the chain
     bool on;                              // has channels
     int c, over;                          // first channel; those of them that the piece before has too
-    long long t0, t;                      // first token of the tile, of the thread
+    int t0, t;                            // first token of the tile, of the thread
     int n;                                // tokens of the thread
-    int* first;                           // [tile + 1] sequence that begins at a token, or -1
+    int* first;                           // [tile + 1] sequence that begins at a token
     int in;                               // sequence that the token before the thread's belongs to
     unsigned starts, ends;                // of the thread's tokens: bit r where a sequence begins, ends
     bool begun;                           // the tile's first token belongs to a sequence that began before it
+    int at, next;                         // a boundary of the thread's, and the one behind it
+
+    __device__ __forceinline__ static int boundary(const LinRecArgs& a, long long i) {
+        return i <= a.n_seqs ? (int)min((long long)max(a.cu[i], 0), a.n_tokens) : 0x7fffffff;
+    }
 
     __device__ __forceinline__ void find(const LinRecArgs& a, Shared& sh, bool backward) {
-        const int tid = threadIdx.x;
+        const int tid = threadIdx.x, nt = blockDim.x;
         cb = blockIdx.x % a.blocks;
+        unsigned ticket = 0;
+        if (a.tiles > 1 && tid == 0)
+            ticket = __hip_atomic_fetch_add(a.tickets + cb * kTicketStep, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // meanwhile: one of nt boundaries spread over all
+        if (a.cu) {
+            const int step = a.n_seqs / nt + 1;
+            at = boundary(a, (long long)tid * step);
+            if (step == 1) next = boundary(a, tid + 1);
+        }
+        for (int i = tid; i <= a.tile / 32; i += nt) sh.mask[i] = 0;
         place = 0;
         if (a.tiles > 1) {
-            if (tid == 0)
-                sh.ticket = (int)__hip_atomic_fetch_add(a.tickets + cb * kTicketStep, 1u, __ATOMIC_RELAXED,
-                                                        __HIP_MEMORY_SCOPE_AGENT);
+            if (tid == 0) sh.ticket = (int)ticket;
             __syncthreads();
             place = __builtin_amdgcn_readfirstlane(sh.ticket);
         }
@@ -107,90 +115,88 @@ struct Place {
         x = tid - y * a.cols;
         const int p = cb * a.cols + x;
         on = y < a.lanes && p * V < a.channels;
+        y = on ? y : 0;
         c = on ? min(p * V, a.channels - V) : 0;
         over = on ? p * V - c : 0;
-        t0 = (long long)tile * a.tile;
+        t0 = tile * a.tile;
         t = t0 + y * R;
         n = on ? (int)min((long long)R, max(0ll, a.n_tokens - t)) : 0;
     }
 
-    // Marks the tokens at which sequences begin.
+    __device__ __forceinline__ void set(Shared& sh, int token, int seq) {
+        const int i = token - t0;
+        first[i] = seq;
+        atomicOr(sh.mask + (i >> 5), 1u << (i & 31));
+    }
+    // Marks the tokens at which sequences begin (where several do, all but the last are
+    // empty), and finds the thread's.
     __device__ __forceinline__ void mark(const LinRecArgs& a, Shared& sh) {
-        const int tid = threadIdx.x;
-        const long long t1 = min(t0 + a.tile, a.n_tokens);
+        const int tid = threadIdx.x, nt = blockDim.x;
+        const int t1 = (int)min((long long)t0 + a.tile, a.n_tokens);
         int before;                                           // sequence of the token before the tile
         if (a.cu) {
-            for (int i = tid; i <= a.tile; i += NT) first[i] = -1;
-            if (tid < NT / 32) sh.has[tid] = 0;
-            // the first boundary at t0 or behind it, from NT at a time (and at least one barrier)
-            int lo = 0, hi = a.n_seqs + 1;
-            while (hi - lo > 0) {
-                const int step = (hi - lo + NT - 1) / NT;
-                const long long i = lo + (long long)tid * step;
-                const int k = __syncthreads_count(i < hi && max(a.cu[i], 0) < t0);
-                if (step == 1) {
-                    lo += k;
-                    break;
+            // the first boundary at t0 or behind it is in [lo, hi]
+            int step = a.n_seqs / nt + 1, k = __syncthreads_count(at < t0), lo = k, hi = k;
+            if (step == 1) {
+                if (at >= t0 && at <= t1 && next != at) set(sh, at, tid);
+            } else {
+                lo = k ? (k - 1) * step + 1 : 0;
+                hi = k ? (int)min((long long)k * step, a.n_seqs + 1ll) : 0;
+                while (hi > lo) {
+                    step = (hi - lo + nt - 1) / nt;
+                    const long long i = lo + (long long)tid * step;
+                    k = __syncthreads_count(i < hi && boundary(a, i) < t0);
+                    const int from = lo;
+                    lo = step == 1 ? from + k : k ? from + (k - 1) * step + 1 : from;
+                    hi = step == 1 ? lo : k ? (int)min((long long)hi, from + (long long)k * step) : from;
                 }
-                hi = k == 0 ? lo : (int)min((long long)hi, lo + (long long)k * step);
-                lo = k == 0 ? lo : lo + (k - 1) * step + 1;
+                for (long long i = lo + tid; i <= a.n_seqs; i += nt) {
+                    const int here = boundary(a, i);
+                    if (here > t1) break;
+                    if (here >= t0 && boundary(a, i + 1) != here) set(sh, here, (int)i);
+                }
             }
             before = lo - 1;
-            for (long long i = lo + tid; i <= a.n_seqs; i += NT) {
-                const long long at = min((long long)max(a.cu[i], 0), a.n_tokens);
-                if (at > t1) break;
-                if (at >= t0) atomicMax(first + (at - t0), (int)i);
-            }
         } else {
-            const unsigned len = (unsigned)a.seq_len;
-            for (int i = tid; i <= a.tile; i += NT) {
-                const unsigned at = (unsigned)(t0 + i), s = at / len;
-                first[i] = at == s * len ? (int)s : -1;
-            }
-            if (tid < NT / 32) sh.has[tid] = 0;
-            before = t0 ? (int)((unsigned)(t0 - 1) / len) : -1;
+            const int len = a.seq_len, s = (t0 + len - 1) / len;
+            before = t0 ? (t0 - 1) / len : -1;
+            if (a.tiles <= 1) __syncthreads();                // the masks are clear
+            for (long long i = s + tid; i * len <= t1; i += nt) set(sh, (int)(i * len), (int)i);
         }
         __syncthreads();
-        starts = ends = 0;
-        int last = -1;
-        if (y < a.lanes) {
-            int next = first[y * R];
-            #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                if (next >= 0) starts |= 1u << r, last = next;
-                next = first[y * R + r + 1];
-                if (next >= 0 || t + r + 1 >= a.n_tokens) ends |= 1u << r;
-            }
-            if (x == 0 && last >= 0) {
-                sh.last[y] = last;
-                atomicOr(sh.has + (y >> 5), 1u << (y & 31));
-            }
-        }
-        begun = first[0] < 0 && before >= 0 && before < a.n_seqs;
-        __syncthreads();
-        in = before;
-        unsigned m = sh.has[y >> 5] & ((1u << (y & 31)) - 1);
-        for (int k = y >> 5;; m = sh.has[--k]) {
-            if (m) {
-                in = sh.last[32 * k + 31 - __builtin_clz(m)];
-                break;
-            }
-            if (k == 0) break;
-        }
+        const int i = y * R;
+        starts = sh.mask[i >> 5] >> (i & 31) & ((1u << n) - 1);
+        ends = n == 0 ? 0 : starts >> 1 | (n < R || sh.begins(i + R) || t + R >= a.n_tokens ? 1u << (n - 1) : 0);
+        begun = !(sh.mask[0] & 1) && before >= 0 && before < a.n_seqs;
+        unsigned m = sh.mask[i >> 5] & ((1u << (i & 31)) - 1);
+        int k = i >> 5;
+        while (!m && k > 0) m = sh.mask[--k];
+        in = m ? first[32 * k + 31 - __builtin_clz(m)] : before;
     }
 };
 
 template <class T, int V, int R>
-__device__ __forceinline__ void load(Piece<T, V> (&x)[R], const void* base, long long stride, const Place<V, R>& p) {
-    const T* from = (const T*)base + p.t * stride + p.c;
-    #pragma unroll
-    for (int r = 0; r < R; ++r)
-        if (r < p.n) __builtin_memcpy(&x[r], from + r * stride, sizeof(x[r]));
+__device__ __forceinline__ void load(Piece<T, V> (&x)[R], const void* base, long long stride, const Place<V, R>& p,
+                                     bool whole) {
+    const T* from = (const T*)base + (long long)p.t * stride + p.c;
+    if (whole) {
+        #pragma unroll
+        for (int r = 0; r < R; ++r) {
+            __builtin_memcpy(&x[r], from, sizeof(x[r]));
+            from += stride;
+        }
+    } else {
+        #pragma unroll
+        for (int r = 0; r < R; ++r) {
+            x[r] = Piece<T, V>{};
+            if (r < p.n) __builtin_memcpy(&x[r], from + r * stride, sizeof(x[r]));
+        }
+    }
 }
-// A piece without the channels that another thread has too.
-template <class T, int V>
+// A piece; with TAIL without the channels that another thread has too.
+template <bool TAIL, class T, int V>
 __device__ __forceinline__ void store(T* to, const Piece<T, V>& x, int over) {
-    if (over == 0) {
+    if (!TAIL || over == 0) {
         __builtin_memcpy(to, &x, sizeof(x));
     } else {
         #pragma unroll
@@ -199,19 +205,152 @@ __device__ __forceinline__ void store(T* to, const Piece<T, V>& x, int over) {
     }
 }
 template <int V>
-__device__ __forceinline__ void read_state(float (&h)[V], const float* pool, long long stride, int slot, int c) {
-    if (pool && slot >= 0) {
-        __builtin_memcpy(h, pool + slot * stride + c, sizeof(h));
-    } else {
-        #pragma unroll
-        for (int i = 0; i < V; ++i) h[i] = 0.0f;
-    }
+__device__ __forceinline__ Piece<float, V> state_of(const float* pool, long long stride, int slot, int c) {
+    Piece<float, V> h = {};
+    if (pool && slot >= 0) __builtin_memcpy(&h, pool + slot * stride + c, sizeof(h));
+    return h;
 }
+
+// The chain phase: a lane has a channel of the workgroup's and one of four parts of
+// its threads (of the window, while it looks back); waves have sixteen channels.
+struct Chain {
+    int ch, part, lane;
+    bool on;                              // is there such a channel
+    float A[4], L[4];                     // the parts' maps
+    float tA, tL;                         // the tile's
+
+    __device__ __forceinline__ static float from(float x, int lane, int part) { return __shfl(x, (lane & 15) + 16 * part); }
+
+    // Folds the maps in LDS, first to last or (BACK) last to first.
+    template <bool BACK>
+    __device__ __forceinline__ void fold(const LinRecArgs& a, const float* sA, const float* sL, int row, int piece0, int v) {
+        lane = threadIdx.x & 63;
+        ch = (threadIdx.x >> 6) * 16 + (lane & 15);
+        part = lane >> 4;
+        on = ch < a.cols * v && (piece0 + ch / v) * v < a.channels;
+        float mA = 1.0f, mL = 0.0f;
+        const int per = a.lanes / 4;
+        if (on)
+            for (int y0 = 0; y0 < per; y0 += 4) {
+                float x[4], l[4];
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = part * per + y0 + j, y = BACK ? a.lanes - 1 - i : i;
+                    x[j] = sA[y * row + ch], l[j] = sL[y * row + ch];
+                }
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) join(mA, mL, x[j], l[j]);
+            }
+        tA = 1.0f, tL = 0.0f;
+        #pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            A[g] = from(mA, lane, g), L[g] = from(mL, lane, g);
+            join(tA, tL, A[g], L[g]);
+        }
+    }
+    // (A, L), then (x, l)
+    __device__ __forceinline__ static void join(float& A, float& L, float x, float l) {
+        L = x < 0.0f ? l : fmaf(x, L, l);
+        A = x < 0.0f || A < 0.0f ? kCut : A * x;
+    }
+    // Puts the states before the threads, from that before the tile, into sL's place.
+    template <bool BACK>
+    __device__ __forceinline__ void spread(const LinRecArgs& a, const float* sA, float* sL, int row, float state) {
+        const int per = a.lanes / 4;
+        #pragma unroll
+        for (int g = 0; g < 3; ++g)
+            if (g < part) state = A[g] < 0.0f ? L[g] : fmaf(A[g], state, L[g]);
+        if (on)
+            for (int y0 = 0; y0 < per; y0 += 4) {
+                float x[4], l[4];
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = part * per + y0 + j, y = BACK ? a.lanes - 1 - i : i;
+                    x[j] = sA[y * row + ch], l[j] = sL[y * row + ch];
+                }
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = part * per + y0 + j, y = BACK ? a.lanes - 1 - i : i;
+                    sL[y * row + ch] = state;
+                    state = x[j] < 0.0f ? l[j] : fmaf(x[j], state, l[j]);
+                }
+            }
+    }
+    // The state before place p of the chain, after publishing the tile's map; `open`: a
+    // sequence goes on from the place before into this one.
+    __device__ __forceinline__ float before(const LinRecArgs& a, int block, int p, bool open) {
+        // word of this channel at place p
+        unsigned long long* word = a.words + ((long long)block * (a.tiles + kBehind) + kBehind + p) * kChannels + ch;
+        auto publish = [&](float x, float l) {
+            if (on && part == 0) __hip_atomic_store(word, word_of(x, l), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        };
+        publish(open ? tA : kCut, tL);
+        if (!open) return 0.0f;
+        const float state = look_back(word);
+        if (!(tA < 0.0f)) publish(kCut, fmaf(tA, state, tL));
+        return state;
+    }
+    // Looks at the nearest 4 N tiles, N a lane.  True: h is the state, from the nearest
+    // published one through the maps behind it, in their order.  False: there is none
+    // yet; `nearest` says whether the nearest tile has published anything.
+    template <int N>
+    __device__ __forceinline__ bool look(const unsigned long long* word, float& h, bool& nearest) {
+        enum { kThrough, kKnown, kBlocked };                 // what a part knows: its maps, a state, nothing
+        unsigned long long w[N];
+        #pragma unroll
+        for (int j = 0; j < N; ++j)
+            w[j] = __hip_atomic_load(word - (part * N + j + 1) * kChannels, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        float x = 0.0f;
+        int mode = kThrough;
+        #pragma unroll
+        for (int j = N - 1; j >= 0; --j) {                   // the nearest published state goes last
+            if ((unsigned)w[j] == kUnset) mode = kBlocked;
+            else if (map_a(w[j]) < 0.0f) mode = kKnown, x = map_l(w[j]);
+            else x = fmaf(map_a(w[j]), x, map_l(w[j]));
+        }
+        // states from the farther parts through the nearer ones' maps
+        #pragma unroll
+        for (int g = 2; g >= 0; --g) {
+            const float in = from(x, lane, g + 1);
+            const int known = __shfl(mode, (lane & 15) + 16 * (g + 1));
+            if (part == g && mode == kThrough) {
+                mode = known == kKnown ? kKnown : kThrough;
+                x = in;
+                #pragma unroll
+                for (int j = N - 1; j >= 0; --j) x = fmaf(map_a(w[j]), x, map_l(w[j]));
+            }
+        }
+        h = from(x, lane, 0);
+        mode = __shfl(mode, lane & 15);
+        nearest = __all(!on || part > 0 || (unsigned)w[0] != kUnset);
+        return __all(!on || mode == kKnown);
+    }
+    // A word a lane until the nearest tile has published something (a state, where a
+    // sequence begins in it), then eight.
+    __device__ __forceinline__ float look_back(const unsigned long long* word) {
+        const unsigned long long t0 = wall_clock64();
+        float h;
+        bool nearest;
+        while (!look<1>(word, h, nearest)) {
+            if (nearest) {
+                while (!look<kWindow>(word, h, nearest)) {
+                    if (wall_clock64() - t0 > kPatience) return __builtin_nanf("");
+                    __builtin_amdgcn_s_sleep(1);
+                }
+                break;
+            }
+            if (wall_clock64() - t0 > kPatience) return __builtin_nanf("");
+            __builtin_amdgcn_s_sleep(1);
+        }
+        return h;
+    }
+};
 
 // Copies the states of sequences without tokens: workgroup b of those behind the tiles.
 __device__ void empty_sequences(const LinRecArgs& a, int b, const float* from, long long fs, float* to, long long ts) {
     __shared__ int which[NT];
-    const long long seq = (long long)b * NT + threadIdx.x;
+    const int nt = blockDim.x;
+    const long long seq = (long long)b * nt + threadIdx.x;
     int slot = -1;
     if (seq < a.n_seqs) {
         bool none = a.n_tokens == 0;
@@ -223,385 +362,318 @@ __device__ void empty_sequences(const LinRecArgs& a, int b, const float* from, l
     }
     which[threadIdx.x] = slot;
     __syncthreads();
-    for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < nt; ++i)
         if (which[i] >= 0)
-            for (int c = threadIdx.x; c < a.channels; c += NT)
+            for (int c = threadIdx.x; c < a.channels; c += nt)
                 to[which[i] * ts + c] = from ? from[which[i] * fs + c] : 0.0f;
 }
 
-template <class T, int V, int R>
-__global__ __launch_bounds__(NT) void k_linrec(const LinRecArgs a) {
+template <class T, int V, int R, bool TAIL>
+__global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const LinRecArgs a) {
     extern __shared__ __align__(16) char smem[];
     __shared__ Shared sh;
     if (blockIdx.x >= (unsigned)(a.tiles * a.blocks)) {
         empty_sequences(a, blockIdx.x - a.tiles * a.blocks, a.s_in, a.si, a.s_out, a.so);
         return;
     }
-    const int cb = a.cols * V;                               // channels of a workgroup, and of a row of LDS
-    float* sA = (float*)smem;                                // [lanes][cb]
-    float* sL = sA + a.lanes * cb;
+    const int row = a.cols * V + 4;                          // a row of LDS: the workgroup's channels, and four
+    float* sA = (float*)smem;                                // [lanes][row]
+    float* sL = sA + a.lanes * row;
     Place<V, R> p;
-    p.first = (int*)(sL + a.lanes * cb);
+    p.first = (int*)(sL + a.lanes * row);
     p.find(a, sh, false);
-
-    Piece<T, V> g[R] = {}, v[R] = {}, q[R] = {};
-    load(g, a.g, a.gt, p);
-    load(v, a.v, a.vt, p);
-    if (a.q) load(q, a.q, a.qt, p);
+    const bool whole = p.t0 + a.tile <= a.n_tokens;
+    Piece<T, V> g[R], v[R], q[R];
+    load(g, a.g, a.gt, p, whole);
+    load(v, a.v, a.vt, p, whole);
+    if (a.q) load(q, a.q, a.qt, p, whole);
     p.mark(a, sh);
 
-    // Token r with state h behind it.
-    auto finish = [&](int r, const float (&h)[V], int slot) {
-        if (slot < 0 && !a.carries) return;                  // of no sequence: stays, zero with carries
-        Piece<T, V> y;
-        #pragma unroll
-        for (int i = 0; i < V; ++i) y.v[i] = (T)(slot < 0 ? 0.0f : a.q ? (float)q[r].v[i] * h[i] : h[i]);
-        store((T*)a.out + (p.t + r) * a.ot + p.c, y, p.over);
-        if (a.s_out && slot >= 0 && (p.ends >> r & 1)) {
-            Piece<float, V> s;
-            #pragma unroll
-            for (int i = 0; i < V; ++i) s.v[i] = h[i];
-            store(a.s_out + slot * a.so + p.c, s, p.over);
-        }
-    };
-
-    // the thread's map; tokens from its first beginning of a sequence on are done here
-    float c[R][V], A[V], h[V];
+    // The thread's map.  The last state that comes in is kept: its sequence may end
+    // in another thread, which may write to its slot before this one is here again.
+    float f[R][V], A[V];
+    Piece<float, V> h = {}, last = {};
     #pragma unroll
-    for (int i = 0; i < V; ++i) A[i] = 1.0f, h[i] = 0.0f;
-    bool cut = false;
-    int slot = -1;
+    for (int i = 0; i < V; ++i) A[i] = 1.0f;
     #pragma unroll
     for (int r = 0; r < R; ++r) {
-        if (r < p.n && (p.starts >> r & 1)) {
-            cut = true;
-            slot = linrec_slot(a, p.first[p.y * R + r]);
-            read_state(h, a.s_in, a.si, slot, p.c);
-        }
+        if (p.starts >> r & 1) last = h = state_of<V>(a.s_in, a.si, linrec_slot(a, p.first[p.y * R + r]), p.c);
         #pragma unroll
         for (int i = 0; i < V; ++i) {
-            c[r][i] = gate_of((float)g[r].v[i]);
-            h[i] = through(c[r][i], h[i]) + (float)v[r].v[i];
-            A[i] = through(c[r][i], A[i]);
+            f[r][i] = gate_of((float)g[r].v[i]).a;
+            h.v[i] = fmaf(f[r][i], h.v[i], (float)v[r].v[i]);
+            A[i] *= f[r][i];
         }
-        if (cut && r < p.n) finish(r, h, slot);
     }
     if (p.on) {
         #pragma unroll
         for (int i = 0; i < V; ++i) {
-            sA[p.y * cb + p.x * V + i] = cut ? kCut : A[i];
-            sL[p.y * cb + p.x * V + i] = h[i];
+            sA[p.y * row + p.x * V + i] = p.starts ? kCut : A[i];
+            sL[p.y * row + p.x * V + i] = h.v[i];
         }
     }
+    #pragma unroll
+    for (int r = 0; r < R; ++r) opaque(v[r]);
+    opaque(p.t), opaque(p.c);
     __syncthreads();
 
-    // a thread a channel: the tile's map, the state before it, and those before its threads
-    const int k = threadIdx.x;
-    if (k < cb && (p.cb * a.cols + k / V) * V < a.channels) {
-        float state = 0.0f;
-        if (a.tiles > 1) {
-            float tA = 1.0f, tL = 0.0f;
-            for (int y = 0; y < a.lanes; ++y) {
-                const float yA = sA[y * cb + k], yL = sL[y * cb + k];
-                tL = yA < 0.0f ? yL : fmaf(yA, tL, yL);
-                tA = yA < 0.0f || tA < 0.0f ? kCut : tA * yA;
-            }
-            const long long step = (long long)a.blocks * cb;
-            unsigned long long* words = a.words + p.cb * cb + k;
-            auto publish = [&](float A, float L) {
-                __hip_atomic_store(words + p.place * step, word_of(A, L), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            };
-            publish(p.begun ? tA : kCut, tL);
-            if (p.begun) {
-                state = look_back(words, p.place, step);
-                if (!(tA < 0.0f)) publish(kCut, fmaf(tA, state, tL));
-                if (a.carries) {
-                    const int col = (p.cb * a.cols + k / V) * V, at = min(col, a.channels - V) + k % V;
-                    if (at >= col) a.carries[(long long)p.tile * a.channels + at] = state;
-                }
-            }
-        }
-        for (int y = 0; y < a.lanes; ++y) {
-            const float yA = sA[y * cb + k], yL = sL[y * cb + k];
-            sL[y * cb + k] = state;
-            state = yA < 0.0f ? yL : fmaf(yA, state, yL);
-        }
-    }
+    // the tile's map, the state before it, and those before its threads
+    Chain chain;
+    chain.fold<false>(a, sA, sL, row, p.cb * a.cols, V);
+    const float state = a.tiles > 1 ? chain.before(a, p.cb, p.place, p.begun) : 0.0f;
+    chain.spread<false>(a, sA, sL, row, state);
     __syncthreads();
-    if (p.n == 0 || (p.starts & 1)) return;
+    if (p.n == 0) return;
     #pragma unroll
-    for (int i = 0; i < V; ++i) h[i] = sL[p.y * cb + p.x * V + i];
-    slot = linrec_slot(a, p.in);
+    for (int i = 0; i < V; ++i) h.v[i] = sL[p.y * row + p.x * V + i];
+    if (a.carries && p.t % a.carry == 0)
+        store<TAIL>(a.carries + (long long)(p.t / a.carry) * a.channels + p.c, h, p.over);
+    int slot = linrec_slot(a, p.in);
+    T* out = (T*)a.out + (long long)p.t * a.ot + p.c;
     #pragma unroll
     for (int r = 0; r < R; ++r) {
-        if (r >= p.n || (p.starts >> r & 1)) break;
+        if (p.starts >> r & 1) {
+            slot = linrec_slot(a, p.first[p.y * R + r]);
+            h = p.starts >> r == 1 ? last : state_of<V>(a.s_in, a.si, slot, p.c);
+        }
+        Piece<T, V> y;
         #pragma unroll
-        for (int i = 0; i < V; ++i) h[i] = through(c[r][i], h[i]) + (float)v[r].v[i];
-        finish(r, h, slot);
+        for (int i = 0; i < V; ++i) {
+            h.v[i] = fmaf(f[r][i], h.v[i], (float)v[r].v[i]);
+            y.v[i] = (T)(a.q ? (float)q[r].v[i] * h.v[i] : h.v[i]);
+        }
+        if (slot >= 0 && r < p.n) {
+            store<TAIL>(out, y, p.over);
+            if (a.s_out && (p.ends >> r & 1)) store<TAIL>(a.s_out + slot * a.so + p.c, h, p.over);
+        } else if (a.carries && r < p.n) {                   // of no sequence: zeros
+            store<TAIL>(out, Piece<T, V>{}, p.over);
+        }
+        out += a.ot;
     }
 }
 
-template <class T, int V, int R>
-__global__ __launch_bounds__(NT) void k_linrec_backward(const LinRecArgs a) {
+template <class T, int V, int R, bool TAIL>
+__global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(const LinRecArgs a) {
     extern __shared__ __align__(16) char smem[];
     __shared__ Shared sh;
     if (blockIdx.x >= (unsigned)(a.tiles * a.blocks)) {
         empty_sequences(a, blockIdx.x - a.tiles * a.blocks, a.ds_out, a.dso, a.ds_in, a.dsi);
         return;
     }
-    const int cb = a.cols * V;
+    const int row = a.cols * V + 4;
     float* sA = (float*)smem;
-    float* sL = sA + a.lanes * cb;
+    float* sL = sA + a.lanes * row;
     Place<V, R> p;
-    p.first = (int*)(sL + a.lanes * cb);
+    p.first = (int*)(sL + a.lanes * row);
     p.find(a, sh, true);
-
-    Piece<T, V> g[R] = {}, v[R] = {}, q[R] = {}, d[R] = {};
-    load(g, a.g, a.gt, p);
-    load(v, a.v, a.vt, p);
-    if (a.q) load(q, a.q, a.qt, p);
-    if (a.dout) load(d, a.dout, a.dot, p);
+    const bool whole = p.t0 + a.tile <= a.n_tokens;
+    Piece<T, V> g[R], v[R], q[R], d[R];
+    load(g, a.g, a.gt, p, whole);
+    load(v, a.v, a.vt, p, whole);
+    if (a.q) load(q, a.q, a.qt, p, whole);
+    if (a.dout) load(d, a.dout, a.dot, p, whole);
     p.mark(a, sh);
 
-    // states, as the forward pass had them: hs[r] before token r, hs[R] behind the last
-    float c[R][V], A[V], h[V], hs[R + 1][V];
+    // states, as the forward pass had them: hs[r] behind token r, h0 before the first;
+    // w: the gates' slopes
+    float f[R][V], w[R][V], A[V], hs[R][V];
+    Piece<float, V> h = {}, h0;
     #pragma unroll
-    for (int i = 0; i < V; ++i) A[i] = 1.0f, h[i] = 0.0f;
-    bool cut = false;
+    for (int i = 0; i < V; ++i) A[i] = 1.0f;
     #pragma unroll
     for (int r = 0; r < R; ++r) {
-        if (r < p.n && (p.starts >> r & 1)) {
-            cut = true;
-            read_state(h, a.s_in, a.si, linrec_slot(a, p.first[p.y * R + r]), p.c);
-        }
+        if (p.starts >> r & 1) h = state_of<V>(a.s_in, a.si, linrec_slot(a, p.first[p.y * R + r]), p.c);
         #pragma unroll
         for (int i = 0; i < V; ++i) {
-            c[r][i] = gate_of((float)g[r].v[i]);
-            hs[r][i] = h[i];
-            h[i] = through(c[r][i], h[i]) + (float)v[r].v[i];
-            A[i] = through(c[r][i], A[i]);
+            const Gate gate = gate_of((float)g[r].v[i]);
+            f[r][i] = gate.a, w[r][i] = gate.slope;
+            h.v[i] = fmaf(f[r][i], h.v[i], (float)v[r].v[i]);
+            A[i] *= f[r][i];
         }
     }
     if (p.on) {
         #pragma unroll
         for (int i = 0; i < V; ++i) {
-            sA[p.y * cb + p.x * V + i] = cut ? kCut : A[i];
-            sL[p.y * cb + p.x * V + i] = h[i];
+            sA[p.y * row + p.x * V + i] = p.starts ? kCut : A[i];
+            sL[p.y * row + p.x * V + i] = h.v[i];
         }
     }
+    #pragma unroll
+    for (int r = 0; r < R; ++r) opaque(v[r]);
     __syncthreads();
-    const int k = threadIdx.x;
-    const int col = (p.cb * a.cols + k / V) * V, at = min(col, a.channels - V) + k % V;
-    const bool chain = k < cb && col < a.channels;
-    if (chain) {
-        float state = p.begun && a.tiles > 1 ? a.carries[(long long)p.tile * a.channels + at] : 0.0f;
-        for (int y = 0; y < a.lanes; ++y) {
-            const float yA = sA[y * cb + k], yL = sL[y * cb + k];
-            sL[y * cb + k] = state;
-            state = yA < 0.0f ? yL : fmaf(yA, state, yL);
-        }
-    }
+    Chain chain;
+    chain.fold<false>(a, sA, sL, row, p.cb * a.cols, V);
+    const int col = (p.cb * a.cols + chain.ch / V) * V, at = min(col, a.channels - V) + chain.ch % V;
+    chain.spread<false>(a, sA, sL, row,
+                        p.begun && a.tiles > 1 && chain.on ? a.carries[(long long)p.tile * a.channels + at] : 0.0f);
     __syncthreads();
     #pragma unroll
-    for (int i = 0; i < V; ++i) hs[R][i] = h[i];
-    if (p.on) {
+    for (int i = 0; i < V; ++i) h0.v[i] = h.v[i] = p.on ? sL[p.y * row + p.x * V + i] : 0.0f;
+    #pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (p.starts >> r & 1) h = state_of<V>(a.s_in, a.si, linrec_slot(a, p.first[p.y * R + r]), p.c);
         #pragma unroll
-        for (int i = 0; i < V; ++i) h[i] = sL[p.y * cb + p.x * V + i];
-        bool before = true;                                  // of the thread's first beginning
-        #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if (p.starts >> r & 1) before = false;
-            #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (before) {
-                    hs[r][i] = h[i];
-                    h[i] = through(c[r][i], h[i]) + (float)v[r].v[i];
-                }
-        }
-        #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (before) hs[R][i] = h[i];
+        for (int i = 0; i < V; ++i) hs[r][i] = h.v[i] = fmaf(f[r][i], h.v[i], (float)v[r].v[i]);
     }
     __syncthreads();
 
-    // Token r with the gradient of its state.
-    auto finish = [&](int r, const float (&dh)[V], int slot) {
-        Piece<T, V> y;
-        const long long t = p.t + r;
-        if (a.dv) {
-            #pragma unroll
-            for (int i = 0; i < V; ++i) y.v[i] = (T)(slot < 0 ? 0.0f : dh[i]);
-            store((T*)a.dv + t * a.dvt + p.c, y, p.over);
-        }
-        if (a.dg) {
-            #pragma unroll
-            for (int i = 0; i < V; ++i) y.v[i] = (T)(slot < 0 ? 0.0f : dh[i] * hs[r][i] * slope_of(c[r][i]));
-            store((T*)a.dg + t * a.dgt + p.c, y, p.over);
-        }
-        if (a.dq) {
-            #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float behind = through(c[r][i], hs[r][i]) + (float)v[r].v[i];
-                y.v[i] = (T)(slot < 0 ? 0.0f : (float)d[r].v[i] * behind);
-            }
-            store((T*)a.dq + t * a.dqt + p.c, y, p.over);
-        }
-        if (a.ds_in && slot >= 0 && (p.starts >> r & 1)) {
-            Piece<float, V> s;
-            #pragma unroll
-            for (int i = 0; i < V; ++i) s.v[i] = through(c[r][i], dh[i]);
-            store(a.ds_in + slot * a.dsi + p.c, s, p.over);
-        }
-    };
     // sequence of token r
-    auto seq_of = [&](int r) {
+    auto slot_at = [&](int r) {
         const unsigned m = p.starts & ((2u << r) - 1);
         return linrec_slot(a, m ? p.first[p.y * R + 31 - __builtin_clz(m)] : p.in);
     };
-
-    // the map of messages; tokens up to the last end of a sequence are done here
-    float m[V];
-    #pragma unroll
-    for (int i = 0; i < V; ++i) A[i] = 1.0f, m[i] = 0.0f;
-    cut = false;
+    // what token r adds to its state's gradient
+    auto read_out = [&](int r, int i) {
+        const float y = a.dout ? (float)d[r].v[i] : 0.0f;
+        return a.q ? (float)q[r].v[i] * y : y;
+    };
+    // the map of messages
+    Piece<float, V> m = {};
     #pragma unroll
     for (int r = R - 1; r >= 0; --r) {
-        if (r < p.n && (p.ends >> r & 1)) {
-            cut = true;
-            read_state(m, a.ds_out, a.dso, seq_of(r), p.c);
-        }
-        float dh[V];
-        #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float e = a.q ? (float)q[r].v[i] * (float)d[r].v[i] : (float)d[r].v[i];
-            dh[i] = e + m[i];
-        }
-        if (cut && r < p.n) finish(r, dh, seq_of(r));
-        #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            m[i] = r < p.n ? through(c[r][i], dh[i]) : 0.0f;
-            A[i] = r < p.n ? through(c[r][i], A[i]) : A[i];
+        if (p.ends >> r & 1) m = state_of<V>(a.ds_out, a.dso, slot_at(r), p.c);
+        if (r < p.n) {
+            #pragma unroll
+            for (int i = 0; i < V; ++i) m.v[i] = f[r][i] * (read_out(r, i) + m.v[i]);
         }
     }
     if (p.on) {
         #pragma unroll
         for (int i = 0; i < V; ++i) {
-            sA[p.y * cb + p.x * V + i] = cut ? kCut : A[i];
-            sL[p.y * cb + p.x * V + i] = m[i];
+            sA[p.y * row + p.x * V + i] = p.ends ? kCut : A[i];
+            sL[p.y * row + p.x * V + i] = m.v[i];
         }
     }
-    __syncthreads();
-    if (chain) {
-        float state = 0.0f;
-        if (a.tiles > 1) {
-            float tA = 1.0f, tL = 0.0f;
-            for (int y = a.lanes - 1; y >= 0; --y) {
-                const float yA = sA[y * cb + k], yL = sL[y * cb + k];
-                tL = yA < 0.0f ? yL : fmaf(yA, tL, yL);
-                tA = yA < 0.0f || tA < 0.0f ? kCut : tA * yA;
-            }
-            // a sequence that goes on behind the tile
-            const bool open = p.place > 0 && p.first[a.tile] < 0;
-            const long long step = (long long)a.blocks * cb;
-            unsigned long long* words = a.words + p.cb * cb + k;
-            auto publish = [&](float A, float L) {
-                __hip_atomic_store(words + p.place * step, word_of(A, L), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            };
-            publish(open ? tA : kCut, tL);
-            if (open) {
-                state = look_back(words, p.place, step);
-                if (!(tA < 0.0f)) publish(kCut, fmaf(tA, state, tL));
-            }
-        }
-        for (int y = a.lanes - 1; y >= 0; --y) {
-            const float yA = sA[y * cb + k], yL = sL[y * cb + k];
-            sL[y * cb + k] = state;
-            state = yA < 0.0f ? yL : fmaf(yA, state, yL);
-        }
-    }
-    __syncthreads();
-    if (p.n == 0 || (p.ends >> (p.n - 1) & 1)) return;
     #pragma unroll
-    for (int i = 0; i < V; ++i) m[i] = sL[p.y * cb + p.x * V + i];
-    const int slot = seq_of(R - 1);
-    bool behind = true;                                      // behind the last end
+    for (int r = 0; r < R; ++r) opaque(d[r]), opaque(q[r]);
+    opaque(p.t), opaque(p.c);
+    __syncthreads();
+    chain.fold<true>(a, sA, sL, row, p.cb * a.cols, V);
+    // a sequence that goes on behind the tile
+    const bool open = p.place > 0 && !sh.begins(a.tile);
+    const float state = a.tiles > 1 ? chain.before(a, p.cb, p.place, open) : 0.0f;
+    chain.spread<true>(a, sA, sL, row, state);
+    __syncthreads();
+    if (p.n == 0) return;
+    #pragma unroll
+    for (int i = 0; i < V; ++i) m.v[i] = sL[p.y * row + p.x * V + i];
+    int slot = slot_at(R - 1);
+    T* dg = (T*)a.dg + (long long)(p.t + R - 1) * a.dgt + p.c;
+    T* dv = (T*)a.dv + (long long)(p.t + R - 1) * a.dvt + p.c;
+    T* dq = (T*)a.dq + (long long)(p.t + R - 1) * a.dqt + p.c;
     #pragma unroll
     for (int r = R - 1; r >= 0; --r) {
-        if (p.ends >> r & 1) behind = false;
-        if (!behind || r >= p.n) continue;
-        float dh[V];
-        #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float e = a.q ? (float)q[r].v[i] * (float)d[r].v[i] : (float)d[r].v[i];
-            dh[i] = e + m[i];
-            m[i] = through(c[r][i], dh[i]);
+        if (p.ends >> r & 1) {
+            slot = slot_at(r);
+            m = state_of<V>(a.ds_out, a.dso, slot, p.c);
         }
-        finish(r, dh, slot);
+        if (r < p.n) {
+            const bool begins = p.starts >> r & 1, none = slot < 0;      // of no sequence: zeros
+            Piece<T, V> yv, yg, yq;
+            Piece<float, V> was;                             // state before the token
+            #pragma unroll
+            for (int i = 0; i < V; ++i) was.v[i] = r ? hs[r ? r - 1 : 0][i] : h0.v[i];
+            if (begins) was = state_of<V>(a.s_in, a.si, slot, p.c);
+            #pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float dh = read_out(r, i) + m.v[i];
+                yv.v[i] = (T)dh;
+                yg.v[i] = (T)(dh * was.v[i] * w[r][i]);
+                yq.v[i] = (T)(a.dout ? (float)d[r].v[i] * hs[r][i] : 0.0f);
+                m.v[i] = f[r][i] * dh;
+            }
+            if (none) yv = yg = yq = Piece<T, V>{};
+            if (a.dg) store<TAIL>(dg, yg, p.over);
+            if (a.dv) store<TAIL>(dv, yv, p.over);
+            if (a.dq) store<TAIL>(dq, yq, p.over);
+            if (a.ds_in && begins && !none) store<TAIL>(a.ds_in + slot * a.dsi + p.c, m, p.over);
+        }
+        dg -= a.dgt, dv -= a.dvt, dq -= a.dqt;
     }
 }
 
 // Empties the chain: no word is published, no ticket taken.
-__global__ __launch_bounds__(NT) void k_linrec_clear(unsigned long long* words, long long n, unsigned* tickets, int nt) {
-    const long long i = (long long)blockIdx.x * NT + threadIdx.x;
-    if (i < n) words[i] = ~0ull;
-    if (i < nt) tickets[i] = 0;
+__global__ __launch_bounds__(NT) void k_linrec_clear(ulonglong2* words, long long n, unsigned* tickets, int nt) {
+    const long long id = (long long)blockIdx.x * NT + threadIdx.x;
+    for (long long i = id; i < n; i += (long long)gridDim.x * NT) words[i] = ulonglong2{~0ull, ~0ull};
+    for (long long i = id; i < nt; i += (long long)gridDim.x * NT) tickets[i] = 0;
 }
 
 size_t lds_bytes(const LinRecArgs& a) {
-    return (size_t)a.lanes * a.cols * a.vec * 8 + ((size_t)a.tile + 1) * 4;
+    return (size_t)a.lanes * (a.cols * a.vec + 4) * 8 + ((size_t)a.tile + 1) * 4;
 }
 
-template <int V> constexpr int kTokens = V == 8 ? 4 : 8;     // of a thread
+// Channels of a thread: 16 bytes; its tokens.
+template <class T> constexpr int kVec = 16 / sizeof(T);
+#ifndef FR
+#define FR 8
+#define BR 4
+#define FR2 4
+#define BR2 2
+#endif
+constexpr int tokens_of(bool wide, bool backward) { return wide ? backward ? BR : FR : backward ? BR2 : FR2; }
 
-template <class T>
-hipError_t launch(const LinRecArgs& a, bool backward, hipStream_t st) {
-    constexpr int V = 16 / sizeof(T);
+template <class T, bool BACKWARD, int V, bool TAIL>
+const void* kernel() {
+    constexpr int R = tokens_of(sizeof(T) == 4, BACKWARD);
+    if constexpr (BACKWARD) return (const void*)k_linrec_backward<T, V, R, TAIL>;
+    else return (const void*)k_linrec<T, V, R, TAIL>;
+}
+
+template <class T, bool BACKWARD>
+hipError_t launch(const LinRecArgs& a, hipStream_t st) {
     LinRecArgs args = a;
+    const int nt = (a.cols * a.lanes + 63) / 64 * 64;
     if (a.tiles > 1) {
-        long long n = (long long)linrec_words(a);
-        int nt = a.blocks * kTicketStep;
-        void* pc[] = {&args.words, &n, &args.tickets, &nt};
-        const long long most = n > nt ? n : nt;
-        const hipError_t e = hipLaunchKernel((const void*)k_linrec_clear, dim3((unsigned)((most + NT - 1) / NT)), dim3(NT),
-                                             pc, 0, st);
+        long long n = (long long)linrec_words(a) / 2;
+        int tickets = a.blocks * kTicketStep;
+        void* pc[] = {&args.words, &n, &args.tickets, &tickets};
+        const long long wgs = (n + 4 * NT - 1) / (4 * NT);   // four stores a thread
+        const hipError_t e = hipLaunchKernel((const void*)k_linrec_clear, dim3((unsigned)(wgs < 1024 ? wgs : 1024)),
+                                             dim3(NT), pc, 0, st);
         if (e != hipSuccess) return e;
     }
-    const bool states = backward ? a.ds_in != nullptr : a.s_out && a.s_out != a.s_in;
-    const long long empties = states && (a.cu || !a.n_tokens) ? ((long long)a.n_seqs + NT - 1) / NT : 0;
+    const bool states = BACKWARD ? a.ds_in != nullptr : a.s_out && a.s_out != a.s_in;
+    const long long empties = states && (a.cu || !a.n_tokens) ? ((long long)a.n_seqs + nt - 1) / nt : 0;
     const long long wgs = (long long)a.tiles * a.blocks + empties;
     if (!wgs) return hipSuccess;
     void* pa[] = {&args};
-    const void* f = backward ? a.vec > 1 ? (const void*)k_linrec_backward<T, V, kTokens<V>>
-                                         : (const void*)k_linrec_backward<T, 1, kTokens<1>>
-                    : a.vec > 1 ? (const void*)k_linrec<T, V, kTokens<V>>
-                                : (const void*)k_linrec<T, 1, kTokens<1>>;
-    return hipLaunchKernel(f, dim3((unsigned)wgs), dim3(NT), pa, lds_bytes(a), st);
+    const void* f = a.vec == 1                ? kernel<T, BACKWARD, 1, false>()
+                    : a.channels % a.vec == 0 ? kernel<T, BACKWARD, kVec<T>, false>()
+                                              : kernel<T, BACKWARD, kVec<T>, true>();
+    return hipLaunchKernel(f, dim3((unsigned)wgs), dim3(nt), pa, lds_bytes(a), st);
+}
+
+// Threads along the channels, and along the tokens.
+void cut(LinRecArgs& a, int vec, int tokens) {
+    a.vec = a.channels < vec ? 1 : vec;
+    const int pieces = (a.channels - 1) / a.vec + 1, most = kChannels / vec;
+    a.blocks = (pieces + most - 1) / most;
+    a.cols = (pieces - 1) / a.blocks + 1;
+    a.lanes = 16;
+    while (2 * a.lanes * a.cols <= kLinRecThreads) a.lanes *= 2;
+    a.tile = a.lanes * tokens;
+    a.tiles = (int)((a.n_tokens + a.tile - 1) / a.tile);
 }
 
 }  // namespace
 
-void linrec_plan(LinRecArgs& a, int dtype) {
-    a.vec = dtype == SSLA_F32 ? 4 : 8;
-    const int tokens = a.vec == 8 ? kTokens<8> : kTokens<4>;
-    static_assert(kTokens<4> == kTokens<1>);
-    if (a.channels < a.vec) a.vec = 1;
-    const int pieces = (a.channels - 1) / a.vec + 1;
-    a.blocks = (pieces + 15) / 16;
-    a.cols = (pieces - 1) / a.blocks + 1;
-    a.lanes = kLinRecThreads / a.cols;
-    a.tile = a.lanes * (a.vec == 1 ? kTokens<1> : tokens);
-    a.tiles = (int)((a.n_tokens + a.tile - 1) / a.tile);
+void linrec_plan(LinRecArgs& a, int dtype, bool backward) {
+    const bool wide = dtype == SSLA_F32;
+    cut(a, wide ? 4 : 8, tokens_of(wide, true));
+    a.carry = a.tile;
+    if (!backward) cut(a, wide ? 4 : 8, tokens_of(wide, false));
 }
 
 hipError_t linrec_launch(const LinRecArgs& a, int dtype, hipStream_t st) {
-    return dtype == SSLA_F32    ? launch<float>(a, false, st)
-           : dtype == SSLA_BF16 ? launch<__bf16>(a, false, st)
-                                : launch<_Float16>(a, false, st);
+    return dtype == SSLA_F32    ? launch<float, false>(a, st)
+           : dtype == SSLA_BF16 ? launch<__bf16, false>(a, st)
+                                : launch<_Float16, false>(a, st);
 }
 hipError_t linrec_launch_backward(const LinRecArgs& a, int dtype, hipStream_t st) {
-    return dtype == SSLA_F32    ? launch<float>(a, true, st)
-           : dtype == SSLA_BF16 ? launch<__bf16>(a, true, st)
-                                : launch<_Float16>(a, true, st);
+    return dtype == SSLA_F32    ? launch<float, true>(a, st)
+           : dtype == SSLA_BF16 ? launch<__bf16, true>(a, st)
+                                : launch<_Float16, true>(a, st);
 }
 
 }  // namespace ssla

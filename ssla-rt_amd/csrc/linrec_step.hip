@@ -32,14 +32,14 @@ __global__ __launch_bounds__(NT) void k_linrec_step(const LinRecArgs a) {
         if (q) __builtin_memcpy(pq, q, sizeof(pq));
         #pragma unroll
         for (int i = 0; i < V; ++i) {
-            h[i] = through(gate_of((float)pg[i]), h[i]) + (float)pv[i];
+            h[i] = fmaf(gate_of((float)pg[i]).a, h[i], (float)pv[i]);
             pv[i] = (T)(q ? (float)pq[i] * h[i] : h[i]);
         }
         __builtin_memcpy(to, h, sizeof(h));
         __builtin_memcpy(out, pv, sizeof(pv));
     } else {
         for (int i = 0; i < a.channels - c; ++i) {
-            const float h = through(gate_of((float)g[i]), from[i]) + (float)v[i];
+            const float h = fmaf(gate_of((float)g[i]).a, from[i], (float)v[i]);
             to[i] = h;
             out[i] = (T)(q ? (float)q[i] * h : h);
         }

@@ -120,15 +120,14 @@ LinRecArgs linrec_args(const SslaHipLinRec* d, const SslaHipLinRecGrad* g) {
         a.dot = g->dout_stride, a.dgt = g->dgate_stride, a.dvt = g->dv_stride, a.dqt = g->dq_stride;
         a.dso = g->dstate_out_stride, a.dsi = g->dstate_in_stride;
     }
-    linrec_plan(a, d->dtype);
+    linrec_plan(a, d->dtype, g != nullptr);
     return a;
 }
 
 // The grid's limit, and the workspace.
 int linrec_bind(LinRecArgs& a, void* workspace, size_t bytes, const char* fn) {
     if (!launchable(a.tiles, a.blocks, 1, kLinRecThreads) ||
-        !launchable((long long)a.tiles * a.blocks + a.n_seqs / kLinRecThreads + 1, 1, 1, kLinRecThreads) ||
-        !launchable((long long)linrec_words(a) + kLinRecThreads, 1, 1, 1))
+        !launchable((long long)a.tiles * a.blocks + a.n_seqs / kLinRecThreads + 1, 1, 1, kLinRecThreads))
         return refuse(std::string(fn) + ": too many tokens and channels");
     const size_t need = linrec_bytes(a);
     if (!need) return SSLA_OK;
@@ -222,8 +221,7 @@ int ssla_hip_linrec_carries(const SslaHipLinRec* d, size_t* nbytes) try {
     if (!nbytes) return refuse("ssla_hip_linrec_carries: null argument");
     *nbytes = 0;
     if (const int rc = check_linrec(d, kSizes, "ssla_hip_linrec_carries")) return rc;
-    const LinRecArgs a = linrec_args(d, nullptr);
-    *nbytes = (size_t)a.tiles * a.channels * 4;
+    *nbytes = linrec_carries(linrec_args(d, nullptr));
     return SSLA_OK;
 } catch (const std::exception&) {
     return SSLA_ERR_ARG;
@@ -233,7 +231,9 @@ int ssla_hip_linrec_workspace(const SslaHipLinRec* d, size_t* nbytes) try {
     if (!nbytes) return refuse("ssla_hip_linrec_workspace: null argument");
     *nbytes = 0;
     if (const int rc = check_linrec(d, kSizes, "ssla_hip_linrec_workspace")) return rc;
-    *nbytes = linrec_bytes(linrec_args(d, nullptr));
+    const SslaHipLinRecGrad none{};
+    const size_t one = linrec_bytes(linrec_args(d, nullptr)), other = linrec_bytes(linrec_args(d, &none));
+    *nbytes = one > other ? one : other;
     return SSLA_OK;
 } catch (const std::exception&) {
     return SSLA_ERR_ARG;

@@ -13,7 +13,7 @@ namespace ssla {
 struct LayerNormArgs {
     const void *x, *res, *weight, *bias;
     void* out;
-    float* stats;                         // [row] of a Norm
+    float* stats;                         // [row] mean (two floats) and scale
     long long xr, rr, orow;               // strides between rows, elements
     // backward
     const void* dout;
@@ -23,11 +23,15 @@ struct LayerNormArgs {
     int rows, channels;
     int wide;                             // weight, bias and their gradients are fp32
     float eps;
+    double inv_channels;
+    // how the call is cut (layer_norm_plan)
+    int vec, reps;                        // channels of a piece; pieces a thread keeps (0: rows in strides)
+    int lanes;                            // threads of a row (over 64: a workgroup)
+    int threads, wgs;
     int parts;                            // of the rows, for the sums over them
 };
 
-// How the backward pass is cut; a.parts 0 where no sums over rows are wanted.
-void layer_norm_plan(LayerNormArgs& a, int dtype, bool sums);
+void layer_norm_plan(LayerNormArgs& a, int dtype, bool backward);
 hipError_t layer_norm_launch(const LayerNormArgs& a, int dtype, hipStream_t st);
 hipError_t layer_norm_launch_backward(const LayerNormArgs& a, int dtype, hipStream_t st);
 

@@ -192,7 +192,7 @@ LayerNormArgs layer_norm_args(const SslaHipLayerNorm* d, const SslaHipLayerNormG
         a.dout = g->dout, a.dx = g->dx, a.dw = g->dweight, a.db = g->dbias;
         a.dor = g->dout_stride, a.dxr = g->dx_stride;
     }
-    layer_norm_plan(a, d->dtype, g && (g->dweight || g->dbias));
+    layer_norm_plan(a, d->dtype, g != nullptr);
     return a;
 }
 

@@ -17,6 +17,7 @@
 #include "layernorm.h"
 
 #include "norm.h"
+#include "piece.h"
 
 namespace ssla {
 namespace {
@@ -27,27 +28,6 @@ struct Stat {
     float hi, lo, scale;
 };
 
-template <class T, int V>
-struct Piece {
-    T v[V];
-};
-
-// What the compiler has made of 16-bit values ends here: it would otherwise keep all of
-// them as floats from one use to the next, and from row to row.
-template <class T, int V, int K>
-__device__ __forceinline__ void opaque(Piece<T, V> (&p)[K]) {
-    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
-        #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            unsigned x[V / 2];
-            __builtin_memcpy(x, &p[k], sizeof(x));
-            #pragma unroll
-            for (unsigned& w : x) asm("" : "+v"(w));
-            __builtin_memcpy(&p[k], x, sizeof(x));
-        }
-    }
-}
-
 __device__ __forceinline__ float normed(float x, const Stat& f) {
     return fmaf(fmaf(x, kDown, -f.hi), f.scale, -f.lo * f.scale);
 }
@@ -55,54 +35,57 @@ __device__ __forceinline__ float normed(float x, const Stat& f) {
 // ---- rows in registers -----------------------------------------------------------
 // Where a thread works: l-th of a row's lanes, its pieces l, l + lanes, ...  The last
 // piece of a row whose channels are no whole pieces is the row's last V channels;
-// those that the piece before has too are `over`.
+// those that the piece before has too are `over`.  A piece that is not there is the
+// first one again, with a weight of zero in every sum.
 template <int V, int K, bool TAIL>
 struct Columns {
-    int l, c[K], over[K];
+    int group, l, c[K], over[K];                             // row of those at once; thread of the row
     bool on[K];
 
     __device__ __forceinline__ Columns(const LayerNormArgs& a) {
-        l = threadIdx.x & (a.lanes - 1);
-        if (a.lanes > 64) l = threadIdx.x;
+        group = threadIdx.x / a.lanes;
+        l = threadIdx.x - group * a.lanes;
         #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int at = (l + k * a.lanes) * V;
             on[k] = at < a.channels;
-            c[k] = TAIL ? max(min(at, a.channels - V), 0) : at;
-            over[k] = TAIL ? at - c[k] : 0;
+            c[k] = !on[k] ? 0 : TAIL ? min(at, a.channels - V) : at;
+            over[k] = TAIL && on[k] ? at - c[k] : 0;
         }
     }
-    // Whether value i of piece k is the thread's own.
-    __device__ __forceinline__ bool own(int k, int i) const { return on[k] && (!TAIL || i >= over[k]); }
+    // Whether value i of piece k is the thread's own, where piece k is there.
+    __device__ __forceinline__ bool own(int k, int i) const { return !TAIL || i >= over[k]; }
 
     template <class T>
     __device__ __forceinline__ void load(Piece<T, V> (&x)[K], const void* base, long long at) const {
         #pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (on[k]) __builtin_memcpy(&x[k], (const T*)base + at + c[k], sizeof(x[k]));
+        for (int k = 0; k < K; ++k) x[k].load((const T*)base + at + c[k]);
     }
     template <class T>
     __device__ __forceinline__ void store(void* base, long long at, const Piece<T, V>& x, int k) const {
+        if (!on[k]) return;
         T* to = (T*)base + at + c[k];
-        if (!TAIL || over[k] == 0) {
-            __builtin_memcpy(to, &x, sizeof(x));
-        } else {
-            #pragma unroll
-            for (int i = 1; i < V; ++i)
-                if (i >= over[k]) to[i] = x.v[i];
-        }
+        if (!TAIL || over[k] == 0) x.store(to);
+        else x.store_from(to, over[k]);
     }
     // weight or bias
     template <class W>
     __device__ __forceinline__ void params(Piece<W, V> (&w)[K], const void* p, float none) const {
+        float x[V];
+        #pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = none;
         #pragma unroll
         for (int k = 0; k < K; ++k) {
-            #pragma unroll
-            for (int i = 0; i < V; ++i) w[k].v[i] = (W)none;
-            if (p && on[k]) __builtin_memcpy(&w[k], (const W*)p + c[k], sizeof(w[k]));
+            if (p) w[k].load((const W*)p + c[k]);
+            else w[k].set(x);
         }
     }
 };
+template <class T, int V, int K>
+__device__ __forceinline__ void opaque(Piece<T, V> (&x)[K]) {
+    #pragma unroll
+    for (int k = 0; k < K; ++k) x[k].opaque();
+}
 
 // Sum over a row's threads, in each of them.  Two buffers in turn need one barrier.
 template <bool WHOLE, class F>
@@ -118,53 +101,109 @@ __device__ __forceinline__ F row_sum(F s, int lanes, F* waves) {
     return s;
 }
 
-// Row of a thread's group at step i, and how many there are at a time.
-__device__ __forceinline__ int rows_at_once(const LayerNormArgs& a, bool whole) {
-    return whole ? 1 : blockDim.x / a.lanes;
+template <bool WHOLE>
+__device__ __forceinline__ void row_sums(float& s, float& q, int lanes, float* waves, int group = 0) {
+    s = lanes_sum(s, WHOLE ? 64 : lanes);
+    q = lanes_sum(q, WHOLE ? 64 : lanes);
+    if (WHOLE) {
+        const int n = lanes >> 6, first = group * n;
+        if ((threadIdx.x & 63) == 0) {
+            waves[threadIdx.x >> 6] = s;
+            waves[8 + (threadIdx.x >> 6)] = q;
+        }
+        __syncthreads();
+        s = waves[first], q = waves[8 + first];
+        for (int i = 1; i < n; ++i) s += waves[first + i], q += waves[8 + first + i];
+    }
 }
+
+// Pieces one after another: the scheduler otherwise makes floats of all of them first.
+__device__ __forceinline__ void in_turn() { __builtin_amdgcn_sched_barrier(0); }
 
 template <class T, class W, int V, int K, bool WHOLE, bool TAIL>
 __global__ __launch_bounds__(512) void k_ln_rows(const LayerNormArgs a) {
     __shared__ double sums[2][2][8];
     const Columns<V, K, TAIL> col(a);
-    const int per = rows_at_once(a, WHOLE);
+    const int per = blockDim.x / a.lanes;
     Piece<W, V> w[K], b[K];
     col.params(w, a.weight, 1.0f);
     col.params(b, a.bias, 0.0f);
     const long long step = (long long)gridDim.x * per;
     int turn = 0;
-    for (long long row = (long long)blockIdx.x * per + (WHOLE ? 0 : threadIdx.x / a.lanes); row < a.rows;
+    for (long long row = (long long)blockIdx.x * per + col.group; row < a.rows;
          row += step, turn ^= 1) {
         Piece<T, V> x[K], res[K];
         col.load(x, a.x, row * a.xr);
         if (a.res) col.load(res, a.res, row * a.rr);
-        auto at = [&](int k, int i) { return a.res ? (float)x[k].v[i] + (float)res[k].v[i] : (float)x[k].v[i]; };
+        auto at = [&](int k, int i) { return a.res ? x[k].at(i) + res[k].at(i) : x[k].at(i); };
         double sum = 0.0;
         #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            double one = 0.0;
             #pragma unroll
-            for (int i = 0; i < V; ++i) sum += col.own(k, i) ? (double)at(k, i) : 0.0;
+            for (int i = 0; i < V; ++i) one += col.own(k, i) ? (double)at(k, i) : 0.0;
+            sum += col.on[k] ? one : 0.0;
+        }
         opaque(x), opaque(res);
         const double mean = row_sum<WHOLE>(sum, a.lanes, sums[turn][0]) * a.inv_channels;
-        double sq = 0.0;
-        #pragma unroll
-        for (int k = 0; k < K; ++k)
+        // squares in 64 bits
+        auto squares = [&] {
+            double sq = 0.0;
             #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const double d = (double)at(k, i) - mean;
-                sq = col.own(k, i) ? fma(d, d, sq) : sq;
+            for (int k = 0; k < K; ++k) {
+                double one = 0.0;
+                #pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const double d = (double)at(k, i) - mean;
+                    one = col.own(k, i) ? fma(d, d, one) : one;
+                }
+                sq += col.on[k] ? one : 0.0;
             }
-        opaque(x), opaque(res), opaque(w), opaque(b);
-        sq = row_sum<WHOLE>(sq, a.lanes, sums[turn][1]);
-        const Norm n = norm_of(mean, sq * a.inv_channels, a.eps);
+            opaque(x), opaque(res);
+            return row_sum<WHOLE>(sq, a.lanes, sums[turn][1]) * a.inv_channels;
+        };
+        double var;
+        if constexpr (sizeof(T) == 4) {
+            var = squares();
+        } else {
+            // in 32 bits, a third of the forward pass faster: of differences from the mean's
+            // float, whose own mean is what that leaves of the mean
+            const float m = (float)mean;
+            float sq = 0.0f;
+            #pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float one = 0.0f;
+                #pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float d = col.own(k, i) ? at(k, i) - m : 0.0f;
+                    one = fmaf(d, d, one);
+                }
+                sq += col.on[k] ? one : 0.0f;
+            }
+            opaque(x), opaque(res);
+            sq = row_sum<WHOLE>(sq, a.lanes, (float*)sums[turn][1]);
+            // a row whose squares are too large, or that is not finite; all of a row's lanes
+            // agree
+            if (sq < __builtin_inff()) {
+                const double rest = mean - (double)m;
+                var = fma(-rest, rest, (double)sq * a.inv_channels);
+                var = var < 0.0 ? 0.0 : var;
+            } else {
+                if (WHOLE) __syncthreads();
+                var = squares();
+            }
+        }
+        const Norm n = norm_of(mean, var, a.eps);
+        opaque(w), opaque(b);
         const Stat f = {n.hi, n.lo, n.scale};
         if (a.stats && col.l == 0) ((Stat*)a.stats)[row] = f;
         #pragma unroll
         for (int k = 0; k < K; ++k) {
-            if (!col.on[k]) continue;
-            Piece<T, V> y;
+            float o[V];
             #pragma unroll
-            for (int i = 0; i < V; ++i) y.v[i] = (T)fmaf(normed(at(k, i), f), (float)w[k].v[i], (float)b[k].v[i]);
+            for (int i = 0; i < V; ++i) o[i] = fmaf(normed(at(k, i), f), w[k].at(i), b[k].at(i));
+            Piece<T, V> y;
+            y.set(o);
             col.store(a.out, row * a.orow, y, k);
         }
     }
@@ -172,10 +211,10 @@ __global__ __launch_bounds__(512) void k_ln_rows(const LayerNormArgs a) {
 
 template <class T, class W, int V, int K, bool WHOLE, bool TAIL>
 __global__ __launch_bounds__(512) void k_ln_rows_backward(const LayerNormArgs a) {
-    extern __shared__ float joined[];                        // [groups of lanes][2][lanes * K * V], by halves
-    __shared__ float sums[2][2][8];
+    extern __shared__ float joined[];                        // [half of the threads][2 K V + 1]
+    __shared__ float sums[2][16];
     const Columns<V, K, TAIL> col(a);
-    const int per = rows_at_once(a, WHOLE), group = WHOLE ? 0 : threadIdx.x / a.lanes;
+    const int per = blockDim.x / a.lanes, group = col.group;
     const float inv = (float)a.inv_channels;
     Piece<W, V> w[K];
     col.params(w, a.weight, 1.0f);
@@ -186,88 +225,76 @@ __global__ __launch_bounds__(512) void k_ln_rows_backward(const LayerNormArgs a)
         for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.0f;
     const long long step = (long long)gridDim.x * per;
     int turn = 0;
-    for (long long row = (long long)blockIdx.x * per + group; row < a.rows; row += step, turn ^= 1) {
+    for (long long at_row = (long long)blockIdx.x * per; at_row < a.rows; at_row += step, turn ^= 1) {
+        // all rows of a workgroup go through its barriers; one behind the last is that
+        // again, with gradients of zero
+        const bool there = at_row + group < a.rows;
+        const long long row = there ? at_row + group : a.rows - 1;
         Piece<T, V> x[K], res[K], dy[K];
         col.load(x, a.x, row * a.xr);
         if (a.res) col.load(res, a.res, row * a.rr);
         col.load(dy, a.dout, row * a.dor);
         const Stat f = ((const Stat*)a.stats)[row];
-        auto at = [&](int k, int i) { return a.res ? (float)x[k].v[i] + (float)res[k].v[i] : (float)x[k].v[i]; };
+        auto at = [&](int k, int i) { return a.res ? x[k].at(i) + res[k].at(i) : x[k].at(i); };
         float c1 = 0.0f, c2 = 0.0f;
         #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            if (!col.on[k] || !there) dy[k].zero();
             #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float xh = normed(at(k, i), f), g = (float)dy[k].v[i], u = g * (float)w[k].v[i];
-                if (col.own(k, i)) {
-                    dw[k][i] = fmaf(g, xh, dw[k][i]);
-                    db[k][i] += g;
-                    c1 += u;
-                    c2 = fmaf(u, xh, c2);
-                }
+                const float xh = normed(at(k, i), f), g = col.own(k, i) ? dy[k].at(i) : 0.0f, u = g * w[k].at(i);
+                dw[k][i] = fmaf(g, xh, dw[k][i]);
+                db[k][i] += g;
+                c1 += u;
+                c2 = fmaf(u, xh, c2);
             }
-        opaque(x), opaque(res), opaque(dy), opaque(w);
-        if (!a.dx) continue;
-        c1 = lanes_sum(c1, WHOLE ? 64 : a.lanes);
-        c2 = lanes_sum(c2, WHOLE ? 64 : a.lanes);
-        if (WHOLE) {
-            const int n = blockDim.x >> 6;
-            if ((threadIdx.x & 63) == 0) {
-                sums[turn][0][threadIdx.x >> 6] = c1;
-                sums[turn][1][threadIdx.x >> 6] = c2;
-            }
-            __syncthreads();
-            c1 = sums[turn][0][0], c2 = sums[turn][1][0];
-            for (int i = 1; i < n; ++i) c1 += sums[turn][0][i], c2 += sums[turn][1][i];
+            in_turn();
         }
-        c1 *= inv, c2 *= inv;
-        const float r = f.scale * kDown;
-        #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            if (!col.on[k]) continue;
-            Piece<T, V> y;
+        opaque(x), opaque(res), opaque(dy), opaque(w);
+        if (a.dx) {
+            row_sums<WHOLE>(c1, c2, a.lanes, sums[turn], group);
+            c1 *= inv, c2 *= inv;
+            const float r = f.scale * kDown;
             #pragma unroll
-            for (int i = 0; i < V; ++i)
-                y.v[i] = (T)(r * (fmaf((float)dy[k].v[i], (float)w[k].v[i], -c1) - normed(at(k, i), f) * c2));
-            col.store(a.dx, row * a.dxr, y, k);
+            for (int k = 0; k < K; ++k) {
+                float o[V];
+                #pragma unroll
+                for (int i = 0; i < V; ++i) o[i] = r * (fmaf(dy[k].at(i), w[k].at(i), -c1) - normed(at(k, i), f) * c2);
+                Piece<T, V> y;
+                y.set(o);
+                if (there) col.store(a.dx, row * a.dxr, y, k);
+                in_turn();
+            }
         }
     }
     if (!a.parts) return;
     // the workgroup's sums: of its rows' lanes, one half of the groups onto the other
     float* ws = a.ws + (long long)blockIdx.x * 2 * a.channels;
-    if (!WHOLE) {
-        const int width = a.lanes * K * V;
-        for (int n = per / 2; n > 0; n /= 2) {
-            float* to = joined + (group - n) * 2 * width;
-            if (group >= n && group < 2 * n) {
+    constexpr int kOwn = 2 * K * V + 1;
+    for (int n = (per + 1) / 2, m = per; m > 1; m = n, n = (n + 1) / 2) {        // m groups onto n
+        if (group >= n && group < m) {
+            float* to = joined + ((group - n) * a.lanes + col.l) * kOwn;
+            #pragma unroll
+            for (int k = 0; k < K; ++k)
                 #pragma unroll
-                for (int k = 0; k < K; ++k)
-                    #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        to[(k * V + i) * a.lanes + col.l] = dw[k][i];
-                        to[width + (k * V + i) * a.lanes + col.l] = db[k][i];
-                    }
-            }
-            __syncthreads();
-            if (group < n) {
-                const float* from = joined + group * 2 * width;
-                #pragma unroll
-                for (int k = 0; k < K; ++k)
-                    #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        dw[k][i] += from[(k * V + i) * a.lanes + col.l];
-                        db[k][i] += from[width + (k * V + i) * a.lanes + col.l];
-                    }
-            }
-            __syncthreads();
+                for (int i = 0; i < V; ++i) to[k * V + i] = dw[k][i], to[K * V + k * V + i] = db[k][i];
         }
-        if (group) return;
+        __syncthreads();
+        if (group < m - n) {
+            const float* from = joined + (group * a.lanes + col.l) * kOwn;
+            #pragma unroll
+            for (int k = 0; k < K; ++k)
+                #pragma unroll
+                for (int i = 0; i < V; ++i) dw[k][i] += from[k * V + i], db[k][i] += from[K * V + k * V + i];
+        }
+        __syncthreads();
     }
+    if (group) return;
     #pragma unroll
     for (int k = 0; k < K; ++k)
         #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (col.own(k, i)) {
+            if (col.on[k] && col.own(k, i)) {
                 ws[col.c[k] + i] = dw[k][i];
                 ws[a.channels + col.c[k] + i] = db[k][i];
             }
@@ -386,7 +413,8 @@ template <class T, class W>
 const void* kernel(const LayerNormArgs& a, bool backward) {
     constexpr int V = 16 / sizeof(T);
     if (a.vec == 1) return kernel<T, W, 1, 1, false>(a, backward);
-    if (a.lanes > 64) return kernel<T, W, V, 4, true>(a, backward);
+    if (a.lanes > 64)
+        return a.reps == 3 ? kernel<T, W, V, 3, true>(a, backward) : kernel<T, W, V, 4, true>(a, backward);
     return a.reps == 1   ? kernel<T, W, V, 1, false>(a, backward)
            : a.reps == 2 ? kernel<T, W, V, 2, false>(a, backward)
            : a.reps == 3 ? kernel<T, W, V, 3, false>(a, backward)
@@ -410,7 +438,7 @@ hipError_t launch_backward(const LayerNormArgs& a, hipStream_t st) {
     void* pa[] = {&args};
     hipError_t e = hipSuccess;
     if (a.rows && a.reps) {
-        const size_t lds = a.parts && a.lanes <= 64 ? (size_t)(a.threads / 2) * a.reps * a.vec * 2 * 4 : 0;
+        const size_t lds = a.parts ? (size_t)((a.threads / a.lanes) / 2 * a.lanes) * (2 * a.reps * a.vec + 1) * 4 : 0;
         if (lds > 65536) {
             e = hipFuncSetAttribute(kernel<T>(a, true), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
             if (e != hipSuccess) return e;
@@ -435,27 +463,29 @@ void layer_norm_plan(LayerNormArgs& a, int dtype, bool backward) {
     if (a.channels < a.vec) a.vec = 1;
     const int pieces = (a.channels - 1) / a.vec + 1;
     a.parts = 0;
-    a.threads = backward && pieces > 128 ? 512 : NT;
-    if (pieces <= 256) {
-        // as few lanes as hold a row in four pieces each, or in three where that fills them
-        int lanes = 1;
-        while (lanes * 4 < pieces) lanes *= 2;
-        a.lanes = lanes;
-        a.reps = (pieces + lanes - 1) / lanes;
-        if (a.vec == 1) a.lanes = 8, a.reps = 1;
+    // Lanes of a wave, up to four pieces each: more pieces a lane are more bytes in flight
+    // for the registers that a row costs besides.
+    if (a.vec == 1) {
+        a.lanes = 8;
+    } else if (pieces <= 256) {
+        a.lanes = 1;
+        while (a.lanes * 4 < pieces) a.lanes *= 2;
     } else if (pieces <= 2048) {
-        a.threads = (pieces + 255) / 256 * 64;
-        a.lanes = a.threads;
-        a.reps = 4;
+        a.lanes = (pieces + 255) / 256 * 64;
     } else {
         a.threads = NT, a.lanes = NT, a.reps = 0;
         a.wgs = a.rows;
         if (sums) a.parts = a.rows < 256 ? (a.rows + 15) / 16 : 256;
         return;
     }
-    const int per = a.lanes > 64 ? 1 : a.threads / a.lanes;
-    const long long all = ((long long)a.rows + per - 1) / per, most = backward ? 256 * 1024 / a.threads / 2 : 2048 * 256 / a.threads;
-    a.wgs = (int)(all < most ? all : most);
+    a.reps = (pieces + a.lanes - 1) / a.lanes;
+    // Forward: 256 threads, eight workgroups a compute unit.  Backward one of 512 threads
+    // (or two of 256), so that few of them leave sums in the workspace.
+    const int most = !backward ? NT : pieces > 128 ? 512 : NT;
+    a.threads = a.lanes > most || (!backward && a.lanes > 64) ? a.lanes : most / a.lanes * a.lanes;
+    const int per = a.threads / a.lanes;
+    const long long all = ((long long)a.rows + per - 1) / per, cap = (backward ? 256ll * 512 : 2048ll * NT) / a.threads;
+    a.wgs = (int)(all < cap ? all : cap);
     if (sums) a.parts = a.wgs;
 }
 

@@ -27,6 +27,7 @@
 // dh_{t+1} goes through maps, cut where a sequence ends.  States come from those
 // that the forward pass left before each tile (carries).
 #include "linrec.h"
+#include "piece.h"
 
 namespace ssla {
 namespace {
@@ -37,23 +38,6 @@ constexpr int kWindow = kBehind / 4;      // tiles that a lane looks at
 constexpr unsigned long long kPatience = 500000000;          // 5 s at 100 MHz
 constexpr unsigned kUnset = 0xffffffffu;  // an A that was not published: a NaN that no map has
 
-template <class T, int V>
-struct Piece {
-    T v[V];
-};
-
-// What the compiler has made of a piece's values ends here: it would otherwise keep
-// all of them as floats from one use to the next.
-template <class T, int V>
-__device__ __forceinline__ void opaque(Piece<T, V>& p) {
-    if constexpr (sizeof(p) % 4 == 0 && sizeof(T) == 2) {
-        unsigned x[sizeof(p) / 4];
-        __builtin_memcpy(x, &p, sizeof(p));
-        #pragma unroll
-        for (unsigned& w : x) asm("" : "+v"(w));
-        __builtin_memcpy(&p, x, sizeof(p));
-    }
-}
 __device__ __forceinline__ void opaque(int& x) { asm("" : "+v"(x)); }
 
 __device__ __forceinline__ unsigned long long word_of(float A, float L) {
@@ -182,33 +166,42 @@ __device__ __forceinline__ void load(Piece<T, V> (&x)[R], const void* base, long
     if (whole) {
         #pragma unroll
         for (int r = 0; r < R; ++r) {
-            __builtin_memcpy(&x[r], from, sizeof(x[r]));
+            x[r].load(from);
             from += stride;
         }
     } else {
         #pragma unroll
         for (int r = 0; r < R; ++r) {
-            x[r] = Piece<T, V>{};
-            if (r < p.n) __builtin_memcpy(&x[r], from + r * stride, sizeof(x[r]));
+            x[r].zero();
+            if (r < p.n) x[r].load(from + r * stride);
         }
     }
+}
+template <class T, int V, int R>
+__device__ __forceinline__ void opaque(Piece<T, V> (&x)[R]) {
+    #pragma unroll
+    for (int r = 0; r < R; ++r) x[r].opaque();
 }
 // A piece; with TAIL without the channels that another thread has too.
 template <bool TAIL, class T, int V>
 __device__ __forceinline__ void store(T* to, const Piece<T, V>& x, int over) {
-    if (!TAIL || over == 0) {
-        __builtin_memcpy(to, &x, sizeof(x));
-    } else {
-        #pragma unroll
-        for (int i = 1; i < V; ++i)
-            if (i >= over) to[i] = x.v[i];
-    }
+    if (!TAIL || over == 0) x.store(to);
+    else x.store_from(to, over);
+}
+template <bool TAIL, class T, int V>
+__device__ __forceinline__ void store(T* to, const float (&x)[V], int over) {
+    Piece<T, V> y;
+    y.set(x);
+    store<TAIL>(to, y, over);
 }
 template <int V>
-__device__ __forceinline__ Piece<float, V> state_of(const float* pool, long long stride, int slot, int c) {
-    Piece<float, V> h = {};
-    if (pool && slot >= 0) __builtin_memcpy(&h, pool + slot * stride + c, sizeof(h));
-    return h;
+__device__ __forceinline__ void state_of(float (&h)[V], const float* pool, long long stride, int slot, int c) {
+    if (pool && slot >= 0) {
+        __builtin_memcpy(h, pool + slot * stride + c, sizeof(h));
+    } else {
+        #pragma unroll
+        for (int i = 0; i < V; ++i) h[i] = 0.0f;
+    }
 }
 
 // The chain phase: a lane has a channel of the workgroup's and one of four parts of
@@ -391,17 +384,20 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
 
     // The thread's map.  The last state that comes in is kept: its sequence may end
     // in another thread, which may write to its slot before this one is here again.
-    float f[R][V], A[V];
-    Piece<float, V> h = {}, last = {};
+    float f[R][V], A[V], h[V], last[V];
     #pragma unroll
-    for (int i = 0; i < V; ++i) A[i] = 1.0f;
+    for (int i = 0; i < V; ++i) A[i] = 1.0f, h[i] = last[i] = 0.0f;
     #pragma unroll
     for (int r = 0; r < R; ++r) {
-        if (p.starts >> r & 1) last = h = state_of<V>(a.s_in, a.si, linrec_slot(a, p.first[p.y * R + r]), p.c);
+        if (p.starts >> r & 1) {
+            state_of(last, a.s_in, a.si, linrec_slot(a, p.first[p.y * R + r]), p.c);
+            #pragma unroll
+            for (int i = 0; i < V; ++i) h[i] = last[i];
+        }
         #pragma unroll
         for (int i = 0; i < V; ++i) {
-            f[r][i] = gate_of((float)g[r].v[i]).a;
-            h.v[i] = fmaf(f[r][i], h.v[i], (float)v[r].v[i]);
+            f[r][i] = gate_of(g[r].at(i)).a;
+            h[i] = fmaf(f[r][i], h[i], v[r].at(i));
             A[i] *= f[r][i];
         }
     }
@@ -409,11 +405,10 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
         #pragma unroll
         for (int i = 0; i < V; ++i) {
             sA[p.y * row + p.x * V + i] = p.starts ? kCut : A[i];
-            sL[p.y * row + p.x * V + i] = h.v[i];
+            sL[p.y * row + p.x * V + i] = h[i];
         }
     }
-    #pragma unroll
-    for (int r = 0; r < R; ++r) opaque(v[r]);
+    opaque(v), opaque(q);
     opaque(p.t), opaque(p.c);
     __syncthreads();
 
@@ -425,7 +420,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
     __syncthreads();
     if (p.n == 0) return;
     #pragma unroll
-    for (int i = 0; i < V; ++i) h.v[i] = sL[p.y * row + p.x * V + i];
+    for (int i = 0; i < V; ++i) h[i] = sL[p.y * row + p.x * V + i];
     if (a.carries && p.t % a.carry == 0)
         store<TAIL>(a.carries + (long long)(p.t / a.carry) * a.channels + p.c, h, p.over);
     int slot = linrec_slot(a, p.in);
@@ -434,26 +429,33 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
     for (int r = 0; r < R; ++r) {
         if (p.starts >> r & 1) {
             slot = linrec_slot(a, p.first[p.y * R + r]);
-            h = p.starts >> r == 1 ? last : state_of<V>(a.s_in, a.si, slot, p.c);
+            if (p.starts >> r == 1) {
+                #pragma unroll
+                for (int i = 0; i < V; ++i) h[i] = last[i];
+            } else {
+                state_of(h, a.s_in, a.si, slot, p.c);
+            }
         }
-        Piece<T, V> y;
+        float o[V];
         #pragma unroll
         for (int i = 0; i < V; ++i) {
-            h.v[i] = fmaf(f[r][i], h.v[i], (float)v[r].v[i]);
-            y.v[i] = (T)(a.q ? (float)q[r].v[i] * h.v[i] : h.v[i]);
+            h[i] = fmaf(f[r][i], h[i], v[r].at(i));
+            o[i] = a.q ? q[r].at(i) * h[i] : h[i];
         }
         if (slot >= 0 && r < p.n) {
-            store<TAIL>(out, y, p.over);
+            store<TAIL>(out, o, p.over);
             if (a.s_out && (p.ends >> r & 1)) store<TAIL>(a.s_out + slot * a.so + p.c, h, p.over);
         } else if (a.carries && r < p.n) {                   // of no sequence: zeros
-            store<TAIL>(out, Piece<T, V>{}, p.over);
+            Piece<T, V> none;
+            none.zero();
+            store<TAIL>(out, none, p.over);
         }
         out += a.ot;
     }
 }
 
 template <class T, int V, int R, bool TAIL>
-__global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(const LinRecArgs a) {
+__global__ __launch_bounds__(NT, 4) void k_linrec_backward(const LinRecArgs a) {
     extern __shared__ __align__(16) char smem[];
     __shared__ Shared sh;
     if (blockIdx.x >= (unsigned)(a.tiles * a.blocks)) {
@@ -474,20 +476,18 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(
     if (a.dout) load(d, a.dout, a.dot, p, whole);
     p.mark(a, sh);
 
-    // states, as the forward pass had them: hs[r] behind token r, h0 before the first;
-    // w: the gates' slopes
-    float f[R][V], w[R][V], A[V], hs[R][V];
-    Piece<float, V> h = {}, h0;
+    // states, as the forward pass had them; w: the gates' slopes
+    float f[R][V], w[R][V], A[V], h[V];
     #pragma unroll
-    for (int i = 0; i < V; ++i) A[i] = 1.0f;
+    for (int i = 0; i < V; ++i) A[i] = 1.0f, h[i] = 0.0f;
     #pragma unroll
     for (int r = 0; r < R; ++r) {
-        if (p.starts >> r & 1) h = state_of<V>(a.s_in, a.si, linrec_slot(a, p.first[p.y * R + r]), p.c);
+        if (p.starts >> r & 1) state_of(h, a.s_in, a.si, linrec_slot(a, p.first[p.y * R + r]), p.c);
         #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const Gate gate = gate_of((float)g[r].v[i]);
+            const Gate gate = gate_of(g[r].at(i));
             f[r][i] = gate.a, w[r][i] = gate.slope;
-            h.v[i] = fmaf(f[r][i], h.v[i], (float)v[r].v[i]);
+            h[i] = fmaf(f[r][i], h[i], v[r].at(i));
             A[i] *= f[r][i];
         }
     }
@@ -495,11 +495,10 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(
         #pragma unroll
         for (int i = 0; i < V; ++i) {
             sA[p.y * row + p.x * V + i] = p.starts ? kCut : A[i];
-            sL[p.y * row + p.x * V + i] = h.v[i];
+            sL[p.y * row + p.x * V + i] = h[i];
         }
     }
-    #pragma unroll
-    for (int r = 0; r < R; ++r) opaque(v[r]);
+    opaque(v), opaque(q), opaque(d);
     __syncthreads();
     Chain chain;
     chain.fold<false>(a, sA, sL, row, p.cb * a.cols, V);
@@ -507,13 +506,31 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(
     chain.spread<false>(a, sA, sL, row,
                         p.begun && a.tiles > 1 && chain.on ? a.carries[(long long)p.tile * a.channels + at] : 0.0f);
     __syncthreads();
+    // Once more, from the state before the thread: dq is done here; what is left of a
+    // token is its gate, its slope times the state before it, and what it adds to its
+    // state's gradient.
+    float e[R][V];
+    T* dq = (T*)a.dq + (long long)p.t * a.dqt + p.c;
+    int slot = linrec_slot(a, p.in);
     #pragma unroll
-    for (int i = 0; i < V; ++i) h0.v[i] = h.v[i] = p.on ? sL[p.y * row + p.x * V + i] : 0.0f;
+    for (int i = 0; i < V; ++i) h[i] = p.on ? sL[p.y * row + p.x * V + i] : 0.0f;
     #pragma unroll
     for (int r = 0; r < R; ++r) {
-        if (p.starts >> r & 1) h = state_of<V>(a.s_in, a.si, linrec_slot(a, p.first[p.y * R + r]), p.c);
+        if (p.starts >> r & 1) {
+            slot = linrec_slot(a, p.first[p.y * R + r]);
+            state_of(h, a.s_in, a.si, slot, p.c);
+        }
+        float o[V];
         #pragma unroll
-        for (int i = 0; i < V; ++i) hs[r][i] = h.v[i] = fmaf(f[r][i], h.v[i], (float)v[r].v[i]);
+        for (int i = 0; i < V; ++i) {
+            const float y = a.dout ? d[r].at(i) : 0.0f;
+            w[r][i] *= h[i];
+            h[i] = fmaf(f[r][i], h[i], v[r].at(i));
+            e[r][i] = a.q ? q[r].at(i) * y : y;
+            o[i] = slot < 0 ? 0.0f : y * h[i];               // of no sequence: zeros
+        }
+        if (a.dq && r < p.n) store<TAIL>(dq, o, p.over);
+        dq += a.dqt;
     }
     __syncthreads();
 
@@ -522,30 +539,25 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(
         const unsigned m = p.starts & ((2u << r) - 1);
         return linrec_slot(a, m ? p.first[p.y * R + 31 - __builtin_clz(m)] : p.in);
     };
-    // what token r adds to its state's gradient
-    auto read_out = [&](int r, int i) {
-        const float y = a.dout ? (float)d[r].v[i] : 0.0f;
-        return a.q ? (float)q[r].v[i] * y : y;
-    };
     // the map of messages
-    Piece<float, V> m = {};
+    float m[V];
+    #pragma unroll
+    for (int i = 0; i < V; ++i) m[i] = 0.0f;
     #pragma unroll
     for (int r = R - 1; r >= 0; --r) {
-        if (p.ends >> r & 1) m = state_of<V>(a.ds_out, a.dso, slot_at(r), p.c);
+        if (p.ends >> r & 1) state_of(m, a.ds_out, a.dso, slot_at(r), p.c);
         if (r < p.n) {
             #pragma unroll
-            for (int i = 0; i < V; ++i) m.v[i] = f[r][i] * (read_out(r, i) + m.v[i]);
+            for (int i = 0; i < V; ++i) m[i] = f[r][i] * (e[r][i] + m[i]);
         }
     }
     if (p.on) {
         #pragma unroll
         for (int i = 0; i < V; ++i) {
             sA[p.y * row + p.x * V + i] = p.ends ? kCut : A[i];
-            sL[p.y * row + p.x * V + i] = m.v[i];
+            sL[p.y * row + p.x * V + i] = m[i];
         }
     }
-    #pragma unroll
-    for (int r = 0; r < R; ++r) opaque(d[r]), opaque(q[r]);
     opaque(p.t), opaque(p.c);
     __syncthreads();
     chain.fold<true>(a, sA, sL, row, p.cb * a.cols, V);
@@ -556,39 +568,31 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(
     __syncthreads();
     if (p.n == 0) return;
     #pragma unroll
-    for (int i = 0; i < V; ++i) m.v[i] = sL[p.y * row + p.x * V + i];
-    int slot = slot_at(R - 1);
+    for (int i = 0; i < V; ++i) m[i] = sL[p.y * row + p.x * V + i];
+    slot = slot_at(R - 1);
     T* dg = (T*)a.dg + (long long)(p.t + R - 1) * a.dgt + p.c;
     T* dv = (T*)a.dv + (long long)(p.t + R - 1) * a.dvt + p.c;
-    T* dq = (T*)a.dq + (long long)(p.t + R - 1) * a.dqt + p.c;
     #pragma unroll
     for (int r = R - 1; r >= 0; --r) {
         if (p.ends >> r & 1) {
             slot = slot_at(r);
-            m = state_of<V>(a.ds_out, a.dso, slot, p.c);
+            state_of(m, a.ds_out, a.dso, slot, p.c);
         }
         if (r < p.n) {
-            const bool begins = p.starts >> r & 1, none = slot < 0;      // of no sequence: zeros
-            Piece<T, V> yv, yg, yq;
-            Piece<float, V> was;                             // state before the token
-            #pragma unroll
-            for (int i = 0; i < V; ++i) was.v[i] = r ? hs[r ? r - 1 : 0][i] : h0.v[i];
-            if (begins) was = state_of<V>(a.s_in, a.si, slot, p.c);
+            const bool none = slot < 0;
+            float dh[V], z[V];
             #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float dh = read_out(r, i) + m.v[i];
-                yv.v[i] = (T)dh;
-                yg.v[i] = (T)(dh * was.v[i] * w[r][i]);
-                yq.v[i] = (T)(a.dout ? (float)d[r].v[i] * hs[r][i] : 0.0f);
-                m.v[i] = f[r][i] * dh;
+                const float x = e[r][i] + m[i];
+                m[i] = f[r][i] * x;
+                dh[i] = none ? 0.0f : x;
+                z[i] = none ? 0.0f : x * w[r][i];
             }
-            if (none) yv = yg = yq = Piece<T, V>{};
-            if (a.dg) store<TAIL>(dg, yg, p.over);
-            if (a.dv) store<TAIL>(dv, yv, p.over);
-            if (a.dq) store<TAIL>(dq, yq, p.over);
-            if (a.ds_in && begins && !none) store<TAIL>(a.ds_in + slot * a.dsi + p.c, m, p.over);
+            if (a.dg) store<TAIL>(dg, z, p.over);
+            if (a.dv) store<TAIL>(dv, dh, p.over);
+            if (a.ds_in && (p.starts >> r & 1) && !none) store<TAIL>(a.ds_in + slot * a.dsi + p.c, m, p.over);
         }
-        dg -= a.dgt, dv -= a.dvt, dq -= a.dqt;
+        dg -= a.dgt, dv -= a.dvt;
     }
 }
 
@@ -607,8 +611,14 @@ size_t lds_bytes(const LinRecArgs& a) {
 template <class T> constexpr int kVec = 16 / sizeof(T);
 #ifndef FR
 #define FR 8
+#endif
+#ifndef BR
 #define BR 4
+#endif
+#ifndef FR2
 #define FR2 4
+#endif
+#ifndef BR2
 #define BR2 2
 #endif
 constexpr int tokens_of(bool wide, bool backward) { return wide ? backward ? BR : FR : backward ? BR2 : FR2; }

@@ -591,6 +591,7 @@ typedef struct SslaHipLinRec {
     float* state_out;
     long long state_in_stride, state_out_stride;     /* floats, >= channels */
     float* carries;
+    int wait_us;               /* 0: 200; see ssla_hip_linrec */
 } SslaHipLinRec;
 
 /* Gradients of the call *d that kept its carries, from those of out and of the
@@ -615,6 +616,9 @@ typedef struct SslaHipLinRecGrad {
  * n_tokens, n_seqs and whether there are cu_seqlens. */
 int ssla_hip_linrec_carries(const SslaHipLinRec* d, size_t* nbytes);
 int ssla_hip_linrec_workspace(const SslaHipLinRec* d, size_t* nbytes);
+/* Both cut the tokens into tiles that wait for one another's results; one that has
+ * waited for wait_us (negative: not at all) makes what it lacks itself, to the same
+ * bits. */
 int ssla_hip_linrec(const SslaHipLinRec* d, void* workspace, size_t workspace_bytes, void* stream);
 int ssla_hip_linrec_backward(const SslaHipLinRec* d, const SslaHipLinRecGrad* g, void* workspace,
                              size_t workspace_bytes, void* stream);

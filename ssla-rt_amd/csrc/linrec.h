@@ -34,13 +34,12 @@ struct LinRecArgs {
     int cols, blocks;                     // threads along the channels; workgroups along them
     int lanes, tile, tiles;               // threads along the tokens, their tokens, tiles of all tokens
     int carry;                            // tokens of a tile of the backward pass
-    unsigned* tickets;                    // workspace: a counter for each block of channels
-    unsigned long long* words;            // [block][kBehind + place in the chain][kChannels] maps and states
+    unsigned patience;                    // ticks of 10 ns that a workgroup waits for another
+    unsigned long long* words;            // workspace: [block][kBehind + place in the chain][kChannels] maps and states
 };
 
 constexpr int kLinRecThreads = 256;
 constexpr int kChannels = 64;             // most of a workgroup
-constexpr int kTicketStep = 32;           // counters lie 128 bytes apart
 constexpr int kBehind = 32;               // places before a chain's first one, never published
 
 void linrec_plan(LinRecArgs& a, int dtype, bool backward);
@@ -49,7 +48,7 @@ inline size_t linrec_words(const LinRecArgs& a) {
     return a.tiles > 1 ? ((size_t)a.tiles + kBehind) * a.blocks * kChannels : 0;
 }
 inline size_t linrec_bytes(const LinRecArgs& a) {
-    return a.tiles > 1 ? linrec_words(a) * 8 + (size_t)a.blocks * kTicketStep * 4 : 0;
+    return linrec_words(a) * 8;
 }
 inline size_t linrec_carries(const LinRecArgs& a) {
     return (size_t)((a.n_tokens + a.carry - 1) / a.carry) * a.channels * 4;
@@ -66,6 +65,7 @@ struct Gate {
     float a, slope;
 };
 __device__ __forceinline__ Gate gate_of(float x) {
+    #pragma clang fp contract(off)
     const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(x));
     const float s = e * __builtin_amdgcn_rcpf(1.0f + e);
     return Gate{x > 0.0f ? 1.0f - s : s, fmaf(-s, s, s)};

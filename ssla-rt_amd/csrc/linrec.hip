@@ -20,8 +20,10 @@
 // tokens, so that reruns give the same bits whatever was published when.  A
 // published word is 64 bits, {A, L}, stored and loaded by relaxed device-scope
 // atomics: whoever sees A sees L, with no fence (a release fence would write back
-// the L2).  Tiles are taken by tickets, so a tile waits only for ones
-// that run already; the wait is bounded all the same (then states are NaN).
+// the L2).  A tile that has waited for long makes the missing maps itself, from the
+// tensors and in the same steps (made_here), so that none depends on another's
+// workgroup being started.  Drawing tiles by tickets instead cost 12 us of 57 where one
+// block of channels has 1565 of them (8 ns an atomic on one address).
 //
 // Backward, the same from the last token to the first: the message m_t = a_{t+1}
 // dh_{t+1} goes through maps, cut where a sequence ends.  States come from those
@@ -29,13 +31,15 @@
 #include "linrec.h"
 #include "piece.h"
 
+// Maps are made in two places, to the same bits: nothing is fused but by fmaf.
+#pragma clang fp contract(off)
+
 namespace ssla {
 namespace {
 
 constexpr int NT = kLinRecThreads;
 constexpr float kCut = -1.0f;             // in place of a map's A, which is >= 0 or NaN
 constexpr int kWindow = kBehind / 4;      // tiles that a lane looks at
-constexpr unsigned long long kPatience = 500000000;          // 5 s at 100 MHz
 constexpr unsigned kUnset = 0xffffffffu;  // an A that was not published: a NaN that no map has
 
 __device__ __forceinline__ void opaque(int& x) { asm("" : "+v"(x)); }
@@ -52,10 +56,14 @@ constexpr int kMaxTile = NT * 8;          // one thread along the channels, eigh
 // What a workgroup knows of its tile's tokens: where sequences begin (the token behind
 // the tile too), and which.
 struct Shared {
-    int ticket;
     unsigned mask[kMaxTile / 32 + 1];
     __device__ __forceinline__ bool begins(int i) const { return mask[i >> 5] >> (i & 31) & 1; }
 };
+
+// First token of sequence i (the last one's end for i = n_seqs), of those in a.cu.
+__device__ __forceinline__ int boundary(const LinRecArgs& a, long long i) {
+    return i <= a.n_seqs ? (int)min((long long)max(a.cu[i], 0), a.n_tokens) : 0x7fffffff;
+}
 
 // Where a thread works.
 template <int V, int R>
@@ -71,30 +79,22 @@ struct Place {
     bool begun;                           // the tile's first token belongs to a sequence that began before it
     int at, next;                         // a boundary of the thread's, and the one behind it
 
-    __device__ __forceinline__ static int boundary(const LinRecArgs& a, long long i) {
-        return i <= a.n_seqs ? (int)min((long long)max(a.cu[i], 0), a.n_tokens) : 0x7fffffff;
-    }
-
     __device__ __forceinline__ void find(const LinRecArgs& a, Shared& sh, bool backward) {
         const int tid = threadIdx.x, nt = blockDim.x;
-        cb = blockIdx.x % a.blocks;
-        unsigned ticket = 0;
-        if (a.tiles > 1 && tid == 0)
-            ticket = __hip_atomic_fetch_add(a.tickets + cb * kTicketStep, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        // meanwhile: one of nt boundaries spread over all
+        // Blocks go to the eight XCDs, each with an L2 of its own, in turn: a tile's are put
+        // on one, as rows that are no whole lines share lines between them.
+        const int eight = blockIdx.x / (8 * a.blocks), k = blockIdx.x - eight * 8 * a.blocks,
+                  wide = min(8, a.tiles - 8 * eight);
+        cb = k / wide;
+        place = 8 * eight + k - cb * wide;
+        tile = backward ? a.tiles - 1 - place : place;
+        // one of nt boundaries spread over all
         if (a.cu) {
             const int step = a.n_seqs / nt + 1;
             at = boundary(a, (long long)tid * step);
             if (step == 1) next = boundary(a, tid + 1);
         }
         for (int i = tid; i <= a.tile / 32; i += nt) sh.mask[i] = 0;
-        place = 0;
-        if (a.tiles > 1) {
-            if (tid == 0) sh.ticket = (int)ticket;
-            __syncthreads();
-            place = __builtin_amdgcn_readfirstlane(sh.ticket);
-        }
-        tile = backward ? a.tiles - 1 - place : place;
         y = tid / a.cols;
         x = tid - y * a.cols;
         const int p = cb * a.cols + x;
@@ -144,7 +144,7 @@ struct Place {
         } else {
             const int len = a.seq_len, s = (t0 + len - 1) / len;
             before = t0 ? (t0 - 1) / len : -1;
-            if (a.tiles <= 1) __syncthreads();                // the masks are clear
+            __syncthreads();                                  // the masks are clear
             for (long long i = s + tid; i * len <= t1; i += nt) set(sh, (int)(i * len), (int)i);
         }
         __syncthreads();
@@ -204,6 +204,95 @@ __device__ __forceinline__ void state_of(float (&h)[V], const float* pool, long 
     }
 }
 
+// The sequences' first tokens, as one walks over the tokens: seq is the last sequence
+// that begins at token t or before it.
+struct Walk {
+    const LinRecArgs& a;
+    int t, seq;
+
+    __device__ __forceinline__ int first(int i) const {
+        return a.cu ? boundary(a, i) : i <= a.n_seqs ? i * a.seq_len : 0x7fffffff;
+    }
+    __device__ Walk(const LinRecArgs& args, int token) : a(args), t(token) {
+        int lo = -1, hi = a.n_seqs + 1;                      // first(lo) <= t < first(hi)
+        while (hi - lo > 1) {
+            const int mid = lo + (hi - lo) / 2;
+            if (first(mid) <= t) lo = mid;
+            else hi = mid;
+        }
+        seq = lo;
+    }
+    __device__ __forceinline__ void up() {
+        ++t;
+        while (first(seq + 1) <= t) ++seq;
+    }
+    __device__ __forceinline__ void down() {
+        --t;
+        while (seq >= 0 && first(seq) > t) --seq;
+    }
+};
+
+// (A, L), then (x, l)
+__device__ __forceinline__ void join(float& A, float& L, float x, float l) {
+    L = x < 0.0f ? l : fmaf(x, L, l);
+    A = x < 0.0f || A < 0.0f ? kCut : A * x;
+}
+
+// Word of a tile for one channel, in the steps of its own workgroup: what that would
+// publish first.
+template <class T, int R, bool BACK>
+__device__ unsigned long long made_here(const LinRecArgs& a, int place, int channel) {
+    const int tile = BACK ? a.tiles - 1 - place : place, t0 = tile * a.tile, per = a.lanes / 4;
+    auto value = [&](const void* p, long long stride, int t) { return (float)((const T*)p)[t * stride + channel]; };
+    float tA = 1.0f, tL = 0.0f;
+    for (int part = 0; part < 4; ++part) {
+        float mA = 1.0f, mL = 0.0f;
+        for (int i = part * per; i < part * per + per; ++i) {
+            const int y = BACK ? a.lanes - 1 - i : i, t = t0 + y * R;
+            float A = 1.0f, x = 0.0f;
+            bool cut = false;
+            if (!BACK) {
+                Walk at(a, t - 1);
+                for (int r = 0; r < R; ++r) {
+                    const int was = at.seq;
+                    at.up();
+                    if (at.seq != was) {
+                        const int slot = linrec_slot(a, at.seq);
+                        cut = true;
+                        x = a.s_in && slot >= 0 ? a.s_in[slot * a.si + channel] : 0.0f;
+                    }
+                    const float f = gate_of(value(a.g, a.gt, t + r)).a;
+                    x = fmaf(f, x, value(a.v, a.vt, t + r));
+                    A *= f;
+                }
+            } else {
+                for (int r = 0; r < R; ++r) A *= gate_of(t + r < a.n_tokens ? value(a.g, a.gt, t + r) : 0.0f).a;
+                Walk at(a, t + R);
+                for (int r = R - 1; r >= 0; --r) {
+                    const int was = at.seq;
+                    at.down();
+                    if (t + r >= a.n_tokens) continue;
+                    if (at.seq != was || t + r + 1 >= a.n_tokens) {
+                        const int slot = linrec_slot(a, at.seq);
+                        cut = true;
+                        x = a.ds_out && slot >= 0 ? a.ds_out[slot * a.dso + channel] : 0.0f;
+                    }
+                    const float d = a.dout ? value(a.dout, a.dot, t + r) : 0.0f;
+                    const float e = a.q ? value(a.q, a.qt, t + r) * d : d;
+                    x = gate_of(value(a.g, a.gt, t + r)).a * (e + x);
+                }
+            }
+            join(mA, mL, cut ? kCut : A, x);
+        }
+        join(tA, tL, mA, mL);
+    }
+    const Walk at(a, BACK ? t0 + a.tile - 1 : t0 - 1);
+    Walk next = at;
+    next.up();
+    const bool open = BACK ? place > 0 && next.seq == at.seq : next.seq == at.seq && at.seq >= 0 && at.seq < a.n_seqs;
+    return word_of(open ? tA : kCut, tL);
+}
+
 // The chain phase: a lane has a channel of the workgroup's and one of four parts of
 // its threads (of the window, while it looks back); waves have sixteen channels.
 struct Chain {
@@ -241,11 +330,6 @@ struct Chain {
             join(tA, tL, A[g], L[g]);
         }
     }
-    // (A, L), then (x, l)
-    __device__ __forceinline__ static void join(float& A, float& L, float x, float l) {
-        L = x < 0.0f ? l : fmaf(x, L, l);
-        A = x < 0.0f || A < 0.0f ? kCut : A * x;
-    }
     // Puts the states before the threads, from that before the tile, into sL's place.
     template <bool BACK>
     __device__ __forceinline__ void spread(const LinRecArgs& a, const float* sA, float* sL, int row, float state) {
@@ -270,8 +354,9 @@ struct Chain {
             }
     }
     // The state before place p of the chain, after publishing the tile's map; `open`: a
-    // sequence goes on from the place before into this one.
-    __device__ __forceinline__ float before(const LinRecArgs& a, int block, int p, bool open) {
+    // sequence goes on from the place before into this one.  `channel`: this one's.
+    template <class T, int R, bool BACK>
+    __device__ __forceinline__ float before(const LinRecArgs& a, int block, int p, bool open, int channel) {
         // word of this channel at place p
         unsigned long long* word = a.words + ((long long)block * (a.tiles + kBehind) + kBehind + p) * kChannels + ch;
         auto publish = [&](float x, float l) {
@@ -279,9 +364,38 @@ struct Chain {
         };
         publish(open ? tA : kCut, tL);
         if (!open) return 0.0f;
-        const float state = look_back(word);
+        float state;
+        if (!look_back(word, state, a.patience)) state = on ? alone<T, R, BACK>(a, word, p, channel) : 0.0f;
         if (!(tA < 0.0f)) publish(kCut, fmaf(tA, state, tL));
         return state;
+    }
+    // The same without waiting for anyone.  What is made here is published in the tile's
+    // place, unless something is by now, which then counts: whoever knows a state has seen
+    // all words from its sequence's beginning on, and only then may it write the sequence's
+    // last state, perhaps in the place of the first.  A map made from that too late is thus
+    // never used.
+    template <class T, int R, bool BACK>
+    __device__ float alone(const LinRecArgs& a, unsigned long long* word, int p, int channel) {
+        auto map = [&](int j) {
+            unsigned long long* at = word - (p - j) * kChannels;
+            unsigned long long w = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if ((unsigned)w != kUnset) return w;
+            const unsigned long long made = made_here<T, R, BACK>(a, j, channel);
+            w = ~0ull;
+            return __hip_atomic_compare_exchange_strong(at, &w, made, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                                        __HIP_MEMORY_SCOPE_AGENT)
+                       ? made
+                       : w;
+        };
+        int j = p - 1;
+        unsigned long long w = map(j);
+        while (!(map_a(w) < 0.0f) && j > 0) w = map(--j);    // the first place's is a state
+        float h = map_l(w);
+        while (++j < p) {
+            w = map(j);
+            h = map_a(w) < 0.0f ? map_l(w) : fmaf(map_a(w), h, map_l(w));
+        }
+        return h;
     }
     // Looks at the nearest 4 N tiles, N a lane.  True: h is the state, from the nearest
     // published one through the maps behind it, in their order.  False: there is none
@@ -319,23 +433,22 @@ struct Chain {
         return __all(!on || mode == kKnown);
     }
     // A word a lane until the nearest tile has published something (a state, where a
-    // sequence begins in it), then eight.
-    __device__ __forceinline__ float look_back(const unsigned long long* word) {
+    // sequence begins in it), then eight.  False: patience ran out.
+    __device__ __forceinline__ bool look_back(const unsigned long long* word, float& h, unsigned patience) {
         const unsigned long long t0 = wall_clock64();
-        float h;
         bool nearest;
         while (!look<1>(word, h, nearest)) {
             if (nearest) {
                 while (!look<kWindow>(word, h, nearest)) {
-                    if (wall_clock64() - t0 > kPatience) return __builtin_nanf("");
+                    if (wall_clock64() - t0 > patience) return false;
                     __builtin_amdgcn_s_sleep(1);
                 }
                 break;
             }
-            if (wall_clock64() - t0 > kPatience) return __builtin_nanf("");
+            if (wall_clock64() - t0 > patience) return false;
             __builtin_amdgcn_s_sleep(1);
         }
-        return h;
+        return true;
     }
 };
 
@@ -415,7 +528,8 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
     // the tile's map, the state before it, and those before its threads
     Chain chain;
     chain.fold<false>(a, sA, sL, row, p.cb * a.cols, V);
-    const float state = a.tiles > 1 ? chain.before(a, p.cb, p.place, p.begun) : 0.0f;
+    const int channel = min((p.cb * a.cols + chain.ch / V) * V, a.channels - V) + chain.ch % V;
+    const float state = a.tiles > 1 ? chain.before<T, R, false>(a, p.cb, p.place, p.begun, channel) : 0.0f;
     chain.spread<false>(a, sA, sL, row, state);
     __syncthreads();
     if (p.n == 0) return;
@@ -563,7 +677,7 @@ __global__ __launch_bounds__(NT, 4) void k_linrec_backward(const LinRecArgs a) {
     chain.fold<true>(a, sA, sL, row, p.cb * a.cols, V);
     // a sequence that goes on behind the tile
     const bool open = p.place > 0 && !sh.begins(a.tile);
-    const float state = a.tiles > 1 ? chain.before(a, p.cb, p.place, open) : 0.0f;
+    const float state = a.tiles > 1 ? chain.before<T, R, true>(a, p.cb, p.place, open, at) : 0.0f;
     chain.spread<true>(a, sA, sL, row, state);
     __syncthreads();
     if (p.n == 0) return;
@@ -596,11 +710,10 @@ __global__ __launch_bounds__(NT, 4) void k_linrec_backward(const LinRecArgs a) {
     }
 }
 
-// Empties the chain: no word is published, no ticket taken.
-__global__ __launch_bounds__(NT) void k_linrec_clear(ulonglong2* words, long long n, unsigned* tickets, int nt) {
-    const long long id = (long long)blockIdx.x * NT + threadIdx.x;
-    for (long long i = id; i < n; i += (long long)gridDim.x * NT) words[i] = ulonglong2{~0ull, ~0ull};
-    for (long long i = id; i < nt; i += (long long)gridDim.x * NT) tickets[i] = 0;
+// Empties the chain: no word is published.
+__global__ __launch_bounds__(NT) void k_linrec_clear(ulonglong2* words, long long n) {
+    for (long long i = (long long)blockIdx.x * NT + threadIdx.x; i < n; i += (long long)gridDim.x * NT)
+        words[i] = ulonglong2{~0ull, ~0ull};
 }
 
 size_t lds_bytes(const LinRecArgs& a) {
@@ -636,8 +749,7 @@ hipError_t launch(const LinRecArgs& a, hipStream_t st) {
     const int nt = (a.cols * a.lanes + 63) / 64 * 64;
     if (a.tiles > 1) {
         long long n = (long long)linrec_words(a) / 2;
-        int tickets = a.blocks * kTicketStep;
-        void* pc[] = {&args.words, &n, &args.tickets, &tickets};
+        void* pc[] = {&args.words, &n};
         const long long wgs = (n + 4 * NT - 1) / (4 * NT);   // four stores a thread
         const hipError_t e = hipLaunchKernel((const void*)k_linrec_clear, dim3((unsigned)(wgs < 1024 ? wgs : 1024)),
                                              dim3(NT), pc, 0, st);

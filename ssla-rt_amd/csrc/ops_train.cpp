@@ -44,6 +44,7 @@ int check_linrec(const SslaHipLinRec* d, Call call, const char* fn) {
     if (!is_dtype(d->dtype)) return refuse(f + "dtype must be SSLA_F32, SSLA_BF16 or SSLA_F16");
     if (d->channels < 1 || d->channels > kMaxCount) return refuse(f + "channels must be 1 .. 2^31 - 2^16");
     if (d->n_seqs < 0 || d->n_slots < 0) return refuse(f + "negative count");
+    if (d->wait_us > 1000000) return refuse(f + "wait_us must be at most 10^6");
     if (d->n_seqs > kMaxCount) return refuse(f + "n_seqs must be at most 2^31 - 2^16");
     if (!is_stride(d->gate_stride) || !is_stride(d->v_stride) || !is_stride(d->q_stride) || !is_stride(d->out_stride))
         return refuse(f + "strides must be 0 .. 2^40");
@@ -110,6 +111,7 @@ LinRecArgs linrec_args(const SslaHipLinRec* d, const SslaHipLinRecGrad* g) {
     a.cu = d->cu_seqlens, a.slots = d->slots;
     a.s_in = d->state_in, a.s_out = d->state_out, a.si = d->state_in_stride, a.so = d->state_out_stride;
     a.carries = d->carries;
+    a.patience = d->wait_us < 0 ? 0 : (d->wait_us ? d->wait_us : 200) * 100u;
     a.n_tokens = d->n_tokens, a.n_seqs = d->n_seqs, a.n_slots = d->n_slots, a.channels = d->channels;
     if (!d->slots && !d->state_in && !d->state_out) a.n_slots = d->n_seqs;
     a.seq_len = d->n_seqs ? (int)(d->n_tokens / d->n_seqs) : 0;
@@ -124,17 +126,23 @@ LinRecArgs linrec_args(const SslaHipLinRec* d, const SslaHipLinRecGrad* g) {
     return a;
 }
 
+// Workspace of either pass.
+size_t linrec_need(const SslaHipLinRec* d) {
+    const SslaHipLinRecGrad none{};
+    const size_t one = linrec_bytes(linrec_args(d, nullptr)), other = linrec_bytes(linrec_args(d, &none));
+    return one > other ? one : other;
+}
+
 // The grid's limit, and the workspace.
-int linrec_bind(LinRecArgs& a, void* workspace, size_t bytes, const char* fn) {
+int linrec_bind(LinRecArgs& a, const SslaHipLinRec* d, void* workspace, size_t bytes, const char* fn) {
     if (!launchable(a.tiles, a.blocks, 1, kLinRecThreads) ||
         !launchable((long long)a.tiles * a.blocks + a.n_seqs / kLinRecThreads + 1, 1, 1, kLinRecThreads))
         return refuse(std::string(fn) + ": too many tokens and channels");
-    const size_t need = linrec_bytes(a);
+    const size_t need = linrec_need(d);
     if (!need) return SSLA_OK;
     if (!workspace || bytes < need || !aligned(workspace, 16))
         return refuse(std::string(fn) + ": the workspace is missing, too small or not 16-byte aligned");
     a.words = (unsigned long long*)workspace;
-    a.tickets = (unsigned*)(a.words + linrec_words(a));
     return SSLA_OK;
 }
 
@@ -231,9 +239,7 @@ int ssla_hip_linrec_workspace(const SslaHipLinRec* d, size_t* nbytes) try {
     if (!nbytes) return refuse("ssla_hip_linrec_workspace: null argument");
     *nbytes = 0;
     if (const int rc = check_linrec(d, kSizes, "ssla_hip_linrec_workspace")) return rc;
-    const SslaHipLinRecGrad none{};
-    const size_t one = linrec_bytes(linrec_args(d, nullptr)), other = linrec_bytes(linrec_args(d, &none));
-    *nbytes = one > other ? one : other;
+    *nbytes = linrec_need(d);
     return SSLA_OK;
 } catch (const std::exception&) {
     return SSLA_ERR_ARG;
@@ -243,7 +249,7 @@ int ssla_hip_linrec(const SslaHipLinRec* d, void* workspace, size_t workspace_by
     const char* fn = "ssla_hip_linrec";
     if (const int rc = check_linrec(d, kForward, fn)) return rc;
     LinRecArgs a = linrec_args(d, nullptr);
-    if (const int rc = linrec_bind(a, workspace, workspace_bytes, fn)) return rc;
+    if (const int rc = linrec_bind(a, d, workspace, workspace_bytes, fn)) return rc;
     const hipError_t e = linrec_launch(a, d->dtype, (hipStream_t)stream);
     return e == hipSuccess ? SSLA_OK : hip_failed(fn, e);
 } catch (const std::exception&) {
@@ -256,7 +262,7 @@ int ssla_hip_linrec_backward(const SslaHipLinRec* d, const SslaHipLinRecGrad* g,
     if (const int rc = check_linrec(d, kBackward, fn)) return rc;
     if (const int rc = check_linrec_grad(d, g)) return rc;
     LinRecArgs a = linrec_args(d, g);
-    if (const int rc = linrec_bind(a, workspace, workspace_bytes, fn)) return rc;
+    if (const int rc = linrec_bind(a, d, workspace, workspace_bytes, fn)) return rc;
     const hipError_t e = linrec_launch_backward(a, d->dtype, (hipStream_t)stream);
     return e == hipSuccess ? SSLA_OK : hip_failed(fn, e);
 } catch (const std::exception&) {

@@ -154,7 +154,7 @@ class SslaHipLinRec(ctypes.Structure):
         (n, ctypes.c_longlong) for n in ("gate_stride", "v_stride", "q_stride", "out_stride")] + [
         (n, ctypes.c_void_p) for n in ("cu_seqlens", "slots", "state_in", "state_out")] + [
         (n, ctypes.c_longlong) for n in ("state_in_stride", "state_out_stride")] + [
-        ("carries", ctypes.c_void_p)]
+        ("carries", ctypes.c_void_p), ("wait_us", ctypes.c_int)]
 
 
 class SslaHipLinRecGrad(ctypes.Structure):

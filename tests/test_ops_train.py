@@ -143,6 +143,7 @@ def test_grids_that_cannot_be_launched_are_refused():
         g = linrec_grad(**{n + "_stride": 1 << 32 for n in ("dout", "dgate", "dv", "dq", "dstate_in", "dstate_out")})
         assert L.ssla_hip_linrec_backward(at(d), at(g), P, 1 << 62, None) == abi.SSLA_ERR_ARG
         assert b"too many" in L.ssla_hip_last_error()
+    assert L.ssla_hip_linrec(at(linrec(wait_us=1000001)), P, 1 << 40, None) == abi.SSLA_ERR_ARG
     d = linrec(n_seqs=big, n_slots=big, channels=1 << 20, gate_stride=1 << 20, v_stride=1 << 20, q_stride=1 << 20,
                out_stride=1 << 20, state_in_stride=1 << 20, state_out_stride=1 << 20, state_out=P + (4 << 24))
     assert L.ssla_hip_linrec_step(at(d), None) == abi.SSLA_ERR_ARG

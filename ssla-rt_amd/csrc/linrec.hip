@@ -215,6 +215,7 @@ struct Walk {
     }
     __device__ Walk(const LinRecArgs& args, int token) : a(args), t(token) {
         int lo = -1, hi = a.n_seqs + 1;                      // first(lo) <= t < first(hi)
+        #pragma unroll 1
         while (hi - lo > 1) {
             const int mid = lo + (hi - lo) / 2;
             if (first(mid) <= t) lo = mid;
@@ -224,10 +225,12 @@ struct Walk {
     }
     __device__ __forceinline__ void up() {
         ++t;
+        #pragma unroll 1
         while (first(seq + 1) <= t) ++seq;
     }
     __device__ __forceinline__ void down() {
         --t;
+        #pragma unroll 1
         while (seq >= 0 && first(seq) > t) --seq;
     }
 };
@@ -245,14 +248,17 @@ __device__ unsigned long long made_here(const LinRecArgs& a, int place, int chan
     const int tile = BACK ? a.tiles - 1 - place : place, t0 = tile * a.tile, per = a.lanes / 4;
     auto value = [&](const void* p, long long stride, int t) { return (float)((const T*)p)[t * stride + channel]; };
     float tA = 1.0f, tL = 0.0f;
+    #pragma unroll 1
     for (int part = 0; part < 4; ++part) {
         float mA = 1.0f, mL = 0.0f;
+        #pragma unroll 1
         for (int i = part * per; i < part * per + per; ++i) {
             const int y = BACK ? a.lanes - 1 - i : i, t = t0 + y * R;
             float A = 1.0f, x = 0.0f;
             bool cut = false;
             if (!BACK) {
                 Walk at(a, t - 1);
+                #pragma unroll 1
                 for (int r = 0; r < R; ++r) {
                     const int was = at.seq;
                     at.up();
@@ -266,8 +272,10 @@ __device__ unsigned long long made_here(const LinRecArgs& a, int place, int chan
                     A *= f;
                 }
             } else {
+                #pragma unroll 1
                 for (int r = 0; r < R; ++r) A *= gate_of(t + r < a.n_tokens ? value(a.g, a.gt, t + r) : 0.0f).a;
                 Walk at(a, t + R);
+                #pragma unroll 1
                 for (int r = R - 1; r >= 0; --r) {
                     const int was = at.seq;
                     at.down();
@@ -365,7 +373,8 @@ struct Chain {
         publish(open ? tA : kCut, tL);
         if (!open) return 0.0f;
         float state;
-        if (!look_back(word, state, a.patience)) state = on ? alone<T, R, BACK>(a, word, p, channel) : 0.0f;
+        if (__builtin_expect_with_probability(!look_back(word, state, a.patience), 0, 0.999999))
+            state = on ? alone<T, R, BACK>(a, word, p, channel) : 0.0f;
         if (!(tA < 0.0f)) publish(kCut, fmaf(tA, state, tL));
         return state;
     }
@@ -389,8 +398,10 @@ struct Chain {
         };
         int j = p - 1;
         unsigned long long w = map(j);
+        #pragma unroll 1
         while (!(map_a(w) < 0.0f) && j > 0) w = map(--j);    // the first place's is a state
         float h = map_l(w);
+        #pragma unroll 1
         while (++j < p) {
             w = map(j);
             h = map_a(w) < 0.0f ? map_l(w) : fmaf(map_a(w), h, map_l(w));

@@ -34,6 +34,7 @@ struct LinRecArgs {
     int cols, blocks;                     // threads along the channels; workgroups along them
     int lanes, tile, tiles;               // threads along the tokens, their tokens, tiles of all tokens
     int carry;                            // tokens of a tile of the backward pass
+    int brief;                            // a thread a channel, without tiles
     unsigned patience;                    // ticks of 10 ns that a workgroup waits for another
     unsigned long long* words;            // workspace: [block][kBehind + place in the chain][kChannels] maps and states
 };

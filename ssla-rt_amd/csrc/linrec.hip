@@ -301,6 +301,33 @@ __device__ unsigned long long made_here(const LinRecArgs& a, int place, int chan
     return word_of(open ? tA : kCut, tL);
 }
 
+template <int V>
+__device__ __forceinline__ void put(float* to, const float (&x)[V]) {
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    if constexpr (V % 4 == 0) {
+        #pragma unroll
+        for (int i = 0; i < V; i += 4) *(f4*)(to + i) = f4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+    } else {
+        #pragma unroll
+        for (int i = 0; i < V; ++i) to[i] = x[i];
+    }
+}
+template <int V>
+__device__ __forceinline__ void get(float (&x)[V], const float* from) {
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    if constexpr (V % 4 == 0) {
+        #pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const f4 y = *(const f4*)(from + i);
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) x[i + j] = y[j];
+        }
+    } else {
+        #pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = from[i];
+    }
+}
+
 // The chain phase: a lane has a channel of the workgroup's and one of four parts of
 // its threads (of the window, while it looks back); waves have sixteen channels.
 struct Chain {
@@ -494,7 +521,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
         return;
     }
     const int row = a.cols * V + 4;                          // a row of LDS: the workgroup's channels, and four
-    float* sA = (float*)smem;                                // [lanes][row]
+    float* sA = (float*)smem;                                // maps of the threads: A and L
     float* sL = sA + a.lanes * row;
     Place<V, R> p;
     p.first = (int*)(sL + a.lanes * row);
@@ -525,12 +552,13 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
             A[i] *= f[r][i];
         }
     }
+    const int own = p.y * row + p.x * V;
     if (p.on) {
+        float x[V];
         #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            sA[p.y * row + p.x * V + i] = p.starts ? kCut : A[i];
-            sL[p.y * row + p.x * V + i] = h[i];
-        }
+        for (int i = 0; i < V; ++i) x[i] = p.starts ? kCut : A[i];
+        put(sA + own, x);
+        put(sL + own, h);
     }
     opaque(v), opaque(q);
     opaque(p.t), opaque(p.c);
@@ -544,8 +572,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
     chain.spread<false>(a, sA, sL, row, state);
     __syncthreads();
     if (p.n == 0) return;
-    #pragma unroll
-    for (int i = 0; i < V; ++i) h[i] = sL[p.y * row + p.x * V + i];
+    get(h, sL + own);
     if (a.carries && p.t % a.carry == 0)
         store<TAIL>(a.carries + (long long)(p.t / a.carry) * a.channels + p.c, h, p.over);
     int slot = linrec_slot(a, p.in);
@@ -580,7 +607,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
 }
 
 template <class T, int V, int R, bool TAIL>
-__global__ __launch_bounds__(NT, 4) void k_linrec_backward(const LinRecArgs a) {
+__global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(const LinRecArgs a) {
     extern __shared__ __align__(16) char smem[];
     __shared__ Shared sh;
     if (blockIdx.x >= (unsigned)(a.tiles * a.blocks)) {
@@ -616,12 +643,13 @@ __global__ __launch_bounds__(NT, 4) void k_linrec_backward(const LinRecArgs a) {
             A[i] *= f[r][i];
         }
     }
+    const int own = p.y * row + p.x * V;
     if (p.on) {
+        float x[V];
         #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            sA[p.y * row + p.x * V + i] = p.starts ? kCut : A[i];
-            sL[p.y * row + p.x * V + i] = h[i];
-        }
+        for (int i = 0; i < V; ++i) x[i] = p.starts ? kCut : A[i];
+        put(sA + own, x);
+        put(sL + own, h);
     }
     opaque(v), opaque(q), opaque(d);
     __syncthreads();
@@ -637,8 +665,7 @@ __global__ __launch_bounds__(NT, 4) void k_linrec_backward(const LinRecArgs a) {
     float e[R][V];
     T* dq = (T*)a.dq + (long long)p.t * a.dqt + p.c;
     int slot = linrec_slot(a, p.in);
-    #pragma unroll
-    for (int i = 0; i < V; ++i) h[i] = p.on ? sL[p.y * row + p.x * V + i] : 0.0f;
+    get(h, sL + own);                                        // (a thread that is not on has a row, too)
     #pragma unroll
     for (int r = 0; r < R; ++r) {
         if (p.starts >> r & 1) {
@@ -677,11 +704,11 @@ __global__ __launch_bounds__(NT, 4) void k_linrec_backward(const LinRecArgs a) {
         }
     }
     if (p.on) {
+        float x[V];
         #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            sA[p.y * row + p.x * V + i] = p.ends ? kCut : A[i];
-            sL[p.y * row + p.x * V + i] = m[i];
-        }
+        for (int i = 0; i < V; ++i) x[i] = p.ends ? kCut : A[i];
+        put(sA + own, x);
+        put(sL + own, m);
     }
     opaque(p.t), opaque(p.c);
     __syncthreads();
@@ -692,8 +719,7 @@ __global__ __launch_bounds__(NT, 4) void k_linrec_backward(const LinRecArgs a) {
     chain.spread<true>(a, sA, sL, row, state);
     __syncthreads();
     if (p.n == 0) return;
-    #pragma unroll
-    for (int i = 0; i < V; ++i) m[i] = sL[p.y * row + p.x * V + i];
+    get(m, sL + own);
     slot = slot_at(R - 1);
     T* dg = (T*)a.dg + (long long)(p.t + R - 1) * a.dgt + p.c;
     T* dv = (T*)a.dv + (long long)(p.t + R - 1) * a.dvt + p.c;
@@ -721,6 +747,36 @@ __global__ __launch_bounds__(NT, 4) void k_linrec_backward(const LinRecArgs a) {
     }
 }
 
+// Short sequences, a thread a channel, token after token, kAhead of them in flight: what
+// little there is to do is done before the tiles' kernel has its boundaries.
+template <class T>
+__global__ __launch_bounds__(64) void k_linrec_short(const LinRecArgs a) {
+    constexpr int kAhead = 8;
+    const int per = (a.channels + 63) / 64, seq = blockIdx.x / per, c = (blockIdx.x - seq * per) * 64 + threadIdx.x;
+    const int slot = linrec_slot(a, seq);
+    if (slot < 0 || c >= a.channels) return;
+    const int t0 = a.cu ? boundary(a, seq) : seq * a.seq_len, t1 = a.cu ? boundary(a, seq + 1) : t0 + a.seq_len;
+    float h = a.s_in ? a.s_in[slot * a.si + c] : 0.0f;
+    for (int t = t0; t < t1; t += kAhead) {
+        T g[kAhead], v[kAhead], q[kAhead];
+        #pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const long long at = min(t + j, t1 - 1);
+            g[j] = ((const T*)a.g)[at * a.gt + c];
+            v[j] = ((const T*)a.v)[at * a.vt + c];
+            if (a.q) q[j] = ((const T*)a.q)[at * a.qt + c];
+        }
+        #pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (t + j < t1) {
+                if (a.carries && (t + j) % a.carry == 0) a.carries[(long long)((t + j) / a.carry) * a.channels + c] = h;
+                h = fmaf(gate_of((float)g[j]).a, h, (float)v[j]);
+                ((T*)a.out)[(long long)(t + j) * a.ot + c] = (T)(a.q ? (float)q[j] * h : h);
+            }
+    }
+    if (a.s_out) a.s_out[slot * a.so + c] = h;
+}
+
 // Empties the chain: no word is published.
 __global__ __launch_bounds__(NT) void k_linrec_clear(ulonglong2* words, long long n) {
     for (long long i = (long long)blockIdx.x * NT + threadIdx.x; i < n; i += (long long)gridDim.x * NT)
@@ -733,19 +789,12 @@ size_t lds_bytes(const LinRecArgs& a) {
 
 // Channels of a thread: 16 bytes; its tokens.
 template <class T> constexpr int kVec = 16 / sizeof(T);
-#ifndef FR
-#define FR 8
-#endif
-#ifndef BR
-#define BR 4
-#endif
-#ifndef FR2
-#define FR2 4
-#endif
-#ifndef BR2
-#define BR2 2
-#endif
-constexpr int tokens_of(bool wide, bool backward) { return wide ? backward ? BR : FR : backward ? BR2 : FR2; }
+// Tokens of a thread: more are more bytes in flight for the chain phase's instructions, and
+// longer tiles; fewer leave room for more waves.  In us, half as many, so, twice as many: forward
+// 1 x 40001 of 1024 bf16 channels -, 74, 80 (two waves a SIMD for four), 1.25M records of
+// 48 fp32 ones 498, 260, 672 (an earlier form); backward the latter 435, 347, 473, ragged
+// fp16 -, 160, 167.
+constexpr int tokens_of(bool wide, bool backward) { return wide ? backward ? 4 : 8 : backward ? 2 : 4; }
 
 template <class T, bool BACKWARD, int V, bool TAIL>
 const void* kernel() {
@@ -757,6 +806,11 @@ const void* kernel() {
 template <class T, bool BACKWARD>
 hipError_t launch(const LinRecArgs& a, hipStream_t st) {
     LinRecArgs args = a;
+    void* pa[] = {&args};
+    if (!BACKWARD && a.brief) {
+        const long long wgs = (long long)a.n_seqs * ((a.channels + 63) / 64);
+        return hipLaunchKernel((const void*)k_linrec_short<T>, dim3((unsigned)wgs), dim3(64), pa, 0, st);
+    }
     const int nt = (a.cols * a.lanes + 63) / 64 * 64;
     if (a.tiles > 1) {
         long long n = (long long)linrec_words(a) / 2;
@@ -770,7 +824,6 @@ hipError_t launch(const LinRecArgs& a, hipStream_t st) {
     const long long empties = states && (a.cu || !a.n_tokens) ? ((long long)a.n_seqs + nt - 1) / nt : 0;
     const long long wgs = (long long)a.tiles * a.blocks + empties;
     if (!wgs) return hipSuccess;
-    void* pa[] = {&args};
     const void* f = a.vec == 1                ? kernel<T, BACKWARD, 1, false>()
                     : a.channels % a.vec == 0 ? kernel<T, BACKWARD, kVec<T>, false>()
                                               : kernel<T, BACKWARD, kVec<T>, true>();
@@ -795,7 +848,15 @@ void linrec_plan(LinRecArgs& a, int dtype, bool backward) {
     const bool wide = dtype == SSLA_F32;
     cut(a, wide ? 4 : 8, tokens_of(wide, true));
     a.carry = a.tile;
-    if (!backward) cut(a, wide ? 4 : 8, tokens_of(wide, false));
+    if (backward) return;
+    cut(a, wide ? 4 : 8, tokens_of(wide, false));
+    // A thread a channel, without tiles, where no sequence can have more than 32 tokens (us a
+    // call, so and in tiles: 1 x 17 of 96 fp32 channels 6.2 and 8.0, 1 x 32 7.3 and 7.8, 1 x 64
+    // 11.0 and 7.8, 64 x 32 8.0 and 11.1, 64 x 64 12.1 and 11.0) and the card is not filled
+    // (1000 x 8 of 256 bf16 channels 8.5 and 12.9, 1000 x 32 20.2 and 19.8).  It looks at no
+    // rows of no sequence, which carries want zeros in.
+    a.brief = a.n_seqs > 0 && a.n_tokens > 0 && (a.cu ? a.n_tokens : a.seq_len) <= 32 && !(a.cu && a.carries) &&
+              (long long)a.n_seqs * a.channels <= 1 << 18;
 }
 
 hipError_t linrec_launch(const LinRecArgs& a, int dtype, hipStream_t st) {

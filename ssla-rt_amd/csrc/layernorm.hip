@@ -447,7 +447,7 @@ hipError_t launch_backward(const LayerNormArgs& a, hipStream_t st) {
     } else if (a.rows) {
         if (a.dx) e = hipLaunchKernel((const void*)k_ln_backward<T>, dim3(a.wgs), dim3(NT), pa, 0, st);
         if (e == hipSuccess && a.parts)
-            e = hipLaunchKernel((const void*)k_ln_columns<T>, dim3((a.channels + NT - 1) / NT, a.parts), dim3(NT), pa, 0, st);
+            e = hipLaunchKernel((const void*)k_ln_columns<T>, dim3((a.channels - 1) / NT + 1, a.parts), dim3(NT), pa, 0, st);
     }
     if (e == hipSuccess && (a.dw || a.db))
         e = hipLaunchKernel((const void*)k_ln_join<T>, dim3((unsigned)((2ll * a.channels + 15) / 16)), dim3(1024), pa, 0, st);

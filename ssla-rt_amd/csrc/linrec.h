@@ -44,6 +44,7 @@ constexpr int kChannels = 64;             // most of a workgroup
 constexpr int kBehind = 32;               // places before a chain's first one, never published
 
 void linrec_plan(LinRecArgs& a, int dtype, bool backward);
+inline int linrec_threads(const LinRecArgs& a) { return (a.cols * a.lanes + 63) / 64 * 64; }
 // Workspace: 0 where one tile holds all tokens.
 inline size_t linrec_words(const LinRecArgs& a) {
     return a.tiles > 1 ? ((size_t)a.tiles + kBehind) * a.blocks * kChannels : 0;

@@ -752,7 +752,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(
 template <class T>
 __global__ __launch_bounds__(64) void k_linrec_short(const LinRecArgs a) {
     constexpr int kAhead = 8;
-    const int per = (a.channels + 63) / 64, seq = blockIdx.x / per, c = (blockIdx.x - seq * per) * 64 + threadIdx.x;
+    const int per = (a.channels - 1) / 64 + 1, seq = blockIdx.x / per, c = (blockIdx.x - seq * per) * 64 + threadIdx.x;
     const int slot = linrec_slot(a, seq);
     if (slot < 0 || c >= a.channels) return;
     const int t0 = a.cu ? boundary(a, seq) : seq * a.seq_len, t1 = a.cu ? boundary(a, seq + 1) : t0 + a.seq_len;
@@ -790,10 +790,10 @@ size_t lds_bytes(const LinRecArgs& a) {
 // Channels of a thread: 16 bytes; its tokens.
 template <class T> constexpr int kVec = 16 / sizeof(T);
 // Tokens of a thread: more are more bytes in flight for the chain phase's instructions, and
-// longer tiles; fewer leave room for more waves.  In us, half as many, so, twice as many: forward
-// 1 x 40001 of 1024 bf16 channels -, 74, 80 (two waves a SIMD for four), 1.25M records of
-// 48 fp32 ones 498, 260, 672 (an earlier form); backward the latter 435, 347, 473, ragged
-// fp16 -, 160, 167.
+// longer tiles; fewer leave room for more waves.  Kernels' us, half as many, so, twice as many:
+// forward 1.25M records of 48 fp32 channels 291, 240, 338, 1 x 40001 of 1024 bf16 ones 133,
+// 108, - (earlier forms; now 198 and 74; twice as many bf16 80); backward the former 435, 347,
+// 473, ragged fp16 -, 160, 167.
 constexpr int tokens_of(bool wide, bool backward) { return wide ? backward ? 4 : 8 : backward ? 2 : 4; }
 
 template <class T, bool BACKWARD, int V, bool TAIL>
@@ -808,10 +808,10 @@ hipError_t launch(const LinRecArgs& a, hipStream_t st) {
     LinRecArgs args = a;
     void* pa[] = {&args};
     if (!BACKWARD && a.brief) {
-        const long long wgs = (long long)a.n_seqs * ((a.channels + 63) / 64);
+        const long long wgs = (long long)a.n_seqs * ((a.channels - 1) / 64 + 1);
         return hipLaunchKernel((const void*)k_linrec_short<T>, dim3((unsigned)wgs), dim3(64), pa, 0, st);
     }
-    const int nt = (a.cols * a.lanes + 63) / 64 * 64;
+    const int nt = linrec_threads(a);
     if (a.tiles > 1) {
         long long n = (long long)linrec_words(a) / 2;
         void* pc[] = {&args.words, &n};
@@ -853,10 +853,10 @@ void linrec_plan(LinRecArgs& a, int dtype, bool backward) {
     // A thread a channel, without tiles, where no sequence can have more than 32 tokens (us a
     // call, so and in tiles: 1 x 17 of 96 fp32 channels 6.2 and 8.0, 1 x 32 7.3 and 7.8, 1 x 64
     // 11.0 and 7.8, 64 x 32 8.0 and 11.1, 64 x 64 12.1 and 11.0) and the card is not filled
-    // (1000 x 8 of 256 bf16 channels 8.5 and 12.9, 1000 x 32 20.2 and 19.8).  It looks at no
-    // rows of no sequence, which carries want zeros in.
+    // (1000 x 8 of 256 bf16 channels 8.5 and 12.9, 1000 x 32 20.3 and 18.7, 4096 x 32 of 48 fp32
+    // ones 17.2 and 21.6, of a single one 14.6 and 15.0).  It looks at no rows of no sequence, which carries want zeros in.
     a.brief = a.n_seqs > 0 && a.n_tokens > 0 && (a.cu ? a.n_tokens : a.seq_len) <= 32 && !(a.cu && a.carries) &&
-              (long long)a.n_seqs * a.channels <= 1 << 18;
+              (long long)a.n_seqs * ((a.channels - 1) / 64 + 1) <= 1 << 12;
 }
 
 hipError_t linrec_launch(const LinRecArgs& a, int dtype, hipStream_t st) {

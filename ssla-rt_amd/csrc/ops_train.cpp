@@ -71,8 +71,9 @@ int check_linrec(const SslaHipLinRec* d, Call call, const char* fn) {
         return refuse(f + "a pointer is not aligned to its element");
     if (step && d->n_seqs > 0 && (!d->state_in || !d->state_out))
         return refuse(f + "state_in and state_out are needed");
+    if (d->slots && (call == kBackward || (call == kForward && d->carries)))
+        return refuse(f + "there are no gradients by slots");
     if (writes) return check_pools(d, f);
-    if (call == kBackward && d->slots) return refuse(f + "there are no gradients by slots");
     if (d->state_in && (d->state_in_stride < d->channels || d->state_in_stride > kMaxStride))
         return refuse(f + "state strides must be channels .. 2^40");
     return SSLA_OK;
@@ -136,7 +137,7 @@ size_t linrec_need(const SslaHipLinRec* d) {
 // The grid's limit, and the workspace.
 int linrec_bind(LinRecArgs& a, const SslaHipLinRec* d, void* workspace, size_t bytes, const char* fn) {
     if (!launchable(a.tiles, a.blocks, 1, kLinRecThreads) ||
-        !launchable((long long)a.tiles * a.blocks + a.n_seqs / kLinRecThreads + 1, 1, 1, kLinRecThreads))
+        !launchable((long long)a.tiles * a.blocks + a.n_seqs / linrec_threads(a) + 1, 1, 1, kLinRecThreads))
         return refuse(std::string(fn) + ": too many tokens and channels");
     const size_t need = linrec_need(d);
     if (!need) return SSLA_OK;
@@ -202,6 +203,12 @@ LayerNormArgs layer_norm_args(const SslaHipLayerNorm* d, const SslaHipLayerNormG
     }
     layer_norm_plan(a, d->dtype, g != nullptr);
     return a;
+}
+
+// Grids of the backward pass: the rows', and those of the sums over them.
+bool layer_norm_fits(const LayerNormArgs& a) {
+    return launchable(a.wgs, 1, 1, a.threads) && launchable((a.channels - 1) / 256 + 1, a.reps ? 1 : a.parts, 1, 256) &&
+           launchable((2ll * a.channels - 1) / 16 + 1, a.dw || a.db ? 1 : 0, 1, 1024);
 }
 
 size_t layer_norm_bytes(const LayerNormArgs& a) { return (size_t)a.parts * 2 * a.channels * 4; }
@@ -273,7 +280,8 @@ int ssla_hip_linrec_step(const SslaHipLinRec* d, void* stream) try {
     if (const int rc = check_linrec(d, kStep, "ssla_hip_linrec_step")) return rc;
     if (d->n_seqs == 0) return SSLA_OK;
     const LinRecArgs a = linrec_args(d, nullptr);
-    if (!launchable((long long)a.n_seqs * a.channels + kLinRecThreads, 1, 1, 1))
+    // a thread 16 bytes of values, but where there are few
+    if (!launchable((long long)a.n_seqs * ((a.channels - 1) / (d->dtype == SSLA_F32 ? 4 : 8) + 1) + kLinRecThreads, 1, 1, 1))
         return refuse("ssla_hip_linrec_step: too many sequences and channels");
     const hipError_t e = linrec_launch_step(a, d->dtype, (hipStream_t)stream);
     return e == hipSuccess ? SSLA_OK : hip_failed("ssla_hip_linrec_step", e);
@@ -285,7 +293,7 @@ int ssla_hip_layer_norm(const SslaHipLayerNorm* d, void* stream) try {
     if (const int rc = check_layer_norm(d, false, "ssla_hip_layer_norm")) return rc;
     if (!d->rows || !d->channels) return SSLA_OK;
     const LayerNormArgs a = layer_norm_args(d, nullptr);
-    if (!launchable(a.rows, 1, 1, 256)) return refuse("ssla_hip_layer_norm: too many rows");
+    if (!launchable(a.wgs, 1, 1, a.threads)) return refuse("ssla_hip_layer_norm: too many rows");
     const hipError_t e = layer_norm_launch(a, d->dtype, (hipStream_t)stream);
     return e == hipSuccess ? SSLA_OK : hip_failed("ssla_hip_layer_norm", e);
 } catch (const std::exception&) {
@@ -312,7 +320,7 @@ int ssla_hip_layer_norm_backward(const SslaHipLayerNorm* d, const SslaHipLayerNo
     if (const int rc = check_layer_norm_grad(d, g, fn)) return rc;
     if (!d->channels) return SSLA_OK;
     LayerNormArgs a = layer_norm_args(d, g);
-    if (!launchable(a.rows, 1, 1, 256)) return refuse(std::string(fn) + ": too many rows");
+    if (!layer_norm_fits(a)) return refuse(std::string(fn) + ": too many rows and channels");
     const size_t need = layer_norm_bytes(a);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return refuse(std::string(fn) + ": the workspace is missing, too small or not 16-byte aligned");

@@ -54,7 +54,8 @@ void capturable(const char* fn, const char* name, const at::Tensor* t) {
         refuse(fn, std::string(name) + " has a graph that was recorded on the default stream and still lives: "
                                        "drop it before the capture");
 }
-bool capturing() {
+bool capturing(at::Device dev) {
+    const c10::DeviceGuard guard(dev);
     return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
 }
 
@@ -256,7 +257,7 @@ std::vector<at::Tensor> linear_recurrence(const Args& a) {
         if (given || to || slots)
             refuse(fn, "out, state_out and slots have no gradients: call under torch.no_grad(), or with return_state");
         if (in && in->size(0) != d.n_seqs) refuse(fn, "state_in must have one row for every sequence");
-        if (capturing()) {
+        if (capturing(dev)) {
             capturable(fn, "gate", &gate);
             capturable(fn, "v", &v);
             capturable(fn, "q", q);
@@ -423,7 +424,7 @@ at::Tensor layer_norm(const Args& a) {
     SslaHipLayerNorm d = describe_norm(fn, x, res, w, b, eps);
     if (at::GradMode::is_enabled() && (wanted(&x) || wanted(res) || wanted(w) || wanted(b))) {
         if (given) refuse(fn, "out has no gradient: call under torch.no_grad()");
-        if (capturing()) {
+        if (capturing(x.device())) {
             capturable(fn, "x", &x);
             capturable(fn, "residual", res);
             capturable(fn, "weight", w);

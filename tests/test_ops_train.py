@@ -213,3 +213,12 @@ def test_python_refuses_tensors_off_the_gpu_and_what_is_no_argument():
               lambda: ops.layer_norm(q, eps="1"), lambda: ops._ops.layer_norm(q)):
         with pytest.raises(ValueError):
             f()
+
+
+def test_carries_and_sums_that_cannot_be_are_refused():
+    L, big = lib.load(), 0x7fff0000
+    assert L.ssla_hip_linrec(at(linrec(slots=P)), None, 0, None) == abi.SSLA_ERR_ARG
+    assert b"slots" in L.ssla_hip_last_error()
+    wide = norm(rows=1, channels=big, weight=None, bias=None)
+    assert L.ssla_hip_layer_norm_backward(at(wide), at(norm_grad()), P, 1 << 62, None) == abi.SSLA_ERR_ARG
+    assert b"too many" in L.ssla_hip_last_error()

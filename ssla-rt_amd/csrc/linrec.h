@@ -32,6 +32,7 @@ struct LinRecArgs {
     // how the call is cut (linrec_plan)
     int vec;                              // channels of a thread
     int cols, blocks;                     // threads along the channels; workgroups along them
+    unsigned per_col;                     // 2^16 / cols, rounded up: exact for a workgroup's threads
     int lanes, tile, tiles;               // threads along the tokens, their tokens, tiles of all tokens
     int carry;                            // tokens of a tile of the backward pass
     int brief;                            // a thread a channel, without tiles

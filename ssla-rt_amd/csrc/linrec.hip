@@ -57,12 +57,17 @@ constexpr int kMaxTile = NT * 8;          // one thread along the channels, eigh
 // the tile too), and which.
 struct Shared {
     unsigned mask[kMaxTile / 32 + 1];
+    int some;                             // any begins
+    int counts[2][NT / 64];
     __device__ __forceinline__ bool begins(int i) const { return mask[i >> 5] >> (i & 31) & 1; }
 };
 
 // First token of sequence i (the last one's end for i = n_seqs), of those in a.cu.
+__device__ __forceinline__ int boundary(const LinRecArgs& a, long long i, int value) {
+    return i <= a.n_seqs ? (int)min((long long)max(value, 0), a.n_tokens) : 0x7fffffff;
+}
 __device__ __forceinline__ int boundary(const LinRecArgs& a, long long i) {
-    return i <= a.n_seqs ? (int)min((long long)max(a.cu[i], 0), a.n_tokens) : 0x7fffffff;
+    return i <= a.n_seqs ? boundary(a, i, a.cu[i]) : 0x7fffffff;
 }
 
 // Where a thread works.
@@ -77,6 +82,7 @@ struct Place {
     int in;                               // sequence that the token before the thread's belongs to
     unsigned starts, ends;                // of the thread's tokens: bit r where a sequence begins, ends
     bool begun;                           // the tile's first token belongs to a sequence that began before it
+    bool plain;                           // the tile is full, and no sequence begins or ends in it
     int at, next;                         // a boundary of the thread's, and the one behind it
 
     __device__ __forceinline__ void find(const LinRecArgs& a, Shared& sh, bool backward) {
@@ -85,17 +91,19 @@ struct Place {
         // on one, as rows that are no whole lines share lines between them.
         const int eight = blockIdx.x / (8 * a.blocks), k = blockIdx.x - eight * 8 * a.blocks,
                   wide = min(8, a.tiles - 8 * eight);
-        cb = k / wide;
+        cb = wide == 8 ? k >> 3 : k / wide;
         place = 8 * eight + k - cb * wide;
         tile = backward ? a.tiles - 1 - place : place;
-        // one of nt boundaries spread over all
+        // one of nt boundaries spread over all; looked at in mark, as waiting for it here would
+        // put off the tile's loads (ragged fp16, kernels' us: forward 87 -> 83, backward 155 -> 146)
         if (a.cu) {
             const int step = a.n_seqs / nt + 1;
-            at = boundary(a, (long long)tid * step);
-            if (step == 1) next = boundary(a, tid + 1);
+            at = a.cu[min((long long)tid * step, (long long)a.n_seqs)];
+            next = a.cu[min(tid + 1, a.n_seqs)];
         }
         for (int i = tid; i <= a.tile / 32; i += nt) sh.mask[i] = 0;
-        y = tid / a.cols;
+        if (tid == 0) sh.some = 0;
+        y = (int)((unsigned)tid * a.per_col >> 16);          // tid / a.cols
         x = tid - y * a.cols;
         const int p = cb * a.cols + x;
         on = y < a.lanes && p * V < a.channels;
@@ -111,6 +119,19 @@ struct Place {
         const int i = token - t0;
         first[i] = seq;
         atomicOr(sh.mask + (i >> 5), 1u << (i & 31));
+        sh.some = 1;
+    }
+    // Threads of which x holds, and a barrier.  The library's asks memory for the workgroup's
+    // size, and so waits for all that is on its way.
+    __device__ __forceinline__ static int count(bool x, Shared& sh, int& turn) {
+        int* const counts = sh.counts[turn];
+        const unsigned long long wave = __ballot(x);
+        if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = __popcll(wave);
+        __syncthreads();
+        int n = 0;
+        for (int i = 0; i < (int)blockDim.x >> 6; ++i) n += counts[i];
+        turn ^= 1;
+        return __builtin_amdgcn_readfirstlane(n);
     }
     // Marks the tokens at which sequences begin (where several do, all but the last are
     // empty), and finds the thread's.
@@ -120,8 +141,12 @@ struct Place {
         int before;                                           // sequence of the token before the tile
         if (a.cu) {
             // the first boundary at t0 or behind it is in [lo, hi]
-            int step = a.n_seqs / nt + 1, k = __syncthreads_count(at < t0), lo = k, hi = k;
+            int step = a.n_seqs / nt + 1;
+            opaque(at), opaque(next);
+            at = boundary(a, (long long)tid * step, at);
+            int turn = 0, k = count(at < t0, sh, turn), lo = k, hi = k;
             if (step == 1) {
+                next = boundary(a, tid + 1, next);
                 if (at >= t0 && at <= t1 && next != at) set(sh, at, tid);
             } else {
                 lo = k ? (k - 1) * step + 1 : 0;
@@ -129,7 +154,7 @@ struct Place {
                 while (hi > lo) {
                     step = (hi - lo + nt - 1) / nt;
                     const long long i = lo + (long long)tid * step;
-                    k = __syncthreads_count(i < hi && boundary(a, i) < t0);
+                    k = count(i < hi && boundary(a, i) < t0, sh, turn);
                     const int from = lo;
                     lo = step == 1 ? from + k : k ? from + (k - 1) * step + 1 : from;
                     hi = step == 1 ? lo : k ? (int)min((long long)hi, from + (long long)k * step) : from;
@@ -148,6 +173,13 @@ struct Place {
             for (long long i = s + tid; i * len <= t1; i += nt) set(sh, (int)(i * len), (int)i);
         }
         __syncthreads();
+        plain = !__builtin_amdgcn_readfirstlane(sh.some) && (long long)t0 + a.tile < a.n_tokens;
+        if (plain) {
+            in = __builtin_amdgcn_readfirstlane(before);
+            begun = in >= 0 && in < a.n_seqs;
+            starts = ends = 0;
+            return;
+        }
         const int i = y * R;
         starts = sh.mask[i >> 5] >> (i & 31) & ((1u << n) - 1);
         ends = n == 0 ? 0 : starts >> 1 | (n < R || sh.begins(i + R) || t + R >= a.n_tokens ? 1u << (n - 1) : 0);
@@ -160,8 +192,13 @@ struct Place {
 };
 
 template <class T, int V, int R>
+__device__ __forceinline__ void opaque(Piece<T, V> (&x)[R]) {
+    #pragma unroll
+    for (int r = 0; r < R; ++r) x[r].opaque();
+}
+template <class T, int V, int R>
 __device__ __forceinline__ void load(Piece<T, V> (&x)[R], const void* base, long long stride, const Place<V, R>& p,
-                                     bool whole) {
+                                     bool whole, long long tokens) {
     const T* from = (const T*)base + (long long)p.t * stride + p.c;
     if (whole) {
         #pragma unroll
@@ -169,18 +206,19 @@ __device__ __forceinline__ void load(Piece<T, V> (&x)[R], const void* base, long
             x[r].load(from);
             from += stride;
         }
-    } else {
+    } else {                                                 // as many loads: nothing waits for them here
         #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            x[r].zero();
-            if (r < p.n) x[r].load(from + r * stride);
-        }
+        for (int r = 0; r < R; ++r)
+            x[r].load((const T*)base + min((long long)p.t + r, tokens - 1) * stride + p.c);
     }
 }
+// Tokens behind the last one are read as that one; here they are zeros.
 template <class T, int V, int R>
-__device__ __forceinline__ void opaque(Piece<T, V> (&x)[R]) {
+__device__ __forceinline__ void without(Piece<T, V> (&x)[R], const Place<V, R>& p, bool whole) {
+    if (whole) return;
     #pragma unroll
-    for (int r = 0; r < R; ++r) x[r].opaque();
+    for (int r = 0; r < R; ++r)
+        if (r >= p.n) x[r].zero();
 }
 // A piece; with TAIL without the channels that another thread has too.
 template <bool TAIL, class T, int V>
@@ -301,31 +339,25 @@ __device__ unsigned long long made_here(const LinRecArgs& a, int place, int chan
     return word_of(open ? tA : kCut, tL);
 }
 
+// Maps of a thread's channels in LDS, {A, L} each; the states that take L's place.
+struct alignas(8) Map {
+    float A, L;
+};
 template <int V>
-__device__ __forceinline__ void put(float* to, const float (&x)[V]) {
+__device__ __forceinline__ void put(Map* to, const float (&A)[V], const float (&L)[V]) {
     typedef float f4 __attribute__((ext_vector_type(4)));
-    if constexpr (V % 4 == 0) {
+    if constexpr (V % 2 == 0) {
         #pragma unroll
-        for (int i = 0; i < V; i += 4) *(f4*)(to + i) = f4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+        for (int i = 0; i < V; i += 2) *(f4*)(to + i) = f4{A[i], L[i], A[i + 1], L[i + 1]};
     } else {
         #pragma unroll
-        for (int i = 0; i < V; ++i) to[i] = x[i];
+        for (int i = 0; i < V; ++i) to[i] = Map{A[i], L[i]};
     }
 }
 template <int V>
-__device__ __forceinline__ void get(float (&x)[V], const float* from) {
-    typedef float f4 __attribute__((ext_vector_type(4)));
-    if constexpr (V % 4 == 0) {
-        #pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            const f4 y = *(const f4*)(from + i);
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) x[i + j] = y[j];
-        }
-    } else {
-        #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = from[i];
-    }
+__device__ __forceinline__ void get(float (&x)[V], const Map* from) {
+    #pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = from[i].L;
 }
 
 // The chain phase: a lane has a channel of the workgroup's and one of four parts of
@@ -338,55 +370,69 @@ struct Chain {
 
     __device__ __forceinline__ static float from(float x, int lane, int part) { return __shfl(x, (lane & 15) + 16 * part); }
 
-    // Folds the maps in LDS, first to last or (BACK) last to first.
+    // Folds the maps in LDS, first to last or (BACK) last to first; cuts: there may be some
+    // that are cut.  Without, two instructions a map for seven (of a wave's 1400 backward some
+    // 300 with LDS in pairs; 1.25M records of 48 fp32 channels: 344 -> 328 us).
     template <bool BACK>
-    __device__ __forceinline__ void fold(const LinRecArgs& a, const float* sA, const float* sL, int row, int piece0, int v) {
+    __device__ __forceinline__ void fold(const LinRecArgs& a, const Map* maps, int row, int piece0, int v, bool cuts) {
         lane = threadIdx.x & 63;
         ch = (threadIdx.x >> 6) * 16 + (lane & 15);
         part = lane >> 4;
         on = ch < a.cols * v && (piece0 + ch / v) * v < a.channels;
-        float mA = 1.0f, mL = 0.0f;
-        const int per = a.lanes / 4;
-        if (on)
-            for (int y0 = 0; y0 < per; y0 += 4) {
-                float x[4], l[4];
-                #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = part * per + y0 + j, y = BACK ? a.lanes - 1 - i : i;
-                    x[j] = sA[y * row + ch], l[j] = sL[y * row + ch];
-                }
-                #pragma unroll
-                for (int j = 0; j < 4; ++j) join(mA, mL, x[j], l[j]);
-            }
-        tA = 1.0f, tL = 0.0f;
+        A[0] = tA = 1.0f, L[0] = tL = 0.0f;
+        const Map* m = maps + (BACK ? a.lanes - 1 - part * (a.lanes / 4) : part * (a.lanes / 4)) * row + ch;
+        if (on) {
+            if (cuts) folded<true>(a, m, BACK ? -row : row);
+            else folded<false>(a, m, BACK ? -row : row);
+        }
+        const float mA = A[0], mL = L[0];
         #pragma unroll
         for (int g = 0; g < 4; ++g) {
             A[g] = from(mA, lane, g), L[g] = from(mL, lane, g);
             join(tA, tL, A[g], L[g]);
         }
     }
-    // Puts the states before the threads, from that before the tile, into sL's place.
+    template <bool CUTS>
+    __device__ __forceinline__ void folded(const LinRecArgs& a, const Map* m, int step) {
+        float mA = 1.0f, mL = 0.0f;
+        #pragma unroll 1
+        for (int y = 0; y < a.lanes; y += 16) {
+            Map x[4];
+            #pragma unroll
+            for (int j = 0; j < 4; ++j, m += step) x[j] = *m;
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (CUTS) join(mA, mL, x[j].A, x[j].L);
+                else mL = fmaf(x[j].A, mL, x[j].L), mA *= x[j].A;
+            }
+        }
+        A[0] = mA, L[0] = mL;
+    }
+    // Puts the states before the threads, from that before the tile, into their maps' L.
     template <bool BACK>
-    __device__ __forceinline__ void spread(const LinRecArgs& a, const float* sA, float* sL, int row, float state) {
-        const int per = a.lanes / 4;
+    __device__ __forceinline__ void spread(const LinRecArgs& a, Map* maps, int row, float state, bool cuts) {
         #pragma unroll
         for (int g = 0; g < 3; ++g)
             if (g < part) state = A[g] < 0.0f ? L[g] : fmaf(A[g], state, L[g]);
-        if (on)
-            for (int y0 = 0; y0 < per; y0 += 4) {
-                float x[4], l[4];
-                #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = part * per + y0 + j, y = BACK ? a.lanes - 1 - i : i;
-                    x[j] = sA[y * row + ch], l[j] = sL[y * row + ch];
-                }
-                #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = part * per + y0 + j, y = BACK ? a.lanes - 1 - i : i;
-                    sL[y * row + ch] = state;
-                    state = x[j] < 0.0f ? l[j] : fmaf(x[j], state, l[j]);
-                }
+        Map* m = maps + (BACK ? a.lanes - 1 - part * (a.lanes / 4) : part * (a.lanes / 4)) * row + ch;
+        if (!on) return;
+        if (cuts) spreading<true>(a, m, BACK ? -row : row, state);
+        else spreading<false>(a, m, BACK ? -row : row, state);
+    }
+    template <bool CUTS>
+    __device__ __forceinline__ void spreading(const LinRecArgs& a, Map* m, int step, float state) {
+        #pragma unroll 1
+        for (int y = 0; y < a.lanes; y += 16) {
+            Map x[4];
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = m[j * step];
+            #pragma unroll
+            for (int j = 0; j < 4; ++j, m += step) {
+                m->L = state;
+                const float h = fmaf(x[j].A, state, x[j].L);
+                state = CUTS && x[j].A < 0.0f ? x[j].L : h;
             }
+        }
     }
     // The state before place p of the chain, after publishing the tile's map; `open`: a
     // sequence goes on from the place before into this one.  `channel`: this one's.
@@ -520,17 +566,16 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
         empty_sequences(a, blockIdx.x - a.tiles * a.blocks, a.s_in, a.si, a.s_out, a.so);
         return;
     }
-    const int row = a.cols * V + 4;                          // a row of LDS: the workgroup's channels, and four
-    float* sA = (float*)smem;                                // maps of the threads: A and L
-    float* sL = sA + a.lanes * row;
+    const int row = a.cols * V + 2;                          // a row of LDS: the workgroup's channels, and two
+    Map* maps = (Map*)smem;                                  // of the threads
     Place<V, R> p;
-    p.first = (int*)(sL + a.lanes * row);
+    p.first = (int*)(maps + a.lanes * row);
     p.find(a, sh, false);
     const bool whole = p.t0 + a.tile <= a.n_tokens;
     Piece<T, V> g[R], v[R], q[R];
-    load(g, a.g, a.gt, p, whole);
-    load(v, a.v, a.vt, p, whole);
-    if (a.q) load(q, a.q, a.qt, p, whole);
+    load(g, a.g, a.gt, p, whole, a.n_tokens);
+    load(v, a.v, a.vt, p, whole, a.n_tokens);
+    if (a.q) load(q, a.q, a.qt, p, whole, a.n_tokens);
     p.mark(a, sh);
 
     // The thread's map.  The last state that comes in is kept: its sequence may end
@@ -545,6 +590,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
             #pragma unroll
             for (int i = 0; i < V; ++i) h[i] = last[i];
         }
+        g[r].here(), v[r].here();
         #pragma unroll
         for (int i = 0; i < V; ++i) {
             f[r][i] = gate_of(g[r].at(i)).a;
@@ -552,13 +598,12 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
             A[i] *= f[r][i];
         }
     }
-    const int own = p.y * row + p.x * V;
+    Map* const own = maps + p.y * row + p.x * V;
     if (p.on) {
         float x[V];
         #pragma unroll
         for (int i = 0; i < V; ++i) x[i] = p.starts ? kCut : A[i];
-        put(sA + own, x);
-        put(sL + own, h);
+        put(own, x, h);
     }
     opaque(v), opaque(q);
     opaque(p.t), opaque(p.c);
@@ -566,13 +611,13 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
 
     // the tile's map, the state before it, and those before its threads
     Chain chain;
-    chain.fold<false>(a, sA, sL, row, p.cb * a.cols, V);
+    chain.fold<false>(a, maps, row, p.cb * a.cols, V, !p.plain);
     const int channel = min((p.cb * a.cols + chain.ch / V) * V, a.channels - V) + chain.ch % V;
     const float state = a.tiles > 1 ? chain.before<T, R, false>(a, p.cb, p.place, p.begun, channel) : 0.0f;
-    chain.spread<false>(a, sA, sL, row, state);
+    chain.spread<false>(a, maps, row, state, !p.plain);
     __syncthreads();
     if (p.n == 0) return;
-    get(h, sL + own);
+    get(h, own);
     if (a.carries && p.t % a.carry == 0)
         store<TAIL>(a.carries + (long long)(p.t / a.carry) * a.channels + p.c, h, p.over);
     int slot = linrec_slot(a, p.in);
@@ -597,7 +642,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
         if (slot >= 0 && r < p.n) {
             store<TAIL>(out, o, p.over);
             if (a.s_out && (p.ends >> r & 1)) store<TAIL>(a.s_out + slot * a.so + p.c, h, p.over);
-        } else if (a.carries && r < p.n) {                   // of no sequence: zeros
+        } else if (a.carries && r < p.n) {        // of no sequence: zeros
             Piece<T, V> none;
             none.zero();
             store<TAIL>(out, none, p.over);
@@ -614,19 +659,23 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(
         empty_sequences(a, blockIdx.x - a.tiles * a.blocks, a.ds_out, a.dso, a.ds_in, a.dsi);
         return;
     }
-    const int row = a.cols * V + 4;
-    float* sA = (float*)smem;
-    float* sL = sA + a.lanes * row;
+    const int row = a.cols * V + 2;
+    Map* maps = (Map*)smem;
     Place<V, R> p;
-    p.first = (int*)(sL + a.lanes * row);
+    p.first = (int*)(maps + a.lanes * row);
     p.find(a, sh, true);
     const bool whole = p.t0 + a.tile <= a.n_tokens;
     Piece<T, V> g[R], v[R], q[R], d[R];
-    load(g, a.g, a.gt, p, whole);
-    load(v, a.v, a.vt, p, whole);
-    if (a.q) load(q, a.q, a.qt, p, whole);
-    if (a.dout) load(d, a.dout, a.dot, p, whole);
+    load(g, a.g, a.gt, p, whole, a.n_tokens);
+    load(v, a.v, a.vt, p, whole, a.n_tokens);
+    if (a.q) load(q, a.q, a.qt, p, whole, a.n_tokens);
+    if (a.dout) load(d, a.dout, a.dot, p, whole, a.n_tokens);
+    // the state before the tile, of the channel that this lane has in the chain
+    const int ch = (threadIdx.x >> 6) * 16 + (threadIdx.x & 15), col = (p.cb * a.cols + ch / V) * V,
+              at = min(col, a.channels - V) + ch % V;
+    const float carried = a.tiles > 1 ? a.carries[(long long)p.tile * a.channels + at] : 0.0f;
     p.mark(a, sh);
+    without(g, p, whole);                                    // (messages come from behind them)
 
     // states, as the forward pass had them; w: the gates' slopes
     float f[R][V], w[R][V], A[V], h[V];
@@ -635,6 +684,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(
     #pragma unroll
     for (int r = 0; r < R; ++r) {
         if (p.starts >> r & 1) state_of(h, a.s_in, a.si, linrec_slot(a, p.first[p.y * R + r]), p.c);
+        g[r].here(), v[r].here();
         #pragma unroll
         for (int i = 0; i < V; ++i) {
             const Gate gate = gate_of(g[r].at(i));
@@ -643,21 +693,18 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(
             A[i] *= f[r][i];
         }
     }
-    const int own = p.y * row + p.x * V;
+    Map* const own = maps + p.y * row + p.x * V;
     if (p.on) {
         float x[V];
         #pragma unroll
         for (int i = 0; i < V; ++i) x[i] = p.starts ? kCut : A[i];
-        put(sA + own, x);
-        put(sL + own, h);
+        put(own, x, h);
     }
     opaque(v), opaque(q), opaque(d);
     __syncthreads();
     Chain chain;
-    chain.fold<false>(a, sA, sL, row, p.cb * a.cols, V);
-    const int col = (p.cb * a.cols + chain.ch / V) * V, at = min(col, a.channels - V) + chain.ch % V;
-    chain.spread<false>(a, sA, sL, row,
-                        p.begun && a.tiles > 1 && chain.on ? a.carries[(long long)p.tile * a.channels + at] : 0.0f);
+    chain.fold<false>(a, maps, row, p.cb * a.cols, V, !p.plain);
+    chain.spread<false>(a, maps, row, p.begun ? carried : 0.0f, !p.plain);
     __syncthreads();
     // Once more, from the state before the thread: dq is done here; what is left of a
     // token is its gate, its slope times the state before it, and what it adds to its
@@ -665,7 +712,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(
     float e[R][V];
     T* dq = (T*)a.dq + (long long)p.t * a.dqt + p.c;
     int slot = linrec_slot(a, p.in);
-    get(h, sL + own);                                        // (a thread that is not on has a row, too)
+    get(h, own);                                             // (a thread that is not on has a row, too)
     #pragma unroll
     for (int r = 0; r < R; ++r) {
         if (p.starts >> r & 1) {
@@ -707,19 +754,18 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(
         float x[V];
         #pragma unroll
         for (int i = 0; i < V; ++i) x[i] = p.ends ? kCut : A[i];
-        put(sA + own, x);
-        put(sL + own, m);
+        put(own, x, m);
     }
     opaque(p.t), opaque(p.c);
     __syncthreads();
-    chain.fold<true>(a, sA, sL, row, p.cb * a.cols, V);
+    chain.fold<true>(a, maps, row, p.cb * a.cols, V, !p.plain);
     // a sequence that goes on behind the tile
     const bool open = p.place > 0 && !sh.begins(a.tile);
     const float state = a.tiles > 1 ? chain.before<T, R, true>(a, p.cb, p.place, open, at) : 0.0f;
-    chain.spread<true>(a, sA, sL, row, state);
+    chain.spread<true>(a, maps, row, state, !p.plain);
     __syncthreads();
     if (p.n == 0) return;
-    get(m, sL + own);
+    get(m, own);
     slot = slot_at(R - 1);
     T* dg = (T*)a.dg + (long long)(p.t + R - 1) * a.dgt + p.c;
     T* dv = (T*)a.dv + (long long)(p.t + R - 1) * a.dvt + p.c;
@@ -741,7 +787,8 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec_backward(
             }
             if (a.dg) store<TAIL>(dg, z, p.over);
             if (a.dv) store<TAIL>(dv, dh, p.over);
-            if (a.ds_in && (p.starts >> r & 1) && !none) store<TAIL>(a.ds_in + slot * a.dsi + p.c, m, p.over);
+            if (a.ds_in && (p.starts >> r & 1) && !none)
+                store<TAIL>(a.ds_in + slot * a.dsi + p.c, m, p.over);
         }
         dg -= a.dgt, dv -= a.dvt;
     }
@@ -784,7 +831,7 @@ __global__ __launch_bounds__(NT) void k_linrec_clear(ulonglong2* words, long lon
 }
 
 size_t lds_bytes(const LinRecArgs& a) {
-    return (size_t)a.lanes * (a.cols * a.vec + 4) * 8 + ((size_t)a.tile + 1) * 4;
+    return (size_t)a.lanes * (a.cols * a.vec + 2) * 8 + ((size_t)a.tile + 1) * 4;
 }
 
 // Channels of a thread: 16 bytes; its tokens.
@@ -836,6 +883,7 @@ void cut(LinRecArgs& a, int vec, int tokens) {
     const int pieces = (a.channels - 1) / a.vec + 1, most = kChannels / vec;
     a.blocks = (pieces + most - 1) / most;
     a.cols = (pieces - 1) / a.blocks + 1;
+    a.per_col = 65536 / a.cols + 1;
     a.lanes = 16;
     while (2 * a.lanes * a.cols <= kLinRecThreads) a.lanes *= 2;
     a.tile = a.lanes * tokens;
@@ -854,7 +902,8 @@ void linrec_plan(LinRecArgs& a, int dtype, bool backward) {
     // call, so and in tiles: 1 x 17 of 96 fp32 channels 6.2 and 8.0, 1 x 32 7.3 and 7.8, 1 x 64
     // 11.0 and 7.8, 64 x 32 8.0 and 11.1, 64 x 64 12.1 and 11.0) and the card is not filled
     // (1000 x 8 of 256 bf16 channels 8.5 and 12.9, 1000 x 32 20.3 and 18.7, 4096 x 32 of 48 fp32
-    // ones 17.2 and 21.6, of a single one 14.6 and 15.0).  It looks at no rows of no sequence, which carries want zeros in.
+    // ones 17.2 and 21.6, of a single one 14.6 and 15.0).  It looks at no rows of no sequence,
+    // which carries want zeros in.
     a.brief = a.n_seqs > 0 && a.n_tokens > 0 && (a.cu ? a.n_tokens : a.seq_len) <= 32 && !(a.cu && a.carries) &&
               (long long)a.n_seqs * ((a.channels - 1) / 64 + 1) <= 1 << 12;
 }

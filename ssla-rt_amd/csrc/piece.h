@@ -57,6 +57,13 @@ struct Piece {
             for (int i = 0; i < kWords; ++i) asm("" : "+v"(w[i]));
         }
     }
+    // And here none of it has begun yet, behind a branch either.
+    __device__ __forceinline__ void here() {
+        if constexpr (kHalves) {
+            #pragma unroll
+            for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
+        }
+    }
 };
 
 }  // namespace ssla

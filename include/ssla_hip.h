@@ -574,8 +574,8 @@ int ssla_hip_ops_layout(long long* out, int cap);
  * of a call must not have the same slot.  out must not overlap an input.
  *
  * `carries` (NULL: not kept) takes what ssla_hip_linrec_backward needs besides
- * the inputs: states at some of the tokens, ssla_hip_linrec_carries bytes.  With
- * it, rows of out that belong to no sequence get zeros (a loss over all rows
+ * the inputs: states at some of the tokens, ssla_hip_linrec_carries bytes (slots
+ * must be NULL then).  With it, rows of out that belong to no sequence get zeros (a loss over all rows
  * stays finite). */
 typedef struct SslaHipLinRec {
     int dtype;                 /* of gate, v, q and out */
@@ -631,9 +631,10 @@ int ssla_hip_linrec_step(const SslaHipLinRec* d, void* stream);
  *     out = (s - mean) / sqrt(var + eps) * weight_c + bias_c
  * Element (row, c) of x lies at row * x_stride + c (elements, >= 0), of residual
  * and out likewise.  weight and bias (NULL: 1 and 0) are of weight_dtype, which
- * is dtype or SSLA_F32.  x + residual is an fp32 sum, mean and variance are 64
- * bits wide, the mean is subtracted to 48 bits, out is rounded once.  out may be
- * x or residual itself, else it must not overlap an input.  `stats` (NULL: not
+ * is dtype or SSLA_F32.  x + residual is an fp32 sum, the mean is summed in 64
+ * bits and subtracted to 48, squared differences are summed in 64 bits (fp32) or
+ * 32 (16-bit types, and 64 where that is not finite), out is rounded once.  out
+ * may be x or residual itself, else it must not overlap an input.  `stats` (NULL: not
  * kept) takes three floats a row for the backward pass. */
 typedef struct SslaHipLayerNorm {
     int dtype, weight_dtype;

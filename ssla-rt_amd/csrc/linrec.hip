@@ -28,6 +28,13 @@
 // Backward, the same from the last token to the first: the message m_t = a_{t+1}
 // dh_{t+1} goes through maps, cut where a sequence ends.  States come from those
 // that the forward pass left before each tile (carries).
+//
+// Kernels measured (us; in brackets what moving the bytes once takes at a copy's rate): 1 x 40001
+// of 1024 bf16 channels 73.5 (64); 1 x 8192 of 2048, forward 37.5 (26), backward 57 (46); 1.25M
+// records of 48 fp32 ones in 19200 sequences 200 (187) and 322 (327); 40504 tokens of 1001 fp16 ones
+// in 48, without q, 84 (47) and 150 (79).  fp32 is bound by memory.  With 16 bits a value the
+// rest is a workgroup's own time, of which its waves wait for half: the chain (9 us of 74 without
+// it in the first), barriers, LDS; four waves a SIMD do not fill that in.
 #include "linrec.h"
 #include "piece.h"
 
@@ -558,6 +565,8 @@ __device__ void empty_sequences(const LinRecArgs& a, int b, const float* from, l
                 to[which[i] * ts + c] = from ? from[which[i] * fs + c] : 0.0f;
 }
 
+// Four waves a SIMD with 16-bit values, whose words take half the registers; three with fp32 ones,
+// which four would spill.
 template <class T, int V, int R, bool TAIL>
 __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const LinRecArgs a) {
     extern __shared__ __align__(16) char smem[];

@@ -33,8 +33,8 @@
 // of 1024 bf16 channels 73.5 (64); 1 x 8192 of 2048, forward 37.5 (26), backward 57 (46); 1.25M
 // records of 48 fp32 ones in 19200 sequences 200 (187) and 322 (327); 40504 tokens of 1001 fp16 ones
 // in 48, without q, 84 (47) and 150 (79).  fp32 is bound by memory.  With 16 bits a value the
-// rest is a workgroup's own time, of which its waves wait for half: the chain (9 us of 74 without
-// it in the first), barriers, LDS; four waves a SIMD do not fill that in.
+// rest is a workgroup's own time, of which its waves wait for half: the look along the chain (8 us
+// of 74 in the first), barriers, LDS; four waves a SIMD do not fill that in.
 #include "linrec.h"
 #include "piece.h"
 

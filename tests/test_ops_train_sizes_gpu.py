@@ -150,3 +150,55 @@ def test_two_calls_at_once():
     torch.cuda.synchronize()
     for g in got:
         assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+@pytest.mark.parametrize("dtype,c", [("f32", 48), ("bf16", 96), ("f16", 70), ("f32", 3)])
+def test_sequences_that_end_where_tiles_do_and_stretches_of_none(dtype, c):
+    """Boundaries at powers of two, which tiles end at; before and behind the sequences
+    longer stretches of tokens that belong to none, with NaN in all they have."""
+    from ssla_hip import ops
+    t = R.TYPES[dtype]
+    bounds = [(4096, 4608), (4608, 4672), (4672, 6784)]
+    cu = torch.tensor([4096, 4608, 4672, 6784], dtype=torch.int32, device=DEV)
+    T = 6784 + 4096
+    gate, v, q, dout = (normal(40 + i, T, c).to(t) for i in range(4))
+    for x in (gate, v, q):
+        x[:4096] = float("nan")
+        x[6784:] = float("nan")
+    s, dlast = normal(44, 3, c), normal(45, 3, c)
+    val, tol = R.recurrence(gate, v, q, bounds, s, dout, dlast)
+    mine, rest = slice(4096, 6784), [slice(0, 4096), slice(6784, T)]
+    kept = torch.full((T, c), 7.0, device=DEV, dtype=t)
+    ops.linear_recurrence(gate, v, q, kept, cu_seqlens=cu, state_in=s)
+    R.check("out", kept[mine], val["out"][mine], tol["out"][mine])
+    assert all((kept[i] == 7).all() for i in rest)
+    leaves = [x.requires_grad_() for x in (gate, v, q, s)]
+    out, last = ops.linear_recurrence(gate, v, q, cu_seqlens=cu, state_in=s, return_state=True)
+    got = torch.autograd.grad((out, last), leaves, (dout, dlast))
+    R.check("state", last.detach(), val["state"], tol["state"])
+    R.check("dstate_in", got[3], val["dstate_in"], tol["dstate_in"])
+    for n, x in zip(("out", "dgate", "dv", "dq"), (out.detach(),) + got[:3]):
+        R.check(n, x[mine], val[n][mine], tol[n][mine])
+        assert all((x[i] == 0).all() for i in rest), n
+
+
+@pytest.mark.parametrize("dtype,c,T", [("f32", 48, 1000), ("bf16", 96, 333), ("f16", 70, 4097), ("f32", 3, 1025)])
+def test_an_infinity_in_the_last_token(dtype, c, T):
+    """What a tile has behind the last token is no token: nothing of that one comes from there."""
+    from ssla_hip import ops
+    t = R.TYPES[dtype]
+    gate, v, q, dout = (normal(50 + i, T, c).to(t) for i in range(4))
+    val, tol = R.recurrence(gate, v, q, [(0, T)], None, dout)
+    v[-1] = float("inf")
+    gate[-1] = float("inf")                                  # an open gate
+    leaves = [x.requires_grad_() for x in (gate, v, q)]
+    out = ops.linear_recurrence(gate, v, q)
+    dg, dv, dq = torch.autograd.grad(out, leaves, dout)
+    R.check("out", out.detach()[:-1], val["out"][:-1], tol["out"][:-1])
+    R.check("dq", dq[:-1], val["dq"][:-1], tol["dq"][:-1])
+    assert (dg[-1] == 0).all() and not torch.isfinite(dq[-1]).any()
+    gate, v = gate.detach(), v.detach()
+    v[-1] = 0
+    val, tol = R.recurrence(gate.double().clamp(max=80), v, q, [(0, T)], None, dout)
+    R.check("dv", dv, val["dv"], tol["dv"])
+    R.check("dgate", dg[:-1], val["dgate"][:-1], tol["dgate"][:-1])

@@ -202,3 +202,22 @@ def test_an_infinity_in_the_last_token(dtype, c, T):
     val, tol = R.recurrence(gate.double().clamp(max=80), v, q, [(0, T)], None, dout)
     R.check("dv", dv, val["dv"], tol["dv"])
     R.check("dgate", dg[:-1], val["dgate"][:-1], tol["dgate"][:-1])
+
+
+@pytest.mark.parametrize("n,c,dtype", [(66000, 5, "f32"), (700, 40, "bf16")])
+def test_more_sequences_than_a_workgroup_has_threads(n, c, dtype):
+    """Boundaries that are searched for in one step more, and two; most sequences are empty."""
+    from ssla_hip import ops
+    lens = [2 * (i % 6 == 0) + (i % 35 == 34) for i in range(n)]
+    first = [0]
+    for k in lens:
+        first.append(first[-1] + k)
+    cu = torch.tensor(first, dtype=torch.int32, device=DEV)
+    gate, v, q, dout = (normal(60 + i, first[-1], c).to(R.TYPES[dtype]) for i in range(4))
+    s, dlast = normal(64, n, c), normal(65, n, c)
+    val, tol = R.recurrence(gate, v, q, list(zip(first[:-1], first[1:])), s, dout, dlast)
+    leaves = [x.requires_grad_() for x in (gate, v, q, s)]
+    out, last = ops.linear_recurrence(gate, v, q, cu_seqlens=cu, state_in=s, return_state=True)
+    got = torch.autograd.grad((out, last), leaves, (dout, dlast))
+    for k, x in zip(("out", "state", "dgate", "dv", "dq", "dstate_in"), (out.detach(), last.detach()) + got):
+        R.check(k, x, val[k], tol[k])

@@ -594,6 +594,10 @@ typedef struct SslaHipLinRec {
     int wait_us;               /* 0: 200; see ssla_hip_linrec */
 } SslaHipLinRec;
 
+/* A wait_us for tests: the last tiles start first, and none publishes anything but
+ * what it has made for another. */
+#define SSLA_LINREC_ALONE (-2147483647 - 1)
+
 /* Gradients of the call *d that kept its carries, from those of out and of the
  * last states (NULL: zeros):
  *     dh_t = q_t dout_t + sigmoid(gate_{t+1}) dh_{t+1}   (the last token: + dstate_out)

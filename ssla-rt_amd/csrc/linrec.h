@@ -37,6 +37,7 @@ struct LinRecArgs {
     int carry;                            // tokens of a tile of the backward pass
     int brief;                            // a thread a channel, without tiles
     unsigned patience;                    // ticks of 10 ns that a workgroup waits for another
+    int alone;                            // tiles start with the last, and publish nothing of their own
     unsigned long long* words;            // workspace: [block][kBehind + place in the chain][kChannels] maps and states
 };
 

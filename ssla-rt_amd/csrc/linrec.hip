@@ -100,6 +100,7 @@ struct Place {
                   wide = min(8, a.tiles - 8 * eight);
         cb = wide == 8 ? k >> 3 : k / wide;
         place = 8 * eight + k - cb * wide;
+        if (a.alone) place = a.tiles - 1 - place;
         tile = backward ? a.tiles - 1 - place : place;
         // one of nt boundaries spread over all; looked at in mark, as waiting for it here would
         // put off the tile's loads (ragged fp16, kernels' us: forward 87 -> 83, backward 155 -> 146)
@@ -448,7 +449,7 @@ struct Chain {
         // word of this channel at place p
         unsigned long long* word = a.words + ((long long)block * (a.tiles + kBehind) + kBehind + p) * kChannels + ch;
         auto publish = [&](float x, float l) {
-            if (on && part == 0) __hip_atomic_store(word, word_of(x, l), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (on && part == 0 && !a.alone) __hip_atomic_store(word, word_of(x, l), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         };
         publish(open ? tA : kCut, tL);
         if (!open) return 0.0f;

@@ -113,6 +113,7 @@ LinRecArgs linrec_args(const SslaHipLinRec* d, const SslaHipLinRecGrad* g) {
     a.s_in = d->state_in, a.s_out = d->state_out, a.si = d->state_in_stride, a.so = d->state_out_stride;
     a.carries = d->carries;
     a.patience = d->wait_us < 0 ? 0 : (d->wait_us ? d->wait_us : 200) * 100u;
+    a.alone = d->wait_us == SSLA_LINREC_ALONE;
     a.n_tokens = d->n_tokens, a.n_seqs = d->n_seqs, a.n_slots = d->n_slots, a.channels = d->channels;
     if (!d->slots && !d->state_in && !d->state_out) a.n_slots = d->n_seqs;
     a.seq_len = d->n_seqs ? (int)(d->n_tokens / d->n_seqs) : 0;

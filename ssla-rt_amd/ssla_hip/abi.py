@@ -147,6 +147,9 @@ class SslaHipGroupNorm(ctypes.Structure):
         ("eps", ctypes.c_float)]
 
 
+SSLA_LINREC_ALONE = -(1 << 31)
+
+
 class SslaHipLinRec(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in ("dtype", "channels", "n_seqs", "n_slots")] + [
         ("n_tokens", ctypes.c_longlong)] + [

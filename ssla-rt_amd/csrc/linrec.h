@@ -39,6 +39,10 @@ struct LinRecArgs {
     unsigned patience;                    // ticks of 10 ns that a workgroup waits for another
     int alone;                            // tiles start with the last, and publish nothing of their own
     unsigned long long* words;            // workspace: [block][kBehind + place in the chain][kChannels] maps and states
+    // forward, where the last states take the first ones' place (else null): the first state of the
+    // sequence that a tile's last token belongs to, and which that is (-1: it has none)
+    float* firsts;                        // workspace: [tile][channels]
+    int* cut;                             // workspace: [tile]
 };
 
 constexpr int kLinRecThreads = 256;
@@ -51,8 +55,18 @@ inline int linrec_threads(const LinRecArgs& a) { return (a.cols * a.lanes + 63) 
 inline size_t linrec_words(const LinRecArgs& a) {
     return a.tiles > 1 ? ((size_t)a.tiles + kBehind) * a.blocks * kChannels : 0;
 }
-inline size_t linrec_bytes(const LinRecArgs& a) {
-    return linrec_words(a) * 8;
+inline size_t linrec_firsts(const LinRecArgs& a) {
+    return a.tiles > 1 ? (size_t)a.tiles * a.channels : 0;
+}
+// Of the forward pass: with firsts and cut, wherever the states are.
+inline size_t linrec_bytes(const LinRecArgs& a, bool backward) {
+    return linrec_words(a) * 8 + (backward || a.tiles < 2 ? 0 : (linrec_firsts(a) + a.tiles) * 4);
+}
+inline void linrec_bind(LinRecArgs& a, void* workspace) {
+    a.words = (unsigned long long*)workspace;
+    if (a.tiles < 2 || !a.s_in || a.s_in != a.s_out) return;
+    a.firsts = (float*)(a.words + linrec_words(a));
+    a.cut = (int*)(a.firsts + linrec_firsts(a));
 }
 inline size_t linrec_carries(const LinRecArgs& a) {
     return (size_t)((a.n_tokens + a.carry - 1) / a.carry) * a.channels * 4;

@@ -22,7 +22,10 @@
 // atomics: whoever sees A sees L, with no fence (a release fence would write back
 // the L2).  A tile that has waited for long makes the missing maps itself, from the
 // tensors and in the same steps (made_here), so that none depends on another's
-// workgroup being started.  Drawing tiles by tickets instead cost 12 us of 57 where one
+// workgroup being started.  Where the last states take the first ones' place, a last one may so
+// be stored before a tile that is late has read the first: first states of sequences that go on
+// behind a tile are then read from a copy, made by the launch that empties the chain
+// (keep_first).  Drawing tiles by tickets instead cost 12 us of 57 where one
 // block of channels has 1565 of them (8 ns an atomic on one address).
 //
 // Backward, the same from the last token to the first: the message m_t = a_{t+1}
@@ -36,6 +39,9 @@
 // rest is a workgroup's own time, of which its waves wait for half: the look along the chain (8 us
 // of 74 in the first), barriers, LDS; four waves a SIMD do not fill that in.
 #include "linrec.h"
+
+#include <algorithm>
+
 #include "piece.h"
 
 // Maps are made in two places, to the same bits: nothing is fused but by fmaf.
@@ -292,6 +298,10 @@ __device__ __forceinline__ void join(float& A, float& L, float x, float l) {
 template <class T, int R, bool BACK>
 __device__ unsigned long long made_here(const LinRecArgs& a, int place, int channel) {
     const int tile = BACK ? a.tiles - 1 - place : place, t0 = tile * a.tile, per = a.lanes / 4;
+    // Of the first states in a tile its map has the last one only, so that any stands for the others.
+    // (A look at a.cut for each costs registers: 16 bits a value spill.)
+    const float* const from = a.firsts ? a.firsts + (long long)tile * a.channels : a.s_in;
+    const long long by = a.firsts ? 0 : a.si;
     auto value = [&](const void* p, long long stride, int t) { return (float)((const T*)p)[t * stride + channel]; };
     float tA = 1.0f, tL = 0.0f;
     #pragma unroll 1
@@ -311,7 +321,7 @@ __device__ unsigned long long made_here(const LinRecArgs& a, int place, int chan
                     if (at.seq != was) {
                         const int slot = linrec_slot(a, at.seq);
                         cut = true;
-                        x = a.s_in && slot >= 0 ? a.s_in[slot * a.si + channel] : 0.0f;
+                        x = a.s_in && slot >= 0 ? from[slot * by + channel] : 0.0f;
                     }
                     const float f = gate_of(value(a.g, a.gt, t + r)).a;
                     x = fmaf(f, x, value(a.v, a.vt, t + r));
@@ -460,10 +470,7 @@ struct Chain {
         return state;
     }
     // The same without waiting for anyone.  What is made here is published in the tile's
-    // place, unless something is by now, which then counts: whoever knows a state has seen
-    // all words from its sequence's beginning on, and only then may it write the sequence's
-    // last state, perhaps in the place of the first.  A map made from that too late is thus
-    // never used.
+    // place, unless something is by now, which may be a state.
     template <class T, int R, bool BACK>
     __device__ float alone(const LinRecArgs& a, unsigned long long* word, int p, int channel) {
         auto map = [&](int j) {
@@ -589,14 +596,17 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 3) void k_linrec(const Lin
     p.mark(a, sh);
 
     // The thread's map.  The last state that comes in is kept: its sequence may end
-    // in another thread, which may write to its slot before this one is here again.
+    // in another thread, which may write to its slot before this one is here again; or in
+    // another tile, which may have written to it already.
     float f[R][V], A[V], h[V], last[V];
     #pragma unroll
     for (int i = 0; i < V; ++i) A[i] = 1.0f, h[i] = last[i] = 0.0f;
     #pragma unroll
     for (int r = 0; r < R; ++r) {
         if (p.starts >> r & 1) {
-            state_of(last, a.s_in, a.si, linrec_slot(a, p.first[p.y * R + r]), p.c);
+            const int seq = p.first[p.y * R + r];
+            const bool kept = a.firsts && seq == a.cut[p.tile];
+            state_of(last, kept ? a.firsts : a.s_in, kept ? a.channels : a.si, kept ? p.tile : linrec_slot(a, seq), p.c);
             #pragma unroll
             for (int i = 0; i < V; ++i) h[i] = last[i];
         }
@@ -834,10 +844,36 @@ __global__ __launch_bounds__(64) void k_linrec_short(const LinRecArgs a) {
     if (a.s_out) a.s_out[slot * a.so + c] = h;
 }
 
-// Empties the chain: no word is published.
-__global__ __launch_bounds__(NT) void k_linrec_clear(ulonglong2* words, long long n) {
-    for (long long i = (long long)blockIdx.x * NT + threadIdx.x; i < n; i += (long long)gridDim.x * NT)
-        words[i] = ulonglong2{~0ull, ~0ull};
+// Copies the first state of the sequence that the tile's last token belongs to, if it begins in
+// the tile.
+__device__ void keep_first(const LinRecArgs& a, int tile) {
+    const int lane = threadIdx.x & 63, t0 = tile * a.tile;
+    const long long t = min((long long)t0 + a.tile, a.n_tokens) - 1;
+    auto first = [&](long long i) { return a.cu ? (long long)boundary(a, i) : i * a.seq_len; };
+    int lo = -1;
+    long long hi = a.n_seqs + 1ll;                           // first(lo) <= t < first(hi)
+    while (hi - lo > 1) {                                    // 64 of those between at a time
+        const long long step = (hi - lo + 62) / 64, i = lo + 1 + lane * step;
+        const int k = __popcll(__ballot(i < hi && first(i) <= t));
+        hi = min(hi, lo + 1 + k * step);
+        lo = k ? (int)(lo + 1 + (k - 1) * step) : lo;
+    }
+    const int slot = linrec_slot(a, lo), seq = slot >= 0 && first(lo) >= t0 ? lo : -1;
+    if (threadIdx.x == 0) a.cut[tile] = seq;
+    if (seq < 0) return;
+    #pragma unroll 4
+    for (int c = threadIdx.x; c < a.channels; c += NT)
+        a.firsts[(long long)tile * a.channels + c] = a.s_in[slot * a.si + c];
+}
+
+// Empties the chain: no word is published.  Workgroups behind the first `wgs`: keep_first.
+__global__ __launch_bounds__(NT) void k_linrec_clear(const LinRecArgs a, long long n, int wgs) {
+    if ((int)blockIdx.x >= wgs) {
+        keep_first(a, blockIdx.x - wgs);
+        return;
+    }
+    for (long long i = (long long)blockIdx.x * NT + threadIdx.x; i < n; i += (long long)wgs * NT)
+        ((ulonglong2*)a.words)[i] = ulonglong2{~0ull, ~0ull};
 }
 
 size_t lds_bytes(const LinRecArgs& a) {
@@ -871,9 +907,9 @@ hipError_t launch(const LinRecArgs& a, hipStream_t st) {
     const int nt = linrec_threads(a);
     if (a.tiles > 1) {
         long long n = (long long)linrec_words(a) / 2;
-        void* pc[] = {&args.words, &n};
-        const long long wgs = (n + 4 * NT - 1) / (4 * NT);   // four stores a thread
-        const hipError_t e = hipLaunchKernel((const void*)k_linrec_clear, dim3((unsigned)(wgs < 1024 ? wgs : 1024)),
+        int wgs = (int)std::min((n + 4 * NT - 1) / (4 * NT), 1024ll);              // four stores a thread
+        void* pc[] = {&args, &n, &wgs};
+        const hipError_t e = hipLaunchKernel((const void*)k_linrec_clear, dim3((unsigned)(wgs + (a.firsts ? a.tiles : 0))),
                                              dim3(NT), pc, 0, st);
         if (e != hipSuccess) return e;
     }

@@ -131,12 +131,12 @@ LinRecArgs linrec_args(const SslaHipLinRec* d, const SslaHipLinRecGrad* g) {
 // Workspace of either pass.
 size_t linrec_need(const SslaHipLinRec* d) {
     const SslaHipLinRecGrad none{};
-    const size_t one = linrec_bytes(linrec_args(d, nullptr)), other = linrec_bytes(linrec_args(d, &none));
+    const size_t one = linrec_bytes(linrec_args(d, nullptr), false), other = linrec_bytes(linrec_args(d, &none), true);
     return one > other ? one : other;
 }
 
 // The grid's limit, and the workspace.
-int linrec_bind(LinRecArgs& a, const SslaHipLinRec* d, void* workspace, size_t bytes, const char* fn) {
+int bind_linrec(LinRecArgs& a, const SslaHipLinRec* d, void* workspace, size_t bytes, const char* fn) {
     if (!launchable(a.tiles, a.blocks, 1, kLinRecThreads) ||
         !launchable((long long)a.tiles * a.blocks + a.n_seqs / linrec_threads(a) + 1, 1, 1, kLinRecThreads))
         return refuse(std::string(fn) + ": too many tokens and channels");
@@ -144,7 +144,8 @@ int linrec_bind(LinRecArgs& a, const SslaHipLinRec* d, void* workspace, size_t b
     if (!need) return SSLA_OK;
     if (!workspace || bytes < need || !aligned(workspace, 16))
         return refuse(std::string(fn) + ": the workspace is missing, too small or not 16-byte aligned");
-    a.words = (unsigned long long*)workspace;
+    linrec_bind(a, workspace);
+    if (a.firsts && !launchable(a.tiles + 1024ll, 1, 1, kLinRecThreads)) return refuse(std::string(fn) + ": too many tokens");
     return SSLA_OK;
 }
 
@@ -257,7 +258,7 @@ int ssla_hip_linrec(const SslaHipLinRec* d, void* workspace, size_t workspace_by
     const char* fn = "ssla_hip_linrec";
     if (const int rc = check_linrec(d, kForward, fn)) return rc;
     LinRecArgs a = linrec_args(d, nullptr);
-    if (const int rc = linrec_bind(a, d, workspace, workspace_bytes, fn)) return rc;
+    if (const int rc = bind_linrec(a, d, workspace, workspace_bytes, fn)) return rc;
     const hipError_t e = linrec_launch(a, d->dtype, (hipStream_t)stream);
     return e == hipSuccess ? SSLA_OK : hip_failed(fn, e);
 } catch (const std::exception&) {
@@ -270,7 +271,7 @@ int ssla_hip_linrec_backward(const SslaHipLinRec* d, const SslaHipLinRecGrad* g,
     if (const int rc = check_linrec(d, kBackward, fn)) return rc;
     if (const int rc = check_linrec_grad(d, g)) return rc;
     LinRecArgs a = linrec_args(d, g);
-    if (const int rc = linrec_bind(a, d, workspace, workspace_bytes, fn)) return rc;
+    if (const int rc = bind_linrec(a, d, workspace, workspace_bytes, fn)) return rc;
     const hipError_t e = linrec_launch_backward(a, d->dtype, (hipStream_t)stream);
     return e == hipSuccess ? SSLA_OK : hip_failed(fn, e);
 } catch (const std::exception&) {

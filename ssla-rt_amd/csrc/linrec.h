@@ -49,6 +49,9 @@ constexpr int kLinRecThreads = 256;
 constexpr int kChannels = 64;             // most of a workgroup
 constexpr int kBehind = 32;               // places before a chain's first one, never published
 
+// Sequences of len tokens each that begin before token t.
+constexpr int linrec_begun(int t, int len) { return t ? (t - 1) / len + 1 : 0; }
+
 void linrec_plan(LinRecArgs& a, int dtype, bool backward);
 inline int linrec_threads(const LinRecArgs& a) { return (a.cols * a.lanes + 63) / 64 * 64; }
 // Workspace: 0 where one tile holds all tokens.

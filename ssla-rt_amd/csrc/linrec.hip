@@ -181,8 +181,8 @@ struct Place {
             }
             before = lo - 1;
         } else {
-            const int len = a.seq_len, s = (t0 + len - 1) / len;
-            before = t0 ? (t0 - 1) / len : -1;
+            const int len = a.seq_len, s = linrec_begun(t0, len);
+            before = s - 1;
             __syncthreads();                                  // the masks are clear
             for (long long i = s + tid; i * len <= t1; i += nt) set(sh, (int)(i * len), (int)i);
         }

@@ -637,9 +637,9 @@ int ssla_hip_linrec_step(const SslaHipLinRec* d, void* stream);
  * and out likewise.  weight and bias (NULL: 1 and 0) are of weight_dtype, which
  * is dtype or SSLA_F32.  x + residual is an fp32 sum, the mean is summed in 64
  * bits and subtracted to 48, squared differences are summed in 64 bits (fp32) or
- * 32 (16-bit types, and 64 where that is not finite), out is rounded once.  out
- * may be x or residual itself, else it must not overlap an input.  `stats` (NULL: not
- * kept) takes three floats a row for the backward pass. */
+ * 32 (16-bit types, and 64 where those are too large or too small for 32), out is
+ * rounded once.  out may be x or residual itself, else it must not overlap an
+ * input.  `stats` (NULL: not kept) takes three floats a row for the backward pass. */
 typedef struct SslaHipLayerNorm {
     int dtype, weight_dtype;
     int rows, channels;

@@ -8,7 +8,7 @@
 // them; a longer one by a workgroup, joined through LDS; one that no workgroup
 // holds is read in strides, again for each use (k_ln, k_ln_backward, k_ln_columns).
 // The mean is taken first, in 64 bits, then squared differences from it, in 64 bits
-// too, or for 16-bit types in 32 where those are finite (below); mean and scale are kept as
+// too, or for 16-bit types in 32 where those hold them (below); mean and scale are kept as
 // three floats (norm.h) for the backward pass.
 //
 // Measured with 100 MB a tensor: fp32 rows of 96 to 2048 channels, forward 5.2 to 5.8 TB/s,
@@ -174,7 +174,9 @@ __global__ __launch_bounds__(512) void k_ln_rows(const LayerNormArgs a) {
         } else {
             // In 32 bits (6139 x 8192 bf16: 39.9 us, in 64 bits 44.0; 196602 x 256 44.0 and 47.0):
             // of differences from the mean's float, whose own mean is what that leaves of the
-            // mean.  Each is rounded by 2^-24 of itself at most, which the variance keeps.
+            // mean.  Each is rounded by 2^-24 of itself at most, which the variance keeps, but for
+            // squares below 2^-126, of which a row's 2^14 at most lose 2^-112: 2^-32 of a sum of
+            // 2^-80, and nothing beside an eps of 2^-60.
             const float m = (float)mean;
             float sq = 0.0f;
             #pragma unroll
@@ -189,9 +191,9 @@ __global__ __launch_bounds__(512) void k_ln_rows(const LayerNormArgs a) {
             }
             opaque(x), opaque(res);
             sq = row_sum<WHOLE>(sq, a.lanes, (float*)sums[turn][1]);
-            // a row whose squares are too large, or that is not finite; all of a row's lanes
-            // agree
-            if (sq < __builtin_inff()) {
+            // a row whose squares are too large or too small, or that is not finite; all of a
+            // row's lanes agree
+            if (sq < __builtin_inff() && (sq >= 0x1p-80f || a.eps >= 0x1p-60f)) {
                 const double rest = mean - (double)m;
                 var = fma(-rest, rest, (double)sq * a.inv_channels);
                 var = var < 0.0 ? 0.0 : var;

@@ -531,9 +531,10 @@ int ssla_hip_linattn_step(const SslaHipLinAttn* d, void* stream);
  * Element (item, row, c) of x lies at item * stride[0] + row * stride[1] + c
  * (elements, >= 0), of gate and out likewise.  weight and bias (NULL: 1 and 0)
  * have the type of x.  Sums are 64 bits wide, the mean is subtracted to 48 bits,
- * out is rounded once; finite values of any size are taken.  out may be x or gate
- * itself, else it must not overlap an input.  A NaN or infinity reaches its own
- * group of its own item only. */
+ * out is rounded once; finite values of any size are taken, but a group whose
+ * sqrt(var + eps) is 2^-112 (1.9e-34) or less gets infinities and NaNs.  out may be
+ * x or gate itself, else it must not overlap an input.  A NaN or infinity reaches
+ * its own group of its own item only. */
 typedef struct SslaHipGroupNorm {
     int dtype;
     int n, rows, channels, groups, act;
@@ -638,8 +639,10 @@ int ssla_hip_linrec_step(const SslaHipLinRec* d, void* stream);
  * is dtype or SSLA_F32.  x + residual is an fp32 sum, the mean is summed in 64
  * bits and subtracted to 48, squared differences are summed in 64 bits (fp32) or
  * 32 (16-bit types, and 64 where those are too large or too small for 32), out is
- * rounded once.  out may be x or residual itself, else it must not overlap an
- * input.  `stats` (NULL: not kept) takes three floats a row for the backward pass. */
+ * rounded once; finite values of any size are taken, but a row whose
+ * sqrt(var + eps) is 2^-112 (1.9e-34) or less gets infinities and NaNs.  out may be
+ * x or residual itself, else it must not overlap an input.  `stats` (NULL: not kept)
+ * takes three floats a row for the backward pass. */
 typedef struct SslaHipLayerNorm {
     int dtype, weight_dtype;
     int rows, channels;

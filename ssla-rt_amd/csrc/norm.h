@@ -10,9 +10,9 @@ namespace ssla {
 //     (x - mean) / sqrt(var + eps) = (2^-16 x - hi) scale - lo scale.
 // hi + lo is the mean to 48 bits: hi alone would be off by up to 2^-25 of the
 // mean, which is 0.03 standard deviations where the mean is 10^6 of them.
-// 2^-16 x - hi, one fused operation, is finite for all finite x and mean, and scale
-// is a normal number for any spread of them; what the two lose of the smallest x
-// lies below 2^-133.
+// 2^-16 x - hi, one fused operation, is finite for all finite x and mean; what it and lo
+// lose of the smallest x lies below 2^-133.  scale, 2^16 / sqrt(var + eps), is a normal number
+// for any larger spread, and overflows where sqrt(var + eps) is 2^-112 (1.9e-34) or less.
 struct alignas(16) Norm {
     float hi, lo, scale;
 };

@@ -53,3 +53,26 @@ def test_small_spreads(dtype, spread, eps, c, residual):
         R.check(n, got[n], val[n], tol[n])
     assert ok.any()
     R.check("dx", got["dx"][ok.to(x.device)], val["dx"][ok], tol["dx"][ok])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("c", [8, 96, 2048, 20000])
+def test_the_smallest_spread(dtype, c):
+    """A deviation of 2^-111 without eps, in powers of two alone: every value is exact.  A row
+    of a smaller one is not finite, and the others do not see it."""
+    from ssla_hip import ops
+    sign = torch.ones(c, device="cuda")
+    sign[1::2] = -1.0
+    x = (sign * 2.0 ** -111).expand(5, c).to(R.TYPES[dtype]).contiguous()
+    x[2] = 0.0
+    dy = torch.zeros_like(x)
+    dy[:, 0] = 2.0
+    norm = ops.layer_norm(x, eps=0.0), ops.group_norm(x, 1, eps=0.0)
+    got = grads(x, None, None, None, dy, 0.0)
+    rows = [0, 1, 3, 4]
+    for y in norm + (got["y"],):
+        assert (y[rows] == sign).all() and not torch.isfinite(y[2]).any()
+    # dx = 2^111 (dy - 2 / c - sign 2 / c): nothing where sign is -1
+    want = (2.0 ** 111 * (dy.double() - 2.0 / c - sign.double() * (2.0 / c)))[rows]
+    off = 2.0 ** 111 * 100 * R.U32 * (dy.double() + 4.0 / c)[rows] + R.half_step(x.dtype) * want.abs()
+    assert ((got["dx"][rows].double() - want).abs() <= off).all()

@@ -80,8 +80,9 @@ hipError_t linrec_launch_step(const LinRecArgs& a, int dtype, hipStream_t st);
 
 #ifdef __HIPCC__
 // A gate a = sigmoid(x), rounded once from 1 - s where x > 0, and its slope a (1 - a) =
-// s (1 - s), with s = sigmoid(-|x|) to a few roundings of itself: 1 - a would have
-// none of a gate's digits that is nearly open.
+// s (1 - s), with s = sigmoid(-|x|): 1 - a would have none of a gate's digits that is
+// nearly open.  s is off by some ten roundings of itself, and by up to |x| more: the
+// exponential's argument is rounded, which counts where a gate is nearly shut.
 struct Gate {
     float a, slope;
 };

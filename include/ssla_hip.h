@@ -557,7 +557,9 @@ int ssla_hip_ops_layout(long long* out, int cap);
  * gate, v, q and out are rows of tokens: element (token, c) lies at token *
  * stride + c (strides in elements, >= 0).  States, gates and products are fp32,
  * out is rounded once.  An infinity or NaN reaches the outputs of its own token
- * and those behind it in its own sequence and channel only.
+ * and those behind it in its own sequence and channel only, as the one or the other.
+ * Tokens are joined before the state in front of them is known: outputs are finite
+ * where the recurrence from a state of zero at any token is finite as well.
  *
  * Sequences are packed: sequence s holds the tokens cu_seqlens[s] up to
  * cu_seqlens[s + 1] (n_seqs + 1 values in device memory, rising from >= 0 to
@@ -607,7 +609,9 @@ typedef struct SslaHipLinRec {
  * dout, dgate, dv and dq are rows of tokens of d's type, dstate_out and dstate_in
  * rows of sequences; each of the four outputs may be NULL: not wanted.  Rows
  * that belong to no sequence get zeros.  d->slots must be NULL; d->out,
- * d->state_out are not looked at.  No output may overlap an input. */
+ * d->state_out are not looked at.  d->state_in holds the first states, also where
+ * the call wrote the last ones in their place: give a copy then.  No output may
+ * overlap an input. */
 typedef struct SslaHipLinRecGrad {
     const void* dout;
     const float* dstate_out;
@@ -623,7 +627,7 @@ int ssla_hip_linrec_carries(const SslaHipLinRec* d, size_t* nbytes);
 int ssla_hip_linrec_workspace(const SslaHipLinRec* d, size_t* nbytes);
 /* Both cut the tokens into tiles that wait for one another's results; one that has
  * waited for wait_us (negative: not at all) makes what it lacks itself, to the same
- * bits. */
+ * bits, with states in one pool too. */
 int ssla_hip_linrec(const SslaHipLinRec* d, void* workspace, size_t workspace_bytes, void* stream);
 int ssla_hip_linrec_backward(const SslaHipLinRec* d, const SslaHipLinRecGrad* g, void* workspace,
                              size_t workspace_bytes, void* stream);

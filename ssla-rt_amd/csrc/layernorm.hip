@@ -6,15 +6,16 @@
 // Bound by memory: every tensor is read and written once.  A row is kept in registers
 // by some lanes of a wave, in 16-byte pieces a lane, and nothing but shuffles joins
 // them; a longer one by a workgroup, joined through LDS; one that no workgroup
-// holds is read in strides, again for each use (k_ln, k_ln_backward, k_ln_columns).
+// holds is read in strides, again for each use (k_ln, k_ln_backward, k_ln_columns; 20000 bf16
+// values 0.9 TB/s each way).
 // The mean is taken first, in 64 bits, then squared differences from it, in 64 bits
 // too, or for 16-bit types in 32 where those hold them (below); mean and scale are kept as
 // three floats (norm.h) for the backward pass.
 //
 // Measured with 100 MB a tensor: fp32 rows of 96 to 2048 channels, forward 5.2 to 5.8 TB/s,
-// backward 4.9 to 5.1; bf16 rows of 256 to 2048 4.6 to 5.1 and 4.2 to 4.8, of 8192 5.0 and 3.6
-// (its workgroups have barriers in every row, and more sums to leave), of 4099, which no line
-// holds, 3.5 and 2.1.
+// backward 4.9 to 5.1; bf16 rows of 256 to 4096 4.6 to 5.1 and 4.2 to 4.8, of 8192 4.9 and 3.8
+// (its workgroups have barriers in every row, and more sums to leave), of 4104, which take
+// workgroups of three waves a row, 4.0 and 2.5, of 4099, which no line holds either, 3.2 and 2.1.
 //
 // The sums over rows: a workgroup goes through rows a stride apart, each thread's
 // channels stay the same, and so their sums stay in its registers; the

@@ -32,12 +32,14 @@
 // dh_{t+1} goes through maps, cut where a sequence ends.  States come from those
 // that the forward pass left before each tile (carries).
 //
-// Kernels measured (us; in brackets what moving the bytes once takes at a copy's rate): 1 x 40001
-// of 1024 bf16 channels 73.5 (64); 1 x 8192 of 2048, forward 37.5 (26), backward 57 (46); 1.25M
-// records of 48 fp32 ones in 19200 sequences 200 (187) and 322 (327); 40504 tokens of 1001 fp16 ones
-// in 48, without q, 84 (47) and 150 (79).  fp32 is bound by memory.  With 16 bits a value the
-// rest is a workgroup's own time, of which its waves wait for half: the look along the chain (8 us
-// of 74 in the first), barriers, LDS; four waves a SIMD do not fill that in.
+// Kernels measured (us by the profiler; in brackets what moving the bytes once takes at a copy's
+// rate): 1 x 40001 of 1024 bf16 channels 73.8 (64); 1 x 8192 of 2048, forward 37.4 (26), backward 57
+// (46); 1.25M records of 48 fp32 ones in 19200 sequences 200 (187) and 316 (327); 40504 tokens of
+// 1001 fp16 ones in 48, without q, 82 to 86 (47) and 145 to 155 (79).  fp32 is bound by memory.
+// With 16 bits a value a workgroup's own time shows: all its loads are at its beginning, and its
+// waves wait for half of the time: the look along the chain (8 us of 74 in the first), barriers,
+// LDS.  Odd rows' addresses are little of it (the last with 1000 channels 85 and 152, with 1024 77
+// and 136).  First states out of a copy (see above) cost 1.7 us of 78 in the first.
 #include "linrec.h"
 
 #include <algorithm>

@@ -2,7 +2,7 @@
 //
 // Each state is read and written once, with a few operations a value: bound by
 // memory (8000 sequences of 2048 bf16 channels: 38.4 us, 6.0 TB/s, states and all once),
-// and by its launch where there are few (one sequence: 2.1 us).  A thread owns 16 bytes
+// and by its launch where there are few (one sequence: 1.9 us in a graph).  A thread owns 16 bytes
 // of a row's values (what is left over at a row's end goes by single values).
 #include "linrec.h"
 

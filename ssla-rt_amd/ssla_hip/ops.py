@@ -16,11 +16,12 @@ not fit raise ValueError, what the library refuses (values out of range, rows of
 out or pools that overlap) lib.SslaHipError, before anything is queued.
 linear_recurrence and layer_norm are functions of torch's autograd: where it
 records, their outputs are new tensors with first derivatives (second ones are
-refused), and a call in a capture refuses leaves whose older graph, recorded on
-the default stream, still lives.  The others have no gradients: tensors that
-require one are refused while torch records.  Tensors that carry a forward gradient
-are refused everywhere; tensors that a call writes to get a new version.  There is
-no fallback: without the library, or for tensors off the GPU, a call raises.
+refused), and a call in a capture refuses leaves given to it whose older graph,
+recorded on the default stream, still lives.  The others have no gradients:
+tensors that require one are refused while torch records.  Tensors that carry a
+forward gradient are refused everywhere; tensors that a call writes to get a new
+version.  There is no fallback: without the library, or for tensors off the GPU, a
+call raises.
 
 The checks and the calls are in csrc/ops_torch.cpp and csrc/ops_train_torch.cpp
 (_ops.so).

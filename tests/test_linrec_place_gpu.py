@@ -79,3 +79,26 @@ def test_captured():
             torch.cuda.synchronize()
             assert torch.equal(out, want) and torch.equal(place, last), i
             pool.copy_(last)
+
+
+def test_calls_at_once():
+    """Four streams, each with a call in one pool that fills the card by itself."""
+    from ssla_hip import ops
+    cu = torch.tensor([0, 9000, 9000, 9001, 20000], dtype=torch.int32, device=DEV)
+    calls = []
+    for i in range(4):
+        (gate, v, q), pool, _, _ = inputs("bf16", 1024, 20000, 4, 30 + i)
+        last = pool.clone()
+        with torch.no_grad():
+            want = ops.linear_recurrence(gate, v, q, cu_seqlens=cu, state_in=pool, state_out=last)
+        calls.append((gate, v, q, pool, torch.empty_like(want), want, last, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for turn in range(5):
+        places = [c[3].clone() for c in calls]
+        torch.cuda.synchronize()
+        for (gate, v, q, _, out, _, _, stream), place in zip(calls, places):
+            with torch.cuda.stream(stream), torch.no_grad():
+                ops.linear_recurrence(gate, v, q, out, cu_seqlens=cu, state_in=place, state_out=place)
+        torch.cuda.synchronize()
+        for (_, _, _, _, out, want, last, _), place in zip(calls, places):
+            assert torch.equal(out, want) and torch.equal(place, last), turn

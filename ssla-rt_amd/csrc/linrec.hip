@@ -300,8 +300,9 @@ __device__ __forceinline__ void join(float& A, float& L, float x, float l) {
 template <class T, int R, bool BACK>
 __device__ unsigned long long made_here(const LinRecArgs& a, int place, int channel) {
     const int tile = BACK ? a.tiles - 1 - place : place, t0 = tile * a.tile, per = a.lanes / 4;
-    // Of the first states in a tile its map has the last one only, so that any stands for the others.
-    // (A look at a.cut for each costs registers: 16 bits a value spill.)
+    // Of the first states in a tile only the last one is left in its map, so the copy of that one
+    // may stand for the others.  (Looking at a.cut for each costs registers: with 16-bit values
+    // the kernel spilled.)
     const float* const from = a.firsts ? a.firsts + (long long)tile * a.channels : a.s_in;
     const long long by = a.firsts ? 0 : a.si;
     auto value = [&](const void* p, long long stride, int t) { return (float)((const T*)p)[t * stride + channel]; };
@@ -461,7 +462,8 @@ struct Chain {
         // word of this channel at place p
         unsigned long long* word = a.words + ((long long)block * (a.tiles + kBehind) + kBehind + p) * kChannels + ch;
         auto publish = [&](float x, float l) {
-            if (on && part == 0 && !a.alone) __hip_atomic_store(word, word_of(x, l), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (on && part == 0 && !a.alone)
+                __hip_atomic_store(word, word_of(x, l), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         };
         publish(open ? tA : kCut, tL);
         if (!open) return 0.0f;
